@@ -94,6 +94,13 @@ SIGNATURES = {
     "eeggan_maxpool_select": (_i, [_f, C.c_void_p, _f, _sz, _i, _i, _i, _st]),
     "eeggan_dot_workspace": (_sz, []),
     "eeggan_dot": (_i, [_f, _f, _f, _sz, C.c_void_p, _sz, _st]),
+    "eeggan_attention_fwd_workspace": (_sz, [C.c_void_p]),
+    "eeggan_attention_fwd": (_i, [C.c_void_p, _f, _f, _f, C.c_void_p, _sz, _st]),
+    "eeggan_attention_bwd_workspace": (_sz, [C.c_void_p, _i]),
+    "eeggan_attention_bwd": (_i, [C.c_void_p, _f, _f, _f, _f, _f, _f, _f, _f, C.c_void_p, _sz, _st]),
+    "eeggan_relative_bias": (_i, [_f, _f, C.c_void_p, _f, _i, _i, _i, _i, _st]),
+    "eeggan_relative_bias_grad_workspace": (_sz, [C.c_void_p, _i, _i, _i, _i]),
+    "eeggan_relative_bias_grad": (_i, [_f, C.c_void_p, _f, _i, _i, _i, _i, C.c_void_p, _sz, _st]),
     "eeggan_mean_scale": (_i, [_f, _f, _i, _fl, _st]),
     "eeggan_mean_scale_bwd": (_i, [_f, _f, _i, _fl, _st]),
     "eeggan_swd_patches": (_i, [_f, _f, _f, _i, _i, _i, _i, _i, _i, _st]),
@@ -111,6 +118,11 @@ SIGNATURES = {
     "eeggan_feature_stats_workspace": (_sz, [_sz, _i]),
     "eeggan_feature_stats": (_i, [_f, _sz, _i, _f, _f, C.c_void_p, _sz, _st]),
     "eeggan_adam_step": (_i, [C.c_void_p, _i, _fl, _fl, _fl, _fl, _fl, _st]),
+    "eeggan_grad_norm_workspace": (_sz, [C.c_void_p, _i]),
+    "eeggan_grad_norm": (_i, [C.c_void_p, _i, _fl, C.c_double, _f, C.c_void_p, _sz, _st]),
+    "eeggan_grad_scale": (_i, [C.c_void_p, _i, _f, _st]),
+    "eeggan_adam_step_clipped": (_i, [C.c_void_p, _i, C.c_double, C.c_double, C.c_double, C.c_double, _f, C.c_void_p, _sz,
+                                      _st]),
     "eeggan_multi_copy": (_i, [C.c_void_p, _i, _st]),
     "eeggan_multi_axpby": (_i, [C.c_void_p, _i, _fl, _fl, _st]),
     "eeggan_score_loss": (_i, [_i, _f, _f, _i, _fl, _f, _f, _f, _st]),

@@ -1,0 +1,562 @@
+// Backward pass of the fused attention: the probabilities are formed again from q, k and the forward's lse.
+//   P[s,t] = 2^(S log2e - lse[t]);  delta[t] = sum_c O dO;  dP = V^T dO;  dS = P (dP - delta)
+//   dQ[d,t] = scale sum_s K[d,s] dS[s,t]          (attn_dq_kernel: a wave owns 32 queries, the keys stream through LDS)
+//   dV[c,s] = sum_t dO[c,t] P[s,t],  dK[d,s] = scale sum_t Q[d,t] dS[s,t]
+//                                                 (attn_dkv_kernel: a wave owns 32 keys, q and dO stream)
+// Two kernels, each forming S and dP (seven products where one kernel would need five): a sum over keys and a sum over
+// queries cannot both stay in one wave's registers, and one of them through atomics would make the result depend on
+// their order.  Both orientations have their result registers where the next product wants its operand
+// (attention_tiles.h), so nothing crosses lanes.  -delta is the initial accumulator of dP.
+//
+// The position table's gradient rides on attn_dq_kernel: tiles whose distances all lie beyond the last bucket's edge
+// add to one register; a near tile adds its dS to a histogram by distance in LDS, private to the wave, one lane half
+// at a time (no two lanes of an addition share a distance): a fixed order, no races.
+#include "attention_host.h"
+
+namespace eeggan {
+namespace attn {
+
+struct BwdArgs {
+    const void *q, *k, *v;
+    long long qsb, qsc, ksb, ksc, vsb, vsc;
+    const unsigned char* mask;
+    const void *out, *rest, *g;  // [B, H Dv, Tq]; out + rest: the output before its rounding (float32: rest null)
+    const float* lse;
+    float* delta;  // [B, H, Tq]: written by attn_dq_kernel, read by attn_dkv_kernel
+    void *gq, *gk, *gv;
+    float* part;  // dK, dV of a split over the queries; null: not split
+    float* hist;  // [H, B * coltiles, nhist + 2] sums of dS by distance (then: beyond it, behind / ahead); null: not wanted
+    Positions pos;
+    int B, KV, G, Dk, Dv, Tq, Tk;
+    int coltiles, nsplit, nhist;
+    float scale;
+};
+
+template <class T, int DK, int DV, int XT, bool BIAS>
+__global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
+    constexpr int NP = Elem<T>::NP;
+    typedef TTile<NP, DK, XT> KT;
+    typedef NTile<NP, DK, XT> KN;
+    typedef TTile<NP, DV, XT> VT;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char* const kt = smem;
+    char* const kn = kt + KT::BYTES;
+    char* const vt = kn + KN::BYTES;
+
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tile = blockIdx.x % a.coltiles;
+    const int bh = blockIdx.x / a.coltiles;
+    const int H = a.KV * a.G;
+    const int b = bh / H, head = bh - b * H, kvh = head / a.G;
+
+    const int t0 = (tile * 4 + wave) * 32;
+    const bool inside = t0 + l31 < a.Tq;
+    const int t = inside ? t0 + l31 : 0;
+    const long long row = (long long)b * H + head;
+    float lse = a.lse[row * a.Tq + t];
+    const bool live = inside && lse != INFINITY;  // (a query without keys takes no part)
+    if (!live) lse = INFINITY;
+
+    const float c = a.scale * LOG2E;
+    SFrag<NP, DK> fq;
+    SFrag<NP, DV> fg;
+    float delta = 0.f;
+    {
+        const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc + t;
+        fq.fill(h, [&](int d) {
+            const float v = live && d < a.Dk ? ld1(q + d * a.qsc) : 0.f;
+            return NP == 3 ? v * c : v;
+        });
+        const T* g = reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq + t;
+        const T* o = reinterpret_cast<const T*>(a.out) + row * a.Dv * a.Tq + t;
+        const T* rest = reinterpret_cast<const T*>(a.rest) + row * a.Dv * a.Tq + t;
+        fg.fill(h, [&](int d) {
+            const bool ok = live && d < a.Dv;
+            const float v = ok ? ld1(g + (long long)d * a.Tq) : 0.f;
+            if (ok) {
+                float x = ld1(o + (long long)d * a.Tq);
+                if (NP == 1) x += ld1(rest + (long long)d * a.Tq);
+                delta = __builtin_fmaf(v, x, delta);
+            }
+            return v;
+        });
+        delta = half_sum(delta);
+        if (inside && h == 0) a.delta[row * a.Tq + t] = delta;
+    }
+    const T* const kb = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc;
+    const T* const vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc;
+    const unsigned char* const mask = a.mask ? a.mask + (long long)b * a.Tk : nullptr;
+    const float* const rel = BIAS ? a.pos.rel + (long long)head * a.pos.nrel + (a.Tq - 1 - t) : nullptr;
+
+    f32x16 dinit;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dinit[r] = -delta;
+    f32x16 dq[KN::GROUPS];
+#pragma unroll
+    for (int i = 0; i < KN::GROUPS; ++i) dq[i] = zero16();
+
+    double beyond[2] = {0.0, 0.0};  // sums of dS over far tiles, behind / ahead of the query (thousands of terms)
+    float* const hist = BIAS ? reinterpret_cast<float*>(vt + VT::BYTES) + wave * a.nhist : nullptr;
+    const bool want = BIAS && a.hist != nullptr;
+    const int width = a.nhist / 2;  // (distances -width .. width)
+    if (want)
+        for (int i = lane; i < a.nhist; i += 64) hist[i] = 0.f;
+
+    Block<T, DK, XT> kblk;
+    Block<T, DV, XT> vblk;
+    unsigned long long word64 = 0;
+    auto fetch = [&](int s0) {
+        kblk.load(kb, a.ksc, a.Dk, s0, a.Tk, mask, tid);
+        vblk.load(vb, a.vsc, a.Dv, s0, a.Tk, mask, tid);
+        const int s = s0 + lane;
+        word64 = __ballot(lane < XT && s < a.Tk && (!mask || mask[s]));
+    };
+    fetch(0);
+    for (int s0 = 0; s0 < a.Tk; s0 += XT) {
+        __syncthreads();
+        kblk.template store<true, true>(kt, kn, mask != nullptr, tid);
+        vblk.template store<true, false>(vt, nullptr, mask != nullptr, tid);
+        const unsigned long long now = word64;
+        __syncthreads();
+        if (s0 + XT < a.Tk) fetch(s0 + XT);
+#pragma unroll
+        for (int u = 0; u < XT / 32; ++u) {
+            const int x0 = 32 * u;
+            const unsigned word = (unsigned)(now >> x0);
+            if (word == 0) continue;
+            const int s = s0 + x0;
+            f32x16 acc;
+            int side = 0;
+            if constexpr (BIAS) {
+                side = tile_side(a.pos, s, t0);
+                if (side != 0) {
+                    const float bias = rel[(long long)a.pos.step * s] - lse;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[r] = bias;
+                } else {
+                    const float* r0 = rel + (long long)a.pos.step * (s + 4 * h);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = (r & 3) + 8 * (r >> 2);
+                        acc[r] = (s + 4 * h + i < a.Tk ? r0[a.pos.step * i] : 0.f) - lse;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] = -lse;
+            }
+            // (the scores accumulate from zero and meet lse once: on top of -lse every partial sum would be rounded at
+            // its magnitude)
+            const f32x16 raw = mma_scores<NP, DK, XT>(kt + (x0 + l31) * KT::RS, h, fq, zero16());
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[r] + acc[r] : __builtin_fmaf(raw[r], c, acc[r]);
+            if (word != 0xffffffffu) {
+                const unsigned w = word >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] = (w >> ((r & 3) + 8 * (r >> 2))) & 1u ? acc[r] : -INFINITY;
+            }
+            f32x16 ds = mma_scores<NP, DV, XT>(vt + (x0 + l31) * VT::RS, h, fg, dinit);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(acc[r]);
+            if constexpr (BIAS) {
+                if (want) {
+                    if (side != 0) {
+                        float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s4[r & 3] += ds[r];
+                        const float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                        if (side < 0) beyond[0] += (double)sum;
+                        else beyond[1] += (double)sum;
+                    } else {
+                        // (distances of a near tile stay within the histogram: tile_side)
+                        float* const hp = hist + width + a.pos.offset + a.pos.step * (s + 4 * h) - (t0 + l31);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half)
+                            if (h == half && live) {
+#pragma unroll
+                                for (int r = 0; r < 16; ++r)
+                                    __hip_atomic_fetch_add(hp + a.pos.step * ((r & 3) + 8 * (r >> 2)), ds[r],
+                                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                            }
+                    }
+                }
+            }
+            PFrag<NP> p;
+            p.fill(ds);
+            mma_values<NP, DK, XT>(kn, x0, l31, h, p, dq);
+        }
+    }
+    if (inside) {
+        eight_rows<NP, DK>(dq[0]);
+        T* out = reinterpret_cast<T*>(a.gq) + row * a.Dk * a.Tq + t;
+#pragma unroll
+        for (int i = 0; i < KN::GROUPS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * i + acc_row(r, h);
+                if (d < a.Dk && (!KN::P8 || r < 4)) st1(out + (long long)d * a.Tq, live ? dq[i][r] * a.scale : 0.f);
+            }
+    }
+    if constexpr (BIAS) {
+        if (want) {
+            float* const part = a.hist + ((long long)head * a.B * a.coltiles + (long long)b * a.coltiles + tile) * (a.nhist + 2);
+            __syncthreads();
+            const float* const all = reinterpret_cast<const float*>(vt + VT::BYTES);
+            for (int i = tid; i < a.nhist; i += THREADS)
+                part[i] = (all[i] + all[a.nhist + i]) + (all[2 * a.nhist + i] + all[3 * a.nhist + i]);
+            float* const sums = reinterpret_cast<float*>(smem);
+            const float s0 = wave_sum((float)beyond[0]), s1 = wave_sum((float)beyond[1]);
+            if (lane == 0) {
+                sums[wave] = s0;
+                sums[4 + wave] = s1;
+            }
+            __syncthreads();
+            if (tid < 2) part[a.nhist + tid] = (sums[4 * tid] + sums[4 * tid + 1]) + (sums[4 * tid + 2] + sums[4 * tid + 3]);
+        }
+    }
+}
+
+// WK waves along the keys, WT = 4 / WK along the queries of a stage (their sums are joined through LDS at the end).
+template <class T, int DK, int DV, int WK, int XT, bool BIAS>
+__global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 2) void attn_dkv_kernel(BwdArgs a) {
+    constexpr int NP = Elem<T>::NP;
+    constexpr int WT = 4 / WK, SUBS = XT / (32 * WT);
+    typedef TTile<NP, DK, XT> QT;
+    typedef NTile<NP, DK, XT> QN;
+    typedef TTile<NP, DV, XT> GT;
+    typedef NTile<NP, DV, XT> GN;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char* const qt = smem;
+    char* const qn = qt + QT::BYTES;
+    char* const gt = qn + QN::BYTES;
+    char* const gn = gt + GT::BYTES;
+    float* const stats = reinterpret_cast<float*>(gn + GN::BYTES);  // -lse, then -delta, of the stage's queries
+
+    const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wk = wave % WK, wt = wave / WK;
+    int blk = blockIdx.x;
+    const int tile = blk % a.coltiles;
+    blk /= a.coltiles;
+    const int split = blk % a.nsplit;
+    const int bkv = blk / a.nsplit;
+    const int b = bkv / a.KV, kvh = bkv - b * a.KV;
+    const int H = a.KV * a.G;
+
+    const int s_tile = (tile * WK + wk) * 32;
+    const int s = s_tile + l31;
+    const bool inside = s < a.Tk;
+    const bool live = inside && (!a.mask || a.mask[(long long)b * a.Tk + s]);
+
+    const float c = a.scale * LOG2E;
+    SFrag<NP, DK> fk;
+    SFrag<NP, DV> fv;
+    {
+        const T* k = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc + (live ? s : 0);
+        fk.fill(h, [&](int d) {
+            const float v = live && d < a.Dk ? ld1(k + d * a.ksc) : 0.f;
+            return NP == 3 ? v * c : v;
+        });
+        const T* v = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc + (live ? s : 0);
+        fv.fill(h, [&](int d) { return live && d < a.Dv ? ld1(v + d * a.vsc) : 0.f; });
+    }
+    f32x16 dk[QN::GROUPS], dv[GN::GROUPS];
+#pragma unroll
+    for (int i = 0; i < QN::GROUPS; ++i) dk[i] = zero16();
+#pragma unroll
+    for (int i = 0; i < GN::GROUPS; ++i) dv[i] = zero16();
+
+    const int per_head = (a.Tq + XT - 1) / XT;
+    const int stages = a.G * per_head;
+    const int first = (int)((long long)stages * split / a.nsplit), last = (int)((long long)stages * (split + 1) / a.nsplit);
+
+    Block<T, DK, XT> qblk;
+    Block<T, DV, XT> gblk;
+    float stat = 0.f;
+    auto fetch = [&](int stage) {
+        const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
+        const int head = kvh * a.G + g;
+        const long long row = (long long)b * H + head;
+        qblk.load(reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc, a.qsc, a.Dk, t0, a.Tq,
+                  nullptr, tid);
+        gblk.load(reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq, a.Tq, a.Dv, t0, a.Tq, nullptr, tid);
+        if (tid < 2 * XT) {
+            const int t = t0 + tid % XT;
+            const float* p = (tid < XT ? a.lse : a.delta) + row * a.Tq;
+            stat = t < a.Tq ? -p[t] : tid < XT ? -INFINITY : 0.f;
+        }
+    };
+    if (first < last) fetch(first);
+    for (int stage = first; stage < last; ++stage) {
+        __syncthreads();
+        qblk.template store<true, true>(qt, qn, false, tid);
+        gblk.template store<true, true>(gt, gn, false, tid);
+        if (tid < 2 * XT) stats[tid] = stat;
+        __syncthreads();
+        if (stage + 1 < last) fetch(stage + 1);
+        const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
+        const float* rel = nullptr;
+        if constexpr (BIAS) rel = a.pos.rel + (long long)(kvh * a.G + g) * a.pos.nrel + (a.Tq - 1);
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) {
+            const int x0 = 32 * (u * WT + wt);
+            if (t0 + x0 >= a.Tq) continue;  // (the same for every lane of the wave)
+            f32x16 acc, ds;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 e = *reinterpret_cast<const f32x4*>(stats + x0 + 8 * i + 4 * h);
+                const f32x4 f = *reinterpret_cast<const f32x4*>(stats + XT + x0 + 8 * i + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[4 * i + j] = e[j];
+                    ds[4 * i + j] = f[j];
+                }
+            }
+            if constexpr (BIAS) {
+                const int t = t0 + x0;
+                const float* r0 = rel + (long long)a.pos.step * (inside ? s : 0) - t;
+                if (tile_side(a.pos, s_tile, t) != 0) {
+                    const float bias = r0[0];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[r] += bias;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = acc_row(r, h);
+                        acc[r] += t + i < a.Tq ? r0[-i] : 0.f;
+                    }
+                }
+            }
+            const f32x16 raw = mma_scores<NP, DK, XT>(qt + (x0 + l31) * QT::RS, h, fk, zero16());
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[r] + acc[r] : __builtin_fmaf(raw[r], c, acc[r]);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = __builtin_amdgcn_exp2f(acc[r]);
+            ds = mma_scores<NP, DV, XT>(gt + (x0 + l31) * GT::RS, h, fv, ds);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] *= acc[r];
+            PFrag<NP> p;
+            p.fill(acc);
+            mma_values<NP, DV, XT>(gn, x0, l31, h, p, dv);
+            p.fill(ds);
+            mma_values<NP, DK, XT>(qn, x0, l31, h, p, dk);
+        }
+    }
+    if constexpr (WT > 1) {
+        // the sums of the waves wt = 1 .. WT - 1 are added to those of wave wt = 0, in that order
+        constexpr int WORDS = (QN::GROUPS + GN::GROUPS) * 16 * 64;
+        float* const buf = reinterpret_cast<float*>(smem);
+        __syncthreads();
+        if (wt > 0) {
+            float* const mine = buf + ((wt - 1) * WK + wk) * WORDS + lane;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+#pragma unroll
+                for (int i = 0; i < QN::GROUPS; ++i) mine[(16 * i + r) * 64] = dk[i][r];
+#pragma unroll
+                for (int i = 0; i < GN::GROUPS; ++i) mine[(16 * (QN::GROUPS + i) + r) * 64] = dv[i][r];
+            }
+        }
+        __syncthreads();
+        if (wt > 0) return;
+        for (int w = 1; w < WT; ++w) {
+            const float* const other = buf + ((w - 1) * WK + wk) * WORDS + lane;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+#pragma unroll
+                for (int i = 0; i < QN::GROUPS; ++i) dk[i][r] += other[(16 * i + r) * 64];
+#pragma unroll
+                for (int i = 0; i < GN::GROUPS; ++i) dv[i][r] += other[(16 * (QN::GROUPS + i) + r) * 64];
+            }
+        }
+    }
+    if (!inside) return;
+    eight_rows<NP, DK>(dk[0]);
+    auto each = [&](auto&& put_k, auto&& put_v) {
+#pragma unroll
+        for (int i = 0; i < QN::GROUPS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * i + acc_row(r, h);
+                if (d < a.Dk && (!QN::P8 || r < 4)) put_k(d, live ? dk[i][r] * a.scale : 0.f);
+            }
+#pragma unroll
+        for (int i = 0; i < GN::GROUPS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * i + acc_row(r, h);
+                if (d < a.Dv) put_v(d, live ? dv[i][r] : 0.f);
+            }
+    };
+    if (a.part == nullptr) {
+        T* const gk = reinterpret_cast<T*>(a.gk) + (long long)bkv * a.Dk * a.Tk + s;
+        T* const gv = reinterpret_cast<T*>(a.gv) + (long long)bkv * a.Dv * a.Tk + s;
+        each([&](int d, float x) { st1(gk + (long long)d * a.Tk, x); }, [&](int d, float x) { st1(gv + (long long)d * a.Tk, x); });
+    } else {
+        const long long heads = (long long)a.B * a.KV;
+        float* const pk = a.part + ((long long)split * heads + bkv) * a.Dk * a.Tk + s;
+        float* const pv = a.part + (long long)a.nsplit * heads * a.Dk * a.Tk + ((long long)split * heads + bkv) * a.Dv * a.Tk + s;
+        each([&](int d, float x) { pk[(long long)d * a.Tk] = x; }, [&](int d, float x) { pv[(long long)d * a.Tk] = x; });
+    }
+}
+
+// dK and dV of a split over the queries: the parts' sums, in order.
+template <class T>
+__global__ __launch_bounds__(THREADS) void attn_sum_kernel(const float* part, T* gk, T* gv, long long nk, long long nv,
+                                                           int nsplit) {
+    const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
+    if (i >= nk + nv) return;
+    const bool is_k = i < nk;
+    const float* p = is_k ? part + i : part + nsplit * nk + (i - nk);
+    const long long n = is_k ? nk : nv;
+    float s = 0.f;
+    for (int j = 0; j < nsplit; ++j) s += p[j * n];
+    st1(is_k ? gk + i : gv + (i - nk), s);
+}
+
+}  // namespace attn
+}  // namespace eeggan
+
+using namespace eeggan;
+using namespace eeggan::attn;
+
+namespace {
+
+template <class T, int DK, int DV>
+struct Cut {
+    static constexpr bool F32 = Elem<T>::NP == 3;
+    static constexpr int DQ_XT = F32 && DK + DV > 96 ? 32 : 64;
+    static constexpr int WIDE_XT = F32 && DK + DV > 96 ? 32 : 64;
+    static constexpr bool NARROW = !(F32 && DK + DV > 96);  // has a form whose waves share keys
+};
+constexpr int WANTED = 512;
+
+struct BwdPlan {
+    bool narrow;
+    int qtiles, ktiles, nsplit, nhist;
+    size_t rel, delta, part, hist, total;
+};
+
+template <class T, int DK, int DV>
+BwdPlan plan_of(const eeggan_attention& a, bool want_table) {
+    typedef Cut<T, DK, DV> C;
+    BwdPlan p;
+    p.qtiles = (a.Tq + 127) / 128;
+    const long long heads = (long long)a.B * a.KV;
+    p.narrow = C::NARROW && heads * ((a.Tk + 127) / 128) < WANTED;
+    const int keys = p.narrow ? 64 : 128, xt = p.narrow ? 64 : C::WIDE_XT;
+    p.ktiles = (a.Tk + keys - 1) / keys;
+    const long long blocks = heads * p.ktiles, stages = (long long)(a.H / a.KV) * ((a.Tq + xt - 1) / xt);
+    long long n = blocks >= WANTED ? 1 : WANTED / blocks;
+    if (n > stages / 2) n = stages / 2 > 0 ? stages / 2 : 1;
+    p.nsplit = (int)n;
+    p.nhist = a.table && want_table ? 2 * (bucket_far(*a.buckets) + 31 * a.buckets->step + 31) + 1 : 0;
+    auto up = [](size_t x) { return (x + 15) / 16 * 16; };
+    p.rel = positions_bytes(a);
+    p.delta = up((size_t)a.B * a.H * a.Tq * sizeof(float));
+    p.part = n > 1 ? up((size_t)n * heads * (a.Dk + a.Dv) * a.Tk * sizeof(float)) : 0;
+    p.hist = p.nhist ? up((size_t)a.H * a.B * p.qtiles * (p.nhist + 2) * sizeof(float)) : 0;
+    p.total = p.rel + p.delta + p.part + p.hist;
+    return p;
+}
+
+template <class T, int DK, int DV, bool BIAS>
+int launch_dq(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
+    constexpr int NP = Elem<T>::NP, XT = Cut<T, DK, DV>::DQ_XT;
+    constexpr size_t tiles = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES + TTile<NP, DV, XT>::BYTES;
+    constexpr size_t most = tiles + (BIAS ? 4 * (2 * (1024 + 31 * 16 + 31) + 1) * sizeof(float) : 0);
+    static_assert(most <= 160 * 1024, "LDS");
+    auto kernel = &attn_dq_kernel<T, DK, DV, XT, BIAS>;
+    static LdsReady ready;
+    if (ready.reserve("attention backward", reinterpret_cast<const void*>(kernel), most)) return 1;
+    const long long grid = (long long)f.B * f.KV * f.G * p.qtiles;
+    EEGGAN_REQUIRE(grid < (1ll << 31), "attention backward: too many workgroups");
+    BwdArgs a = f;
+    a.coltiles = p.qtiles;
+    a.nhist = p.nhist;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), tiles + 4 * (size_t)p.nhist * sizeof(float), st, a);
+    return check_launch("attention backward (queries)");
+}
+
+template <class T, int DK, int DV, int WK, int XT, bool BIAS>
+int launch_dkv(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
+    constexpr int NP = Elem<T>::NP;
+    constexpr size_t tiles = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES + TTile<NP, DV, XT>::BYTES +
+                             NTile<NP, DV, XT>::BYTES + 2 * XT * sizeof(float);
+    constexpr size_t join = (4 / WK - 1) * WK * (NTile<NP, DK, XT>::GROUPS + NTile<NP, DV, XT>::GROUPS) * 16 * 64 * sizeof(float);
+    constexpr size_t lds = tiles > join ? tiles : join;
+    static_assert(lds <= 160 * 1024 && 2 * XT <= THREADS, "LDS");
+    auto kernel = &attn_dkv_kernel<T, DK, DV, WK, XT, BIAS>;
+    static LdsReady ready;
+    if (ready.reserve("attention backward", reinterpret_cast<const void*>(kernel), lds)) return 1;
+    const long long grid = (long long)f.B * f.KV * p.ktiles * p.nsplit;
+    EEGGAN_REQUIRE(grid < (1ll << 31), "attention backward: too many workgroups");
+    BwdArgs a = f;
+    a.coltiles = p.ktiles;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), lds, st, a);
+    return check_launch("attention backward (keys)");
+}
+
+template <class T, int DK, int DV, bool BIAS>
+int backward(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
+    typedef Cut<T, DK, DV> C;
+    if (launch_dq<T, DK, DV, BIAS>(f, p, st)) return 1;
+    if constexpr (C::NARROW) {
+        if (p.narrow) return launch_dkv<T, DK, DV, 2, 64, BIAS>(f, p, st);
+    }
+    return launch_dkv<T, DK, DV, 4, C::WIDE_XT, BIAS>(f, p, st);
+}
+
+template <class T, int DK, int DV>
+int backward_all(const eeggan_attention& a, const void* out, const void* rest, const float* lse, const void* g, void* gq, void* gk, void* gv,
+                 void* g_table, char* ws, size_t bytes, hipStream_t st) {
+    const BwdPlan p = plan_of<T, DK, DV>(a, g_table != nullptr);
+    EEGGAN_REQUIRE(bytes >= p.total, "attention backward: workspace too small");
+    BwdArgs f;
+    f.q = a.q, f.k = a.k, f.v = a.v;
+    f.qsb = a.q_batch, f.qsc = a.q_channel, f.ksb = a.k_batch, f.ksc = a.k_channel, f.vsb = a.v_batch, f.vsc = a.v_channel;
+    f.mask = a.mask, f.out = out, f.rest = rest, f.g = g, f.lse = lse, f.gq = gq, f.gk = gk, f.gv = gv;
+    f.delta = reinterpret_cast<float*>(ws + p.rel);
+    f.part = p.nsplit > 1 ? reinterpret_cast<float*>(ws + p.rel + p.delta) : nullptr;
+    f.hist = p.nhist ? reinterpret_cast<float*>(ws + p.rel + p.delta + p.part) : nullptr;
+    f.B = a.B, f.KV = a.KV, f.G = a.H / a.KV, f.Dk = a.Dk, f.Dv = a.Dv, f.Tq = a.Tq, f.Tk = a.Tk;
+    f.coltiles = 0, f.nsplit = p.nsplit, f.nhist = 0, f.scale = a.scale;
+    if (positions(a, reinterpret_cast<float*>(ws), &f.pos, st)) return 1;
+    if (a.table ? backward<T, DK, DV, true>(f, p, st) : backward<T, DK, DV, false>(f, p, st)) return 1;
+    if (p.nsplit > 1) {
+        const long long nk = (long long)a.B * a.KV * a.Dk * a.Tk, nv = (long long)a.B * a.KV * a.Dv * a.Tk;
+        const long long blocks = (nk + nv + THREADS - 1) / THREADS;
+        EEGGAN_REQUIRE(blocks < (1ll << 31), "attention backward: too many outputs");
+        hipLaunchKernelGGL(attn_sum_kernel<T>, dim3((unsigned)blocks), dim3(THREADS), 0, st, f.part, reinterpret_cast<T*>(gk),
+                           reinterpret_cast<T*>(gv), nk, nv, p.nsplit);
+        if (check_launch("attention backward (sums)")) return 1;
+    }
+    if (p.nhist) {
+        return bucket_sums(f.hist, g_table, a.table_bf16, *a.buckets, a.H, (long long)a.B * p.qtiles, p.nhist / 2, st);
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" size_t eeggan_attention_bwd_workspace(const eeggan_attention* a, int want_table) {
+    if (check_attention("attention backward", a)) return 0;
+    size_t n = 0;
+    EEGGAN_ATTENTION_CLASS(*a, n = (plan_of<T, DK, DV>(*a, want_table != 0).total))
+    return n;
+}
+
+extern "C" int eeggan_attention_bwd(const eeggan_attention* a, const void* out, const void* rest, const float* lse,
+                                    const void* g, void* gq, void* gk, void* gv, void* g_table, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    if (check_attention("attention backward", a)) return 1;
+    EEGGAN_REQUIRE(out && lse && g && gq && gk && gv && workspace, "attention backward: null pointer");
+    EEGGAN_REQUIRE(!a->bf16 || rest, "attention backward: bfloat16 needs the rest of the output");
+    EEGGAN_REQUIRE(!g_table || a->table, "attention backward: a table gradient without a table");
+    int rc = 1;
+    EEGGAN_ATTENTION_CLASS(*a, rc = (backward_all<T, DK, DV>(*a, out, rest, lse, g, gq, gk, gv, g_table,
+                                                             reinterpret_cast<char*>(workspace), workspace_bytes,
+                                                             as_stream(stream))))
+    return rc;
+}

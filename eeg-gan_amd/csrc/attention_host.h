@@ -1,0 +1,70 @@
+// Host side shared by the fused attention's entry points: argument checks, the choice of the tile class, the table of
+// position biases by distance.
+#pragma once
+#include <atomic>
+
+#include "attention_tiles.h"
+#include "buckets.h"
+
+namespace eeggan {
+namespace attn {
+
+// Opt-in to more than 64 KiB of dynamic LDS, once per kernel and device.
+struct LdsReady {
+    static constexpr int DEVICES = 64;
+    std::atomic<bool> done[DEVICES] = {};
+    int reserve(const char* what, const void* kernel, size_t bytes) {
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= DEVICES) dev = 0;
+        if (done[dev].load(std::memory_order_acquire)) return 0;
+        const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        EEGGAN_REQUIRE(e == hipSuccess, "%s: cannot reserve %zu bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+        done[dev].store(true, std::memory_order_release);
+        return 0;
+    }
+};
+
+int check_attention(const char* what, const eeggan_attention* a);
+// rel table of a call: entries per head, bytes (a multiple of 16), and the launch that fills it (nothing without a bias)
+inline long long positions_entries(const eeggan_attention& a) {
+    return a.table ? (long long)a.Tq + (long long)a.buckets->step * (a.Tk - 1) : 0;
+}
+inline size_t positions_bytes(const eeggan_attention& a) {
+    return ((size_t)a.H * (size_t)positions_entries(a) * sizeof(float) + 15) / 16 * 16;
+}
+int positions(const eeggan_attention& a, float* rel, Positions* p, hipStream_t st);
+// out[bucket, head] from histograms by distance: hist [H][rows][2 width + 3] (distances -width .. width, behind, ahead)
+int bucket_sums(const float* hist, void* out, int out_bf16, const eeggan_buckets& bk, int H, long long rows, int width,
+                hipStream_t st);
+
+// The channel counts are rounded up to the first class that holds them; the classes are the layer's own shapes
+// (Dk = C / 8, Dv = C / 2 for 64, 128 and 256 channels) and equal halves.  bfloat16 has no eight-channel form: one
+// instruction reduces over sixteen.
+#define EEGGAN_ATTENTION_CLASS_T(TYPE, a, ...)                                                            \
+    {                                                                                                     \
+        typedef TYPE T;                                                                                   \
+        if ((a).Dk <= 8 && (a).Dv <= 32) {                                                                \
+            constexpr int DK = Elem<T>::NP == 3 ? 8 : 16, DV = 32;                                        \
+            __VA_ARGS__;                                                                                  \
+        } else if ((a).Dk <= 16 && (a).Dv <= 64) {                                                        \
+            constexpr int DK = 16, DV = 64;                                                               \
+            __VA_ARGS__;                                                                                  \
+        } else if ((a).Dk <= 32 && (a).Dv <= 32) {                                                        \
+            constexpr int DK = 32, DV = 32;                                                               \
+            __VA_ARGS__;                                                                                  \
+        } else if ((a).Dk <= 64 && (a).Dv <= 64) {                                                        \
+            constexpr int DK = 64, DV = 64;                                                               \
+            __VA_ARGS__;                                                                                  \
+        } else if ((a).Dk <= 32) {                                                                        \
+            constexpr int DK = 32, DV = 128;                                                              \
+            __VA_ARGS__;                                                                                  \
+        } else {                                                                                          \
+            constexpr int DK = 128, DV = 128;                                                             \
+            __VA_ARGS__;                                                                                  \
+        }                                                                                                 \
+    }
+#define EEGGAN_ATTENTION_CLASS(a, ...)                                                                    \
+    if ((a).bf16) EEGGAN_ATTENTION_CLASS_T(__bf16, a, __VA_ARGS__) else EEGGAN_ATTENTION_CLASS_T(float, a, __VA_ARGS__)
+
+}  // namespace attn
+}  // namespace eeggan

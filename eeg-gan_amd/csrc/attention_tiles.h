@@ -1,0 +1,376 @@
+// Tiles, fragments and products shared by the fused attention kernels (attention_fwd.hip, attention_bwd.hip).
+//
+// Tensors are channels-first: a head's queries are a [Dk, Tq] matrix with time contiguous, keys [Dk, Tk], values
+// [Dv, Tk].  All products run on v_mfma_f32_32x32x16_bf16 (operand A: row = lane & 31, eight reduction indices per
+// lane half; result: column = lane & 31, row = (r & 3) + 8 (r >> 2) + 4 (lane >> 5)).  Float32 tensors are multiplied
+// through three bf16 pieces per operand (v = p1 + p2 + p3 up to 2^-24 |v|, the six products down to 2^-16 of the
+// leading one: the rounding of an fp32 product); bfloat16 tensors directly.
+//
+// Two products alternate, and the layout makes the second one free of data movement:
+//   * scores-like, rows x = a time axis, reduction over channels: the streamed operand lies in LDS with channels
+//     contiguous ("T" tile, transposed while it is staged), the stationary one in registers (SFrag);
+//   * values-like, rows = channels, reduction over the time axis x: the streamed operand lies in LDS as it lies in
+//     memory ("N" tile), and the other operand is the result registers of the first product as they are: lane half h
+//     holds rows x = 16 kk + 8 a + 4 h + c (kk, a in {0, 1}, c < 4) in registers 8 kk + 4 a + c, so an N tile stores
+//     x at position 16 kk + 8 h + 4 a + c and one 16-byte read yields the matching operand.
+#pragma once
+#include "common.h"
+
+namespace eeggan {
+namespace attn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2u __attribute__((ext_vector_type(2), aligned(2)));  // four bfloat16 from any address
+
+constexpr int THREADS = 256;
+constexpr float LOG2E = 1.44269504088896340736f;
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static constexpr int NP = 3;  // bf16 pieces per operand
+    typedef f32x4 raw4;
+};
+template <>
+struct Elem<__bf16> {
+    static constexpr int NP = 1;
+    typedef u32x2 raw4;
+};
+
+__device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4u*>(p); }
+__device__ __forceinline__ u32x2 load4(const __bf16* p) {
+    const u32x2u v = *reinterpret_cast<const u32x2u*>(p);
+    u32x2 o;
+    o[0] = v[0];
+    o[1] = v[1];
+    return o;
+}
+// the first n (1 .. 3) of four values, the rest zero
+__device__ __forceinline__ f32x4 load_few(const float* p, int n) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    v[0] = p[0];
+    if (n > 1) v[1] = p[1];
+    if (n > 2) v[2] = p[2];
+    return v;
+}
+__device__ __forceinline__ u32x2 load_few(const __bf16* q, int n) {
+    const unsigned short* p = reinterpret_cast<const unsigned short*>(q);
+    u32x2 v = {p[0], 0u};
+    if (n > 1) v[0] |= (unsigned)p[1] << 16;
+    if (n > 2) v[1] = p[2];
+    return v;
+}
+
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    const f32x2_t v = {a, b};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2_t));
+}
+__device__ __forceinline__ float lo_f(unsigned w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float hi_f(unsigned w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+
+// The operand words of two neighbouring values: NP = 1 rounds to bfloat16, NP = 3 splits exactly (each remainder is
+// formed exactly in float32; the third piece is rounded at 2^-24 of the value).
+template <int NP>
+__device__ __forceinline__ void pieces2(float a, float b, unsigned (&w)[NP]) {
+    w[0] = pack2(a, b);
+    if constexpr (NP == 3) {
+        const float ra = a - lo_f(w[0]), rb = b - hi_f(w[0]);
+        w[1] = pack2(ra, rb);
+        w[2] = pack2(ra - lo_f(w[1]), rb - hi_f(w[1]));
+    }
+}
+
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ bf16x8 lds8(const char* p) { return *reinterpret_cast<const bf16x8*>(p); }
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
+}
+
+// the two lane halves' values combined
+__device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+
+// ---- tiles --------------------------------------------------------------------------------------------------
+// Eight channels in three pieces: the pieces share the reduction axis (see SFrag), one row holds all of them.
+template <int NP, int D>
+constexpr bool packed8() { return NP == 3 && D == 8; }
+
+// Row strides are odd multiples of 16 bytes: the 16-byte reads of 32 consecutive rows spread over all banks.
+template <int NP, int D, int XT>
+struct TTile {
+    static constexpr bool P8 = packed8<NP, D>();
+    static constexpr int RS = P8 ? 48 : 2 * D + 16;
+    static constexpr int PIECE = P8 ? 16 : XT * RS;
+    static constexpr int BYTES = P8 ? XT * RS : NP * XT * RS;
+};
+template <int NP, int D, int XT>
+struct NTile {
+    static constexpr bool P8 = packed8<NP, D>();
+    static constexpr int RS = 2 * XT + 16;
+    static constexpr int ROWS = D < 32 ? 32 : D;  // the products read whole groups of 32 rows
+    static constexpr int PIECE = P8 ? 8 * RS : ROWS * RS;
+    static constexpr int BYTES = P8 ? 32 * RS : NP * ROWS * RS;
+    static constexpr int GROUPS = D < 32 ? 1 : D / 32;
+};
+// byte offset of time index x (a multiple of 4) in a row of an N tile
+__device__ __forceinline__ int n_off(int x) { return 2 * ((x & ~31) + (x & 16) + ((x & 4) << 1) + ((x & 8) >> 1)); }
+
+// A [D, XT] block of a channels-first matrix on its way from memory into LDS: 4 x 4 units (four channels, four time
+// steps), neighbouring threads on neighbouring steps.  Units past the matrix are zero, and so are masked steps: what
+// lies there (NaN included) never meets a product.
+template <class T, int D, int XT>
+struct Block {
+    static constexpr int NP = Elem<T>::NP;
+    static constexpr int XQ = XT / 4, UNITS = (D / 4) * XQ, U = (UNITS + THREADS - 1) / THREADS;
+    typename Elem<T>::raw4 r[U][4];
+    unsigned keep[U];
+
+    // base: channel 0, step 0 of the head; steps [x0, x0 + XT) of `len`; mask: this sample's key mask or null
+    __device__ __forceinline__ void load(const T* base, long long stride, int channels, int x0, int len,
+                                         const unsigned char* mask, int tid) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int unit = tid + THREADS * u;
+            const int kq = unit % XQ, db = unit / XQ;
+            const int x = x0 + 4 * kq;
+            const T* p = base + (long long)(4 * db) * stride + x;
+            const bool in = UNITS % THREADS == 0 || unit < UNITS;
+            keep[u] = 0x01010101u;
+            if (mask && in && x < len) {
+                if (x + 3 < len) {
+                    typedef unsigned int u32u __attribute__((aligned(1)));
+                    keep[u] = *reinterpret_cast<const u32u*>(mask + x);
+                } else {
+                    keep[u] = mask[x] | (x + 1 < len ? (unsigned)mask[x + 1] << 8 : 0u) |
+                              (x + 2 < len ? (unsigned)mask[x + 2] << 16 : 0u);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                typename Elem<T>::raw4 z = {};
+                r[u][i] = z;
+                if (in && 4 * db + i < channels) {
+                    if (x + 3 < len) r[u][i] = load4(p + i * stride);
+                    else if (x < len) r[u][i] = load_few(p + i * stride, len - x);
+                }
+            }
+        }
+    }
+
+    // WT / WN: write the T tile / the N tile
+    template <bool WT, bool WN>
+    __device__ __forceinline__ void store(char* tt, char* nt, bool masked, int tid) {
+        typedef TTile<NP, D, XT> TL;
+        typedef NTile<NP, D, XT> NL;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int unit = tid + THREADS * u;
+            if (UNITS % THREADS != 0 && unit >= UNITS) continue;
+            const int kq = unit % XQ, db = unit / XQ;
+            unsigned w[4][2][NP];  // [channel][pair of steps][piece]
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (NP == 3) {
+                    f32x4 v = r[u][i];
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = (keep[u] >> (8 * e)) & 0xffu ? v[e] : 0.f;
+                    }
+                    pieces2<NP>(v[0], v[1], w[i][0]);
+                    pieces2<NP>(v[2], v[3], w[i][1]);
+                } else {
+                    u32x2 v = r[u][i];
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const unsigned lo = (keep[u] >> (16 * e)) & 0xffu ? 0xffffu : 0u;
+                            const unsigned hi = (keep[u] >> (16 * e + 8)) & 0xffu ? 0xffff0000u : 0u;
+                            v[e] &= lo | hi;
+                        }
+                    }
+                    w[i][0][0] = v[0];
+                    w[i][1][0] = v[1];
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                if (WN) {
+                    char* row = nt + p * NL::PIECE + (4 * db) * NL::RS + n_off(4 * kq);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const u32x2 o = {w[i][0][p], w[i][1][p]};
+                        *reinterpret_cast<u32x2*>(row + i * NL::RS) = o;
+                    }
+                }
+                if (WT) {
+                    char* row = tt + p * TL::PIECE + (4 * kq) * TL::RS + 8 * db;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {  // step e: channels (0, 1) and (2, 3)
+                        const unsigned sel = e & 1 ? 0x07060302u : 0x05040100u;
+                        const u32x2 o = {__builtin_amdgcn_perm(w[1][e >> 1][p], w[0][e >> 1][p], sel),
+                                         __builtin_amdgcn_perm(w[3][e >> 1][p], w[2][e >> 1][p], sel)};
+                        *reinterpret_cast<u32x2*>(row + e * TL::RS) = o;
+                    }
+                }
+            }
+        }
+    }
+};
+
+// ---- fragments ----------------------------------------------------------------------------------------------
+// The stationary operand of a scores-like product: this lane's column (one time step) of a [D, T] matrix.  Eight
+// channels in three pieces: two pieces of a term fill the sixteen reduction indices of one instruction, so the six
+// products take three instructions and two fragments.
+template <int NP, int D>
+struct SFrag {
+    static constexpr int N = packed8<NP, D>() ? 2 : NP * D / 16;
+    bf16x8 f[N];
+
+    // value(d) -> the (already scaled) value of channel d, zero past the matrix
+    template <class F>
+    __device__ __forceinline__ void fill(int h, F value) {
+        if constexpr (packed8<NP, D>()) {
+            u32x4 w0, w1, w2;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                unsigned w[3];
+                pieces2<3>(value(2 * i), value(2 * i + 1), w);
+                w0[i] = w[0];
+                w1[i] = w[1];
+                w2[i] = w[2];
+            }
+            f[0] = __builtin_bit_cast(bf16x8, h ? w1 : w0);
+            f[1] = __builtin_bit_cast(bf16x8, h ? w0 : w2);
+        } else {
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                u32x4 ws[NP];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned w[NP];
+                    const int d = 16 * j + 8 * h + 2 * i;
+                    pieces2<NP>(value(d), value(d + 1), w);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) ws[p][i] = w[p];
+                }
+#pragma unroll
+                for (int p = 0; p < NP; ++p) f[p * (D / 16) + j] = __builtin_bit_cast(bf16x8, ws[p]);
+            }
+        }
+    }
+};
+
+// acc[x, column] += sum_d tile[x, d] frag[d, column] for the 32 rows from `row` (= tile + (first row + lane & 31) * RS)
+template <int NP, int D, int XT>
+__device__ __forceinline__ f32x16 mma_scores(const char* row, int h, const SFrag<NP, D>& s, f32x16 acc) {
+    typedef TTile<NP, D, XT> TL;
+    if constexpr (packed8<NP, D>()) {
+        acc = mfma(lds8(row + 32 * h), s.f[1], acc);  // p1 q3 | p3 q1
+        acc = mfma(lds8(row + 16), s.f[0], acc);      // p2 q1 | p2 q2
+        acc = mfma(lds8(row), s.f[0], acc);           // p1 q1 | p1 q2
+    } else {
+        constexpr int J = D / 16;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const char* p = row + 32 * j + 16 * h;
+            const bf16x8 a0 = lds8(p);
+            if constexpr (NP == 3) {
+                const bf16x8 a1 = lds8(p + TL::PIECE), a2 = lds8(p + 2 * TL::PIECE);
+                acc = mfma(a2, s.f[j], acc);
+                acc = mfma(a0, s.f[2 * J + j], acc);
+                acc = mfma(a1, s.f[J + j], acc);
+                acc = mfma(a1, s.f[j], acc);
+                acc = mfma(a0, s.f[J + j], acc);
+            }
+            acc = mfma(a0, s.f[j], acc);
+        }
+    }
+    return acc;
+}
+
+// The result registers of a scores-like product as the operand of a values-like one.
+template <int NP>
+struct PFrag {
+    bf16x8 f[2][NP];  // [kk][piece]
+    __device__ __forceinline__ void fill(const f32x16& v) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            u32x4 ws[NP];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                unsigned w[NP];
+                pieces2<NP>(v[8 * kk + 2 * i], v[8 * kk + 2 * i + 1], w);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) ws[p][i] = w[p];
+            }
+#pragma unroll
+            for (int p = 0; p < NP; ++p) f[kk][p] = __builtin_bit_cast(bf16x8, ws[p]);
+        }
+    }
+};
+
+// acc[g][row, column] += sum_x tile[32 g + row, x] frag[x, column] over the 32 steps from x0.
+// Eight rows in three pieces: the pieces lie one after the other in the rows of ONE instruction (rows 8 p + d), three
+// instructions instead of six; eight_rows() sums the pieces' results.
+template <int NP, int D, int XT>
+__device__ __forceinline__ void mma_values(const char* tile, int x0, int l31, int h, const PFrag<NP>& b,
+                                           f32x16 (&acc)[NTile<NP, D, XT>::GROUPS]) {
+    typedef NTile<NP, D, XT> NL;
+#pragma unroll
+    for (int g = 0; g < NL::GROUPS; ++g) {
+        const char* row = tile + (32 * g + l31) * NL::RS + 2 * x0 + 16 * h;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const bf16x8 a0 = lds8(row + 32 * kk);
+            if constexpr (NL::P8) {
+                acc[g] = mfma(a0, b.f[kk][2], acc[g]);
+                acc[g] = mfma(a0, b.f[kk][1], acc[g]);
+            } else if constexpr (NP == 3) {
+                const bf16x8 a1 = lds8(row + 32 * kk + NL::PIECE), a2 = lds8(row + 32 * kk + 2 * NL::PIECE);
+                acc[g] = mfma(a2, b.f[kk][0], acc[g]);
+                acc[g] = mfma(a0, b.f[kk][2], acc[g]);
+                acc[g] = mfma(a1, b.f[kk][1], acc[g]);
+                acc[g] = mfma(a1, b.f[kk][0], acc[g]);
+                acc[g] = mfma(a0, b.f[kk][1], acc[g]);
+            }
+            acc[g] = mfma(a0, b.f[kk][0], acc[g]);
+        }
+    }
+}
+// channel of result register r (of group 0) and whether the register holds one
+template <int NP, int D>
+__device__ __forceinline__ void eight_rows(f32x16& a) {
+    if constexpr (packed8<NP, D>()) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = (a[8 + i] + a[4 + i]) + a[i];
+    }
+}
+__device__ __forceinline__ int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+// ---- positions ----------------------------------------------------------------------------------------------
+// Key s lies at position step * s + offset, query t at position t; the bias of the pair depends on their difference
+// through its bucket, and is constant from `far` on, on either side.  rel[head][step * s + (Tq - 1) - t] holds it times
+// log2(e) (attn_positions_kernel); -inf bars a pair.
+struct Positions {
+    const float* rel;  // null: no bias
+    int nrel;          // entries per head
+    int step, offset, far;
+};
+
+// -1 / +1: every pair of the 32 x 32 tile lies beyond `far` on that side; 0: near.  s: first key, t: first query.
+__device__ __forceinline__ int tile_side(const Positions& p, long long s, long long t) {
+    const long long lo = p.step * s + p.offset - (t + 31), hi = p.step * (s + 31) + p.offset - t;
+    return lo >= p.far ? 1 : hi <= -p.far ? -1 : 0;
+}
+
+}  // namespace attn
+}  // namespace eeggan

@@ -534,3 +534,305 @@ extern "C" int eeggan_multi_copy(const eeggan_adam_tensor* table, int ntensors, 
     }
     return 0;
 }
+
+namespace eeggan {
+namespace {
+// ---- global gradient norm, clipping ----------------------------------------------------------------
+// norm = |scale| sqrt(sum over all tensors of g^2); multiplier = scale * min(1, max_norm / (norm + 1e-6)).
+// Squares and sums are formed in double (one pass over the gradients, bound by reading them: the double-rate fma keeps
+// up with four bytes per element), so no gradient overflows or vanishes on the way and the result does not depend on the
+// cut.  Every workgroup leaves one partial sum and one workgroup adds those up in a fixed order: two launches, no atomics.
+constexpr int64_t NCHUNK = 256 * 4 * 8;
+constexpr int NMAXT = 160;
+
+struct NormPack {
+    const float* g[NMAXT];
+    int64_t n[NMAXT];
+    int first[NMAXT];  // first chunk of the tensor
+    int count;
+};
+
+// index of the tensor that owns workgroup `blk` (chunk counts ascend)
+template <class P>
+__device__ __forceinline__ int owner(const P& pk, int blk) {
+    int lo = 0, hi = pk.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pk.first[mid] <= blk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__global__ __launch_bounds__(256) void grad_square_kernel(NormPack pk, double* __restrict__ part) {
+    __shared__ double red[4];
+    const int ti = owner(pk, blockIdx.x);
+    const float* g = pk.g[ti];
+    const int64_t start = (int64_t)(blockIdx.x - pk.first[ti]) * NCHUNK;
+    const int64_t left = pk.n[ti] - start;
+    const int n = (int)(left < NCHUNK ? left : NCHUNK);
+    g += start;
+    double s = 0.0;
+    const int n4 = n / 4;
+    if (n4 == (int)(NCHUNK / 4)) {
+        f32x4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4u*>(g + 4 * (threadIdx.x + 256 * u));
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_fma((double)v[u][e], (double)v[u][e], s);
+    } else {
+        for (int i = threadIdx.x; i < n4; i += 256) {
+            const f32x4 v = *reinterpret_cast<const f32x4u*>(g + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_fma((double)v[e], (double)v[e], s);
+        }
+        for (int i = 4 * n4 + threadIdx.x; i < n; i += 256) s = __builtin_fma((double)g[i], (double)g[i], s);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+constexpr int SMAXT = 384;
+struct StepPack {
+    float* step[SMAXT];
+    int count;
+};
+
+// The partial sums' sum -> out[0] = norm, out[1] = multiplier (nparts > 0); then, for an optimizer step, the tensors'
+// step counters advance and their bias corrections are formed (in double: 1 - 0.99^t loses six bits in float32).
+__global__ __launch_bounds__(1024) void grad_norm_final_kernel(const double* __restrict__ part, int64_t nparts, double scale,
+                                                               double max_norm, float* __restrict__ out, StepPack sp,
+                                                               float* __restrict__ factors, double lr, double b1, double b2) {
+    __shared__ double red[16];
+    if (nparts > 0) {
+        double s = 0.0;
+        for (int64_t i = threadIdx.x; i < nparts; i += 1024) s += part[i];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double t = 0.0;
+            for (int i = 0; i < 16; ++i) t += red[i];
+            const double norm = fabs(scale) * sqrt(t);
+            const double c = max_norm / (norm + 1e-6);
+            out[0] = (float)norm;
+            out[1] = (float)(scale * (c > 1.0 ? 1.0 : c));  // (a NaN norm spoils the multiplier, as it should)
+        }
+    }
+    for (int i = threadIdx.x; i < sp.count; i += 1024) {
+        const float step = sp.step[i][0] + 1.f;
+        sp.step[i][0] = step;
+        factors[2 * i] = (float)(lr / (1.0 - pow(b1, (double)step)));
+        factors[2 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)step)));
+    }
+}
+
+// g *= multiplier in place; a multiplier of one leaves the tensors as they are, without touching them
+__global__ __launch_bounds__(256) void grad_scale_kernel(NormPack pk, const float* __restrict__ norm) {
+    const float c = norm[1];
+    if (c == 1.f) return;
+    const int ti = owner(pk, blockIdx.x);
+    float* g = const_cast<float*>(pk.g[ti]);
+    const int64_t start = (int64_t)(blockIdx.x - pk.first[ti]) * NCHUNK;
+    const int64_t left = pk.n[ti] - start;
+    const int n = (int)(left < NCHUNK ? left : NCHUNK);
+    g += start;
+    const int n4 = n / 4;
+    f32x4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int i = threadIdx.x + 256 * u;
+        if (i < n4) v[u] = *reinterpret_cast<const f32x4u*>(g + 4 * i);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int i = threadIdx.x + 256 * u;
+        if (i < n4) {
+            const f32x4u o = v[u] * c;
+            *reinterpret_cast<f32x4u*>(g + 4 * i) = o;
+        }
+    }
+    for (int i = 4 * n4 + threadIdx.x; i < n; i += 256) g[i] *= c;
+}
+
+// Adam on multiplier * g, multiplier and bias corrections read from device memory: the clipped gradients are never
+// written (28 bytes per element plus the second reading of g, against 36 with a pass that rescales them).
+struct ClipPack {
+    eeggan_adam_tensor t[MAXT];
+    int first[MAXT];
+    int count;
+};
+__global__ __launch_bounds__(256) void adam_clip_kernel(ClipPack pk, const float* __restrict__ norm,
+                                                        const float* __restrict__ factors, float b1, float one_b1, float b2,
+                                                        float one_b2, float eps) {
+    const int ti = owner(pk, blockIdx.x);
+    const eeggan_adam_tensor t = pk.t[ti];
+    const int64_t start = (int64_t)(blockIdx.x - pk.first[ti]) * CHUNK;
+    const int64_t left = t.n - start;
+    const int n = (int)(left < CHUNK ? left : CHUNK);
+    const float* g = t.g + start;
+    float *p = t.p + start, *m = t.m + start, *v = t.v + start;
+    constexpr int U = (int)(CHUNK / 4 / 256);
+    const int n4 = n / 4;
+    f32x4 g4[U], m4[U], v4[U], p4[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (all loads of the chunk before its first store)
+        const int i = threadIdx.x + 256 * u;
+        if (i < n4) {
+            g4[u] = *reinterpret_cast<const f32x4u*>(g + 4 * i);
+            m4[u] = *reinterpret_cast<const f32x4u*>(m + 4 * i);
+            v4[u] = *reinterpret_cast<const f32x4u*>(v + 4 * i);
+            p4[u] = *reinterpret_cast<const f32x4u*>(p + 4 * i);
+        }
+    }
+    const float c = norm[1], lr = factors[2 * ti], root = factors[2 * ti + 1];
+    auto step = [&](float gr, float& mr, float& vr, float& pr) {
+        gr *= c;
+        mr = b1 * mr + one_b1 * gr;
+        vr = b2 * vr + one_b2 * gr * gr;
+        pr -= lr * mr / (sqrtf(vr) * root + eps);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = threadIdx.x + 256 * u;
+        if (i < n4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float mr = m4[u][e], vr = v4[u][e], pr = p4[u][e];
+                step(g4[u][e], mr, vr, pr);
+                m4[u][e] = mr, v4[u][e] = vr, p4[u][e] = pr;
+            }
+            *reinterpret_cast<f32x4u*>(m + 4 * i) = m4[u];
+            *reinterpret_cast<f32x4u*>(v + 4 * i) = v4[u];
+            *reinterpret_cast<f32x4u*>(p + 4 * i) = p4[u];
+        }
+    }
+    for (int i = 4 * n4 + threadIdx.x; i < n; i += 256) {
+        float mr = m[i], vr = v[i], pr = p[i];
+        step(g[i], mr, vr, pr);
+        m[i] = mr, v[i] = vr, p[i] = pr;
+    }
+}
+
+int check_grads(const char* what, const eeggan_adam_tensor* table, int ntensors) {
+    EEGGAN_REQUIRE(table && ntensors > 0, "%s: bad table", what);
+    int64_t chunks = 0;
+    for (int i = 0; i < ntensors; ++i) {
+        EEGGAN_REQUIRE(table[i].g && table[i].n > 0 && table[i].n < (1ll << 40) &&
+                           (reinterpret_cast<uintptr_t>(table[i].g) & 3) == 0, "%s: bad descriptor %d", what, i);
+        chunks += (table[i].n + CHUNK - 1) / CHUNK;
+        EEGGAN_REQUIRE(chunks < (1ll << 31), "%s: too many elements", what);
+    }
+    return 0;
+}
+int64_t norm_parts(const eeggan_adam_tensor* table, int ntensors) {
+    int64_t parts = 0;
+    for (int i = 0; i < ntensors; ++i) parts += (table[i].n + NCHUNK - 1) / NCHUNK;
+    return parts;
+}
+int make_norm_pack(const eeggan_adam_tensor* table, int first, int ntensors, NormPack* pk) {
+    pk->count = ntensors - first < NMAXT ? ntensors - first : NMAXT;
+    int blocks = 0;
+    for (int i = 0; i < pk->count; ++i) {
+        pk->g[i] = table[first + i].g;
+        pk->n[i] = table[first + i].n;
+        pk->first[i] = blocks;
+        blocks += (int)((table[first + i].n + NCHUNK - 1) / NCHUNK);
+    }
+    return blocks;
+}
+// the partial sums; their number goes to *nparts
+int launch_squares(const char* what, const eeggan_adam_tensor* table, int ntensors, double* part, int64_t* nparts,
+                   hipStream_t st) {
+    *nparts = 0;
+    for (int first = 0; first < ntensors; first += NMAXT) {
+        NormPack pk;
+        const int blocks = make_norm_pack(table, first, ntensors, &pk);
+        hipLaunchKernelGGL(grad_square_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pk, part + *nparts);
+        if (check_launch(what)) return 1;
+        *nparts += blocks;
+    }
+    return 0;
+}
+}  // namespace
+}  // namespace eeggan
+
+using namespace eeggan;
+
+extern "C" size_t eeggan_grad_norm_workspace(const eeggan_adam_tensor* table, int ntensors) {
+    if (check_grads("grad_norm", table, ntensors)) return 0;
+    // partial sums, then two factors per tensor
+    return (size_t)norm_parts(table, ntensors) * sizeof(double) + 2 * (size_t)ntensors * sizeof(float);
+}
+
+extern "C" int eeggan_grad_norm(const eeggan_adam_tensor* table, int ntensors, float scale, double max_norm, float* norm,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    if (check_grads("grad_norm", table, ntensors)) return 1;
+    EEGGAN_REQUIRE(norm && workspace && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0, "grad_norm: null or misaligned pointer");
+    EEGGAN_REQUIRE(max_norm > 0, "grad_norm: max_norm %g is not positive", max_norm);
+    EEGGAN_REQUIRE(workspace_bytes >= eeggan_grad_norm_workspace(table, ntensors), "grad_norm: workspace too small");
+    double* part = reinterpret_cast<double*>(workspace);
+    int64_t nparts;
+    if (launch_squares("grad_norm", table, ntensors, part, &nparts, as_stream(stream))) return 1;
+    StepPack none;
+    none.count = 0;
+    hipLaunchKernelGGL(grad_norm_final_kernel, dim3(1), dim3(1024), 0, as_stream(stream), part, nparts, (double)scale, max_norm,
+                       norm, none, nullptr, 0.0, 0.0, 0.0);
+    return check_launch("grad_norm (sum)");
+}
+
+extern "C" int eeggan_grad_scale(const eeggan_adam_tensor* table, int ntensors, const float* norm, void* stream) {
+    if (check_grads("grad_scale", table, ntensors)) return 1;
+    EEGGAN_REQUIRE(norm, "grad_scale: null pointer");
+    for (int first = 0; first < ntensors; first += NMAXT) {
+        NormPack pk;
+        const int blocks = make_norm_pack(table, first, ntensors, &pk);
+        hipLaunchKernelGGL(grad_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), pk, norm);
+        if (check_launch("grad_scale")) return 1;
+    }
+    return 0;
+}
+
+extern "C" int eeggan_adam_step_clipped(const eeggan_adam_tensor* table, int ntensors, double lr, double beta1, double beta2,
+                                        double eps, const float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+    if (check_grads("adam_step_clipped", table, ntensors)) return 1;
+    EEGGAN_REQUIRE(norm && workspace && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0,
+                   "adam_step_clipped: null or misaligned pointer");
+    EEGGAN_REQUIRE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adam_step_clipped: betas outside [0, 1)");
+    EEGGAN_REQUIRE(workspace_bytes >= 2 * (size_t)ntensors * sizeof(float), "adam_step_clipped: workspace too small");
+    for (int i = 0; i < ntensors; ++i)
+        EEGGAN_REQUIRE(table[i].p && table[i].m && table[i].v && table[i].step &&
+                           ((reinterpret_cast<uintptr_t>(table[i].p) | reinterpret_cast<uintptr_t>(table[i].m) |
+                             reinterpret_cast<uintptr_t>(table[i].v) | reinterpret_cast<uintptr_t>(table[i].step)) & 3) == 0,
+                       "adam_step_clipped: descriptor %d lacks state pointers", i);
+    float* factors = reinterpret_cast<float*>(workspace);
+    hipStream_t st = as_stream(stream);
+    for (int first = 0; first < ntensors; first += SMAXT) {
+        StepPack sp;
+        sp.count = ntensors - first < SMAXT ? ntensors - first : SMAXT;
+        for (int i = 0; i < sp.count; ++i) sp.step[i] = table[first + i].step;
+        hipLaunchKernelGGL(grad_norm_final_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, 0.0, 0.0, nullptr, sp,
+                           factors + 2 * first, lr, beta1, beta2);
+        if (check_launch("adam_step_clipped (steps)")) return 1;
+    }
+    for (int first = 0; first < ntensors; first += MAXT) {
+        ClipPack pk;
+        pk.count = ntensors - first < MAXT ? ntensors - first : MAXT;
+        int blocks = 0;
+        for (int i = 0; i < pk.count; ++i) {
+            pk.t[i] = table[first + i];
+            pk.first[i] = blocks;
+            blocks += (int)((table[first + i].n + CHUNK - 1) / CHUNK);
+        }
+        hipLaunchKernelGGL(adam_clip_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pk, norm, factors + 2 * first,
+                           (float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps);
+        if (check_launch("adam_step_clipped")) return 1;
+    }
+    return 0;
+}

@@ -1,0 +1,318 @@
+// Learned relative position bias by buckets: on stored scores, its gradient, and the per-distance table the fused
+// attention reads.  (bucket, head) sums run in a fixed order.
+#include "attention_host.h"
+
+namespace eeggan {
+namespace attn {
+namespace {
+
+constexpr int MAX_T = 1 << 27;  // time steps of one call
+
+// rel[head][i] = log2(e) * table[bucket(first + i)][head]; entries at or below -1e30 (a mask written into the table, the
+// type's lowest value among them) bar the pair.
+template <class T>
+__global__ __launch_bounds__(256) void positions_kernel(const T* __restrict__ table, float* __restrict__ rel,
+                                                        eeggan_buckets bk, int heads, int nrel, int first) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= nrel) return;
+    const int head = blockIdx.y;
+    const float v = ld1(table + (long long)bucket_of(bk, (long long)first + i) * heads + head);
+    rel[(long long)head * nrel + i] = v <= -1e30f ? -INFINITY : v * LOG2E;
+}
+
+// The bias of one head by distance, -far .. far, in LDS: what lies beyond has the value at the border.
+__device__ __forceinline__ void fill_lut(float* lut, const float* table, const eeggan_buckets& bk, int H, int h, int far) {
+    for (int i = threadIdx.x; i <= 2 * far; i += 256) lut[i] = table[(long long)bucket_of(bk, far - i) * H + h];
+}
+
+// out[n, s, t] = scores[n, s, t] + table[bucket(step s + offset - t), n % H].  A pure stream: a workgroup takes `rows`
+// consecutive rows (n, s) of one n, its threads neighbouring groups of four steps; the value comes from LDS (one read
+// per element, a tenth of what LDS can deliver at the rate the memory can).
+template <bool NT>
+__global__ __launch_bounds__(256) void relbias_kernel(const float* __restrict__ scores, const float* __restrict__ table,
+                                                      float* __restrict__ out, eeggan_buckets bk, int H, int Tk, int Tq,
+                                                      int rows, int chunks) {
+    extern __shared__ float lut[];
+    const int far = bucket_far(bk);
+    const long long n = blockIdx.x / chunks;
+    const int s0 = (int)(blockIdx.x % chunks) * rows;
+    const int s1 = min(Tk, s0 + rows);
+    fill_lut(lut, table, bk, H, (int)(n % H), far);
+    __syncthreads();
+    const int quads = (Tq + 3) / 4;
+    const int drow = 256 / quads, dq = 256 % quads;  // (a thread's next item, without a division per item)
+    int s = s0 + (int)threadIdx.x / quads, q = (int)threadIdx.x % quads;
+    for (; s < s1;) {
+        const int t = 4 * q;
+        const long long at = (n * Tk + s) * Tq + t;
+        // lut index of the quad's first step (far outside: just outside)
+        const long long wide = (long long)t - (long long)bk.step * s - bk.offset + far;
+        const int i0 = (int)(wide < -4 ? -4 : wide > 2 * far ? 2 * far : wide);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        const int have = min(4, Tq - t);
+        if (scores) {
+            if (have == 4) {
+                const f32x4u* p = reinterpret_cast<const f32x4u*>(scores + at);
+                v = NT ? __builtin_nontemporal_load(p) : *p;
+            } else {
+                v = load_few(scores + at, have);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] += lut[min(max(i0 + e, 0), 2 * far)];
+        }
+        if (have == 4) {
+            const f32x4u o = v;
+            if (NT) __builtin_nontemporal_store(o, reinterpret_cast<f32x4u*>(out + at));
+            else *reinterpret_cast<f32x4u*>(out + at) = o;
+        } else {
+            for (int e = 0; e < have; ++e) out[at + e] = v[e];
+        }
+        q += dq;
+        s += drow;
+        if (q >= quads) {
+            q -= quads;
+            ++s;
+        }
+    }
+}
+
+// Sums of g by distance.  A wave takes every fourth of its workgroup's rows.  In a row the distances beyond the last
+// edge are two contiguous stretches, added up as a stream; the band between them goes to a histogram by distance in LDS
+// whose entries each belong to one lane of the wave: no atomics, a fixed order, and double throughout (the near entries
+// of a long recording sum millions of terms).  hist: [H][rows of partial sums][2 far + 1]: distances -(far - 1) ..
+// far - 1, then everything behind, then everything ahead.
+__global__ __launch_bounds__(256) void relbias_sums_kernel(const float* __restrict__ g, double* __restrict__ hist,
+                                                           eeggan_buckets bk, int B, int H, int Tk, int Tq, int rows,
+                                                           int chunks) {
+    extern __shared__ double band[];
+    const int far = bucket_far(bk), width = far - 1, n = 2 * width + 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double* const mine = band + wave * (n + 2);
+    for (int i = lane; i < n + 2; i += 64) mine[i] = 0.0;
+    const long long bh = blockIdx.x / chunks;
+    const int chunk = (int)(blockIdx.x % chunks);
+    const int s0 = chunk * rows, s1 = min(Tk, s0 + rows);
+    double beyond[2] = {0.0, 0.0};
+    for (int s = s0 + wave; s < s1; s += 4) {
+        const float* row = g + (bh * Tk + s) * Tq;
+        const long long key = (long long)bk.step * s + bk.offset;  // distance of step t: key - t
+        // steps [0, a): ahead of them by `far` or more; [a, b): the band; [b, Tq): behind
+        const int a = (int)min((long long)Tq, max(0ll, key - far + 1)), b = (int)min((long long)Tq, max(0ll, key + far));
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const int from = side ? b : 0, to = side ? Tq : a;
+            double sum = 0.0;
+            int t = from + 4 * lane;
+            for (; t + 3 * 256 + 3 < to; t += 4 * 256) {
+                f32x4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = load4(row + t + 256 * u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) sum += (double)((v[u][0] + v[u][1]) + (v[u][2] + v[u][3]));
+            }
+            for (; t < to; t += 256) {
+                f32x4 v;
+                if (t + 3 < to) v = load4(row + t);
+                else v = load_few(row + t, to - t);
+                sum += (double)((v[0] + v[1]) + (v[2] + v[3]));
+            }
+            beyond[side] += sum;
+        }
+        // band index of step t: key - t + width; lane owns the indices = lane mod 64
+        if (a < b) {
+            const int i0 = (int)(key - (b - 1) + width), i1 = (int)(key - a + width);
+            for (int i = (i0 & ~63) + lane; i <= i1; i += 64)
+                if (i >= i0) mine[i] += (double)row[key + width - i];
+        }
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+        for (int o = 32; o > 0; o >>= 1) beyond[side] += __shfl_xor(beyond[side], o, 64);
+    if (lane == 0) {
+        mine[n] = beyond[1];
+        mine[n + 1] = beyond[0];
+    }
+    __syncthreads();
+    const long long b = bh / H, h = bh % H;
+    double* const out = hist + ((h * B + b) * chunks + chunk) * (n + 2);
+    for (int i = threadIdx.x; i < n + 2; i += 256)
+        out[i] = (band[i] + band[n + 2 + i]) + (band[2 * (n + 2) + i] + band[3 * (n + 2) + i]);
+}
+
+// Bucket sums from histograms by distance (-width .. width, behind, ahead): one workgroup per (bucket, head); a bucket
+// is a stretch of the histogram.
+template <class TH, class TO>
+__global__ __launch_bounds__(256) void bucket_sums_kernel(const TH* __restrict__ hist, TO* __restrict__ out, eeggan_buckets bk,
+                                                          int H, long long rows, int width) {
+    __shared__ double red[256];
+    const int j = blockIdx.x, head = blockIdx.y, side = bucket_side(bk);
+    const bool ahead = j >= side;
+    const int e = ahead ? j - side : j;
+    const bool last = e == side - 1;
+    const int near = bk.edges[e], beyond = last ? width : min(width, bk.edges[last ? e : e + 1] - 1);
+    int lo, hi;
+    if (ahead) {
+        lo = width + max(near, 1);
+        hi = width + beyond;
+    } else {
+        lo = width - beyond;
+        hi = !bk.bidirectional && e == 0 ? 2 * width : width - near;
+    }
+    const int behind_at = last && !ahead ? 2 * width + 1 : -1;
+    const int ahead_at = (ahead && last) || (!bk.bidirectional && e == 0) ? 2 * width + 2 : -1;
+    const int n = max(0, hi - lo + 1), stride = 2 * width + 3;
+    const TH* const h0 = hist + (long long)head * rows * stride;
+    double sum = 0.0;
+    for (long long k = threadIdx.x; k < rows * n; k += 256) sum += (double)h0[(k / n) * stride + lo + k % n];
+    for (long long r = threadIdx.x; r < rows; r += 256) {
+        if (behind_at >= 0) sum += (double)h0[r * stride + behind_at];
+        if (ahead_at >= 0) sum += (double)h0[r * stride + ahead_at];
+    }
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) st1(out + (long long)j * H + head, (float)red[0]);
+}
+
+}  // namespace
+
+int check_attention(const char* what, const eeggan_attention* a) {
+    EEGGAN_REQUIRE(a && a->q && a->k && a->v, "%s: null pointer", what);
+    EEGGAN_REQUIRE(a->B > 0 && a->H > 0 && a->KV > 0 && a->Tq > 0 && a->Tk > 0 && a->Dk > 0 && a->Dv > 0,
+                   "%s: bad shape (B=%d H=%d KV=%d Dk=%d Dv=%d Tq=%d Tk=%d)", what, a->B, a->H, a->KV, a->Dk, a->Dv, a->Tq,
+                   a->Tk);
+    EEGGAN_REQUIRE(a->H % a->KV == 0, "%s: %d query heads cannot share %d key heads", what, a->H, a->KV);
+    EEGGAN_REQUIRE(a->Dk <= 128 && a->Dv <= 128, "%s: heads of up to 128 channels, got %d and %d", what, a->Dk, a->Dv);
+    EEGGAN_REQUIRE(a->Tq <= MAX_T && a->Tk <= MAX_T && (long long)(a->H / a->KV) * a->Tq <= MAX_T,
+                   "%s: more than %d time steps", what, MAX_T);
+    EEGGAN_REQUIRE(a->q_batch >= 0 && a->q_channel >= 0 && a->k_batch >= 0 && a->k_channel >= 0 && a->v_batch >= 0 &&
+                       a->v_channel >= 0,
+                   "%s: negative stride", what);
+    const uintptr_t odd = a->bf16 ? 1 : 3;
+    EEGGAN_REQUIRE(((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
+                     reinterpret_cast<uintptr_t>(a->v)) & odd) == 0, "%s: misaligned tensor", what);
+    if (a->table) {
+        if (check_buckets(what, a->buckets)) return 1;
+        EEGGAN_REQUIRE(positions_entries(*a) < (1ll << 30), "%s: positions out of range", what);
+        EEGGAN_REQUIRE(a->H <= 65535, "%s: too many heads", what);
+    }
+    return 0;
+}
+
+int positions(const eeggan_attention& a, float* rel, Positions* p, hipStream_t st) {
+    if (!a.table) {
+        *p = Positions{nullptr, 0, 1, 0, 1};
+        return 0;
+    }
+    const eeggan_buckets bk = *a.buckets;
+    const int nrel = (int)positions_entries(a);
+    *p = Positions{rel, nrel, bk.step, bk.offset, bucket_far(bk)};
+    const dim3 grid((unsigned)((nrel + 255) / 256), (unsigned)a.H);
+    const int first = bk.offset - (a.Tq - 1);
+    if (a.table_bf16)
+        hipLaunchKernelGGL(positions_kernel<__bf16>, grid, dim3(256), 0, st, reinterpret_cast<const __bf16*>(a.table), rel,
+                           bk, a.H, nrel, first);
+    else
+        hipLaunchKernelGGL(positions_kernel<float>, grid, dim3(256), 0, st, reinterpret_cast<const float*>(a.table), rel, bk,
+                           a.H, nrel, first);
+    return check_launch("attention (positions)");
+}
+
+int bucket_sums(const float* hist, void* out, int out_bf16, const eeggan_buckets& bk, int H, long long rows, int width,
+                hipStream_t st) {
+    const dim3 grid((unsigned)bk.count, (unsigned)H);
+    if (out_bf16)
+        hipLaunchKernelGGL((bucket_sums_kernel<float, __bf16>), grid, dim3(256), 0, st, hist, reinterpret_cast<__bf16*>(out),
+                           bk, H, rows, width);
+    else
+        hipLaunchKernelGGL((bucket_sums_kernel<float, float>), grid, dim3(256), 0, st, hist, reinterpret_cast<float*>(out),
+                           bk, H, rows, width);
+    return check_launch("attention backward (table)");
+}
+
+}  // namespace attn
+}  // namespace eeggan
+
+using namespace eeggan;
+using namespace eeggan::attn;
+
+static int check_relbias(const char* what, const eeggan_buckets* b, int B, int H, int Tk, int Tq) {
+    EEGGAN_REQUIRE(B > 0 && H > 0 && Tk > 0 && Tq > 0 && Tk <= MAX_T && Tq <= MAX_T && H <= 65535,
+                   "%s: bad shape (B=%d H=%d Tk=%d Tq=%d)", what, B, H, Tk, Tq);
+    return check_buckets(what, b);
+}
+
+namespace {
+struct Rows {
+    int rows, chunks;
+    long long blocks;
+};
+// rows (n, s) of one n per workgroup, for about `elements` elements, and the number of workgroups
+Rows rows_of(long long n, int Tk, int Tq, long long elements) {
+    long long rows = elements / Tq;
+    rows = rows < 4 ? 4 : rows;
+    if (rows > Tk) rows = Tk;
+    Rows r;
+    r.rows = (int)rows;
+    r.chunks = (int)((Tk + rows - 1) / rows);
+    r.blocks = n * r.chunks;
+    return r;
+}
+// sums: at most ~2048 workgroups (their partial sums are read again), at least 4 rows each
+Rows sum_rows_of(long long n, int Tk, int Tq) {
+    const long long total = n * Tk * (long long)Tq;
+    return rows_of(n, Tk, Tq, total / 2048 > 32768 ? total / 2048 : 32768);
+}
+}  // namespace
+
+extern "C" int eeggan_relative_bias(const float* scores, const float* table, const eeggan_buckets* buckets, float* out,
+                                    int B, int H, int Tk, int Tq, void* stream) {
+    EEGGAN_REQUIRE(table && out, "relative_bias: null pointer");
+    if (check_relbias("relative_bias", buckets, B, H, Tk, Tq)) return 1;
+    // about 16 K elements to a workgroup: enough to hide the table, few enough to fill the chip
+    const Rows r = rows_of((long long)B * H, Tk, Tq, 16384);
+    EEGGAN_REQUIRE(r.blocks < (1ll << 31), "relative_bias: too many rows");
+    const size_t lds = (2 * (size_t)bucket_far(*buckets) + 1) * sizeof(float);
+    const dim3 grid((unsigned)r.blocks);
+    if (streams_past_caches((size_t)B * H * Tk * Tq * sizeof(float) * (scores ? 2 : 1)))
+        hipLaunchKernelGGL(relbias_kernel<true>, grid, dim3(256), lds, as_stream(stream), scores, table, out, *buckets, H, Tk,
+                           Tq, r.rows, r.chunks);
+    else
+        hipLaunchKernelGGL(relbias_kernel<false>, grid, dim3(256), lds, as_stream(stream), scores, table, out, *buckets, H,
+                           Tk, Tq, r.rows, r.chunks);
+    return check_launch("relative_bias");
+}
+
+extern "C" size_t eeggan_relative_bias_grad_workspace(const eeggan_buckets* buckets, int B, int H, int Tk, int Tq) {
+    if (check_relbias("relative_bias_grad", buckets, B, H, Tk, Tq)) return 0;
+    return (size_t)sum_rows_of((long long)B * H, Tk, Tq).blocks * (2 * (size_t)bucket_far(*buckets) + 1) * sizeof(double);
+}
+
+extern "C" int eeggan_relative_bias_grad(const float* g, const eeggan_buckets* buckets, float* g_table, int B, int H,
+                                         int Tk, int Tq, void* workspace, size_t workspace_bytes, void* stream) {
+    EEGGAN_REQUIRE(g && g_table && workspace, "relative_bias_grad: null pointer");
+    if (check_relbias("relative_bias_grad", buckets, B, H, Tk, Tq)) return 1;
+    EEGGAN_REQUIRE(workspace_bytes >= eeggan_relative_bias_grad_workspace(buckets, B, H, Tk, Tq) &&
+                       (reinterpret_cast<uintptr_t>(workspace) & 7) == 0,
+                   "relative_bias_grad: workspace too small or misaligned");
+    const Rows r = sum_rows_of((long long)B * H, Tk, Tq);
+    EEGGAN_REQUIRE(r.blocks < (1ll << 31), "relative_bias_grad: too many rows");
+    const int far = bucket_far(*buckets);
+    const size_t lds = 4 * (2 * (size_t)far + 1) * sizeof(double);
+    static LdsReady ready;
+    if (ready.reserve("relative_bias_grad", reinterpret_cast<const void*>(&relbias_sums_kernel), 4 * 2049 * sizeof(double)))
+        return 1;
+    double* const hist = reinterpret_cast<double*>(workspace);
+    hipStream_t st = as_stream(stream);
+    hipLaunchKernelGGL(relbias_sums_kernel, dim3((unsigned)r.blocks), dim3(256), lds, st, g, hist, *buckets, B, H, Tk, Tq,
+                       r.rows, r.chunks);
+    if (check_launch("relative_bias_grad")) return 1;
+    hipLaunchKernelGGL((bucket_sums_kernel<double, float>), dim3((unsigned)buckets->count, (unsigned)H), dim3(256), 0, st, hist,
+                       g_table, *buckets, H, (long long)B * r.chunks, far - 1);
+    return check_launch("relative_bias_grad (buckets)");
+}

@@ -122,6 +122,8 @@ class _SplitCriticIteration:
             for p, g in grads.items():
                 p.grad = g
             early = list(grads)
+            if getattr(opt, "max_grad_norm", None) is not None:
+                return []  # the norm spans all gradients: one bucket, one optimizer step
             if bucketed and early:
                 self.bucket_early = sync.pack(dis, params=early, slot="early")
             return early
@@ -449,7 +451,8 @@ class GraphedTrainer(Trainer):
                  float(dis.alpha) if getattr(dis, "input_to_all_layers", False) else None)
         key = (gen.depth, gen.alpha < 1.0, dis.alpha < 1.0, baked, tuple(real.shape), tuple(zs[0].shape), repeats,
                id(self.optimizer_d), id(self.optimizer_g),
-               self.optimizer_d.param_groups[0]["lr"], self.optimizer_g.param_groups[0]["lr"])
+               self.optimizer_d.param_groups[0]["lr"], self.optimizer_g.param_groups[0]["lr"],
+               getattr(self.optimizer_d, "max_grad_norm", None), getattr(self.optimizer_g, "max_grad_norm", None))
         if key != self._key:
             self._capture(real, zs[0], key)
         fakes = None

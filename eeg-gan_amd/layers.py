@@ -331,11 +331,20 @@ class SelfAttention(nn.Module):
     """out = gamma * final(value P) + x with P = softmax over the key positions of key^T query, key and value
     max-pooled by 4 along time; query / key / value / final are linear 1x1 convs without bias and gamma is a scalar
     parameter that starts at zero (reference layers.py:41-64).  Returns (out, P).  Twice differentiable (the critic's
-    gradient penalty passes through it).  float32 tensors only."""
+    gradient penalty passes through it).  float32 tensors only.
 
-    def __init__(self, channels_in, spectral, init="xavier_uniform"):
+    Beyond the reference: ``heads`` splits the channels of query, key and value (P is then [B, heads, T / 4, T]);
+    ``buckets`` > 0 adds a learned bias by relative position to the scores (parameter ``positions`` [buckets, heads],
+    zero at the start; distances in time steps between a query and the middle of a key's window, up to
+    ``max_distance``).  Under ``ops.set_attention('recompute')`` the map is not kept for the backward passes and not
+    returned: (out, None)."""
+
+    def __init__(self, channels_in, spectral, init="xavier_uniform", heads=1, buckets=0, max_distance=128):
         super().__init__()
         d_key = max(channels_in // 8, 2)
+        if heads < 1 or d_key % heads or (channels_in // 2) % heads:
+            raise ValueError(f"SelfAttention: {d_key} key and {channels_in // 2} value channels do not split into {heads} "
+                             "heads")
         conf = dict(kernel_size=1, equalized=False, spectral=spectral, init=init, bias=False, act_alpha=-1)
         self.gamma = nn.Parameter(torch.tensor(0.0), requires_grad=True)
         self.pooling = nn.MaxPool1d(4)  # (parameter-less; kept for module-tree parity)
@@ -345,14 +354,35 @@ class SelfAttention(nn.Module):
         self.final_conv = GeneralConv(channels_in // 2, channels_in, **conf)
         self.softmax = nn.Softmax(dim=-1)
         self.scale = 1.0
+        self.heads = heads
+        self.positions = self.buckets = None
+        if buckets:
+            pool = self.pooling.kernel_size
+            self.buckets = ops.RelativeBuckets(buckets, max_distance, step=pool, offset=pool // 2)
+            self.positions = nn.Parameter(torch.zeros(buckets, heads))
 
     def forward(self, x):
         pool = self.pooling.kernel_size
         query = self.query_conv(x)
         key = ops.maxpool(self.key_conv(x), pool)
         value = ops.maxpool(self.value_conv(x), pool)
-        attention = ops.softmax_dim1(ops.bmm(key, query, trans_a=True, alpha=1.0 / self.scale))
-        out = self.final_conv(ops.bmm(value, attention))
+        if ops.get_attention() == "recompute":
+            attention = None
+            mixed = ops.attention(query, key, value, heads=self.heads, scale=1.0 / self.scale, bias=self.positions,
+                                  buckets=self.buckets)
+        else:
+            split = lambda t: t.reshape(t.shape[0] * self.heads, -1, t.shape[2])  # noqa: E731
+            if self.heads > 1:
+                query, key, value = split(query), split(key), split(value)
+            scores = ops.bmm(key, query, trans_a=True, alpha=1.0 / self.scale)
+            if self.positions is not None:
+                scores = ops.relative_bias(scores, self.positions, self.buckets, heads=self.heads)
+            attention = ops.softmax_dim1(scores)
+            mixed = ops.bmm(value, attention)
+            if self.heads > 1:
+                mixed = mixed.reshape(x.shape[0], -1, x.shape[2])
+                attention = attention.reshape((x.shape[0], self.heads) + tuple(attention.shape[1:]))
+        out = self.final_conv(mixed)
         return ops.axpby(ops.mul_param(out, self.gamma), 1.0, x, 1.0), attention
 
 

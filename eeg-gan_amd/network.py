@@ -137,7 +137,7 @@ class Generator(nn.Module):
                  init, act_alpha, num_classes, deep, z_distribution, spectral=False, latent_size=256, no_tanh=False,
                  per_channel_noise=False, to_rgb_mode="pggan", z_to_bn=False, split_z=False, dropout=0.2,
                  act_norm="pixel", conv_only=False, shared_embedding_size=32, normalize_latents=True,
-                 rgb_generation_mode="pggan"):
+                 rgb_generation_mode="pggan", attention_options=None):
         super().__init__()
         _require(num_classes == 0 or act_norm == "batch", "class conditioning without batch norm layers")
         _require(not conv_only or not split_z, "conv_only with split_z")
@@ -189,7 +189,8 @@ class Generator(nn.Module):
         self.block0 = GBlock(latent_size, nf(1), initial_kernel_size=None if conv_only else initial_kernel_size,
                              **block_settings, **layer_settings)
         self.self_attention = dict()  # (network.py:304-310: stage -> layer; registered through ``dummy``)
-        attention = [SelfAttention(nf(layer + 1), spectral, init) for layer in self_attention_layers or ()]
+        attention = [SelfAttention(nf(layer + 1), spectral, init, **(attention_options or {}))
+                     for layer in self_attention_layers or ()]
         self.self_attention.update(zip(self_attention_layers or (), attention))
         if attention:
             self.dummy = nn.ModuleList(attention)
@@ -313,7 +314,7 @@ class Discriminator(nn.Module):
                  self_attention_layers, progression_scale_up, progression_scale_down, residual, separable, equalized,
                  init, act_alpha, num_classes, deep, spectral=False, dropout=0.2, act_norm=None, group_size=4,
                  temporal_groups_per_window=1, conv_only=False, input_to_all_layers=False, initial_sampling_rate=1.0,
-                 sinc=False):
+                 sinc=False, attention_options=None):
         super().__init__()
         _require(not sinc, "sinc")
         _require(act_norm in (None, "batch", "pixel"), f"act_norm={act_norm!r} in the discriminator")
@@ -342,7 +343,8 @@ class Discriminator(nn.Module):
         up, down = np.array(progression_scale_up), np.array(progression_scale_down)
         lens = [initial_kernel_size * np.sum(up[:i] / down[:i]) for i in range(stages + 1)]
         self.self_attention = dict()  # (network.py:503-509)
-        attention = [SelfAttention(nf(layer + 1), spectral, init) for layer in self_attention_layers or ()]
+        attention = [SelfAttention(nf(layer + 1), spectral, init, **(attention_options or {}))
+                     for layer in self_attention_layers or ()]
         self.self_attention.update(zip(self_attention_layers or (), attention))
         if attention:
             self.dummy = nn.ModuleList(attention)

@@ -1655,6 +1655,291 @@ def mul_param(f, s):
     return _MulParam.apply(f, s)
 
 
+# --------------------------------------------------------------------------------------- attention without stored maps
+class _Buckets(ctypes.Structure):
+    _fields_ = [("count", ctypes.c_int), ("bidirectional", ctypes.c_int), ("step", ctypes.c_int),
+                ("offset", ctypes.c_int), ("edges", ctypes.c_int * 64)]
+
+
+class _AttentionDesc(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int64) for n in ("q_batch", "q_channel", "k_batch", "k_channel", "v_batch", "v_channel")] + \
+        [("mask", ctypes.c_void_p), ("table", ctypes.c_void_p), ("buckets", ctypes.c_void_p)] + \
+        [(n, ctypes.c_int) for n in ("bf16", "table_bf16", "B", "H", "KV", "Dk", "Dv", "Tq", "Tk")] + \
+        [("scale", ctypes.c_float)]
+
+
+class RelativeBuckets:
+    """How a learned bias depends on relative position: ``num_buckets`` rows of a table, by the distance
+    ``step * s + offset - t`` of key s from query t (``step``: time steps per key, e.g. 4 for keys max-pooled by four;
+    ``offset``: position of the first key on the queries' time axis).  Half of a side's buckets hold one distance each,
+    the others grow geometrically up to ``max_distance``, from where on the last one holds everything; the borders are
+    exact (whole-number arithmetic).  ``bidirectional``: keys ahead of the query have the second half of the buckets to
+    themselves; otherwise they share bucket 0 with distance 0.  The object is constant and may be used by any number
+    of calls."""
+
+    def __init__(self, num_buckets=32, max_distance=128, bidirectional=True, step=1, offset=0):
+        side = num_buckets // 2 if bidirectional else num_buckets
+        if side < 2 or side > 64 or (bidirectional and num_buckets % 2):
+            raise ValueError(f"RelativeBuckets: {num_buckets} buckets: 2 .. 64 on a side are supported"
+                             f"{', the same number on both' if bidirectional else ''}")
+        if not 1 <= step <= 16:
+            raise ValueError(f"RelativeBuckets: step {step} outside 1 .. 16")
+        exact = side // 2
+        if not exact < max_distance <= 1024 or max_distance - exact < side - exact:
+            raise ValueError(f"RelativeBuckets: max_distance {max_distance}: up to 1024, and enough for {side} buckets")
+        edges, grown = list(range(exact)), side - exact
+        for i in range(grown):  # smallest d >= exact * (max_distance / exact) ** (i / grown), without rounding
+            lo, hi = exact, max_distance
+            bound = exact ** (grown - i) * max_distance ** i
+            while lo < hi:
+                mid = (lo + hi) // 2
+                lo, hi = (lo, mid) if mid ** grown >= bound else (mid + 1, hi)
+            edges.append(max(lo, edges[-1] + 1))
+        self.num_buckets, self.max_distance, self.bidirectional = int(num_buckets), int(max_distance), bool(bidirectional)
+        self.step, self.offset, self.edges = int(step), int(offset), tuple(edges)
+        self._c = _Buckets(self.num_buckets, int(self.bidirectional), self.step, self.offset)
+        for i, e in enumerate(edges):
+            self._c.edges[i] = e
+
+    def _ptr(self):
+        return ctypes.addressof(self._c)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_c"}
+
+    def __setstate__(self, state):
+        self.__init__(state["num_buckets"], state["max_distance"], state["bidirectional"], state["step"], state["offset"])
+
+    def bucket(self, rel: int) -> int:
+        """The bucket of one distance (the definition the kernels follow)."""
+        dist = abs(rel) if self.bidirectional or rel < 0 else 0
+        side = sum(dist >= e for e in self.edges) - 1
+        return side + (self.num_buckets // 2 if self.bidirectional and rel > 0 else 0)
+
+
+def _on(t):
+    """Launches for ``t``: its device made current (restored afterwards)."""
+    return torch.cuda.device(t.device)
+
+
+def _table_chk(table, buckets, heads, device, what):
+    if buckets is None or not isinstance(buckets, RelativeBuckets):
+        raise RuntimeError(f"{what}: a position table needs its RelativeBuckets")
+    if tuple(table.shape) != (buckets.num_buckets, heads):
+        raise RuntimeError(f"{what}: table {tuple(table.shape)}, expected {(buckets.num_buckets, heads)}")
+    if table.device != device:
+        raise RuntimeError(f"{what}: table on {table.device}, scores on {device}")
+
+
+class _RelBias(Function):
+    """scores + table[bucket]: linear in both; its gradient by the table is _RelBiasSum, whose own gradient is this
+    operator without scores."""
+
+    @staticmethod
+    def forward(ctx, scores, table, buckets, heads, shape):
+        ctx.cfg = (buckets, heads)
+        out = torch.empty(shape, device=table.device, dtype=torch.float32)
+        with _on(table):
+            call("eeggan_relative_bias", _p(scores), table.data_ptr(), buckets._ptr(), out.data_ptr(), shape[0] // heads,
+                 heads, shape[1], shape[2], _stream())
+        return out
+
+    @staticmethod
+    def backward(ctx, g):
+        buckets, heads = ctx.cfg
+        gt = _RelBiasSum.apply(_chk(g, "relative bias cotangent"), buckets, heads) if ctx.needs_input_grad[1] else None
+        return g if ctx.needs_input_grad[0] else None, gt, None, None, None
+
+
+class _RelBiasSum(Function):
+    @staticmethod
+    def forward(ctx, g, buckets, heads):
+        ctx.cfg = (buckets, heads, tuple(g.shape))
+        out = torch.empty((buckets.num_buckets, heads), device=g.device, dtype=torch.float32)
+        dims = (g.shape[0] // heads, heads, g.shape[1], g.shape[2])
+        with _on(g):
+            nbytes = _lib.load().eeggan_relative_bias_grad_workspace(buckets._ptr(), *dims)
+            ws = torch.empty(max(nbytes, 16), device=g.device, dtype=torch.uint8)
+            call("eeggan_relative_bias_grad", g.data_ptr(), buckets._ptr(), out.data_ptr(), *dims, ws.data_ptr(), nbytes,
+                 _stream())
+        return out
+
+    @staticmethod
+    def backward(ctx, q):
+        buckets, heads, shape = ctx.cfg
+        return _RelBias.apply(None, _chk(q, "relative bias second-order cotangent"), buckets, heads, shape), None, None
+
+
+def relative_bias(scores, table, buckets: RelativeBuckets, heads: int = 1):
+    """scores [B * heads, Tk, Tq] + table[bucket(step * s + offset - t), head] (float32; twice differentiable): the
+    learned relative positions on stored scores, before ``softmax_dim1``.  Score row n belongs to head n % heads."""
+    scores, table = _chk(scores, "relative_bias scores"), _chk(table, "relative_bias table")
+    if scores.dim() != 3 or heads < 1 or scores.shape[0] % heads or 0 in scores.shape:
+        raise RuntimeError(f"relative_bias: scores {tuple(scores.shape)} are not [B * {heads}, Tk, Tq]")
+    _table_chk(table, buckets, heads, scores.device, "relative_bias")
+    return _RelBias.apply(scores, table, buckets, int(heads), tuple(scores.shape))
+
+
+_attention_mode = "stored"
+
+
+def set_attention(mode: str) -> str:
+    """How ``layers.SelfAttention`` runs: 'stored' (default: the map is kept for the backward passes and returned) or
+    'recompute' (``attention``: nothing of the map's size is kept, the backward pass forms it again; the layer returns
+    no map).  Process-wide, for the passes that follow; captured graphs keep the mode they were captured in.  Returns
+    the previous mode."""
+    global _attention_mode
+    if mode not in ("stored", "recompute"):
+        raise ValueError(f"attention {mode!r}: expected 'stored' or 'recompute'")
+    previous, _attention_mode = _attention_mode, mode
+    return previous
+
+
+def get_attention() -> str:
+    return _attention_mode
+
+
+def _rows(t):
+    """A [B, C, T] tensor the attention kernels can read: unit stride in time, any strides otherwise (a slice of the
+    channels of a wider tensor, an expanded batch); else a copy."""
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _attention_desc(q, k, v, mask, table, cfg):
+    heads, kv_heads, scale, buckets = cfg
+    a = _AttentionDesc()
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_batch, a.q_channel, a.k_batch, a.k_channel = q.stride(0), q.stride(1), k.stride(0), k.stride(1)
+    a.v_batch, a.v_channel = v.stride(0), v.stride(1)
+    a.mask, a.table = _p(mask), _p(table)
+    a.buckets = buckets._ptr() if table is not None else None
+    a.bf16, a.table_bf16 = _bf(q), _bf(table)
+    a.B, a.H, a.KV = q.shape[0], heads, kv_heads
+    a.Dk, a.Dv, a.Tq, a.Tk = q.shape[1] // heads, v.shape[1] // kv_heads, q.shape[2], k.shape[2]
+    a.scale = scale
+    return a
+
+
+def _attention_stored(q, k, v, table, mask, cfg):
+    """The same function out of the operators with stored scores, which differentiate twice (float32)."""
+    heads, kv, scale, buckets = cfg
+    q, k, v = q.float(), k.float(), v.float()
+    B, G, dk, dv, tq, tk = q.shape[0], heads // kv, q.shape[1] // heads, v.shape[1] // kv, q.shape[2], k.shape[2]
+    if mask is not None:
+        k, v = (t.masked_fill(~mask[:, None, :], 0.0) for t in (k, v))
+    rows = lambda t: t.reshape(B * heads, -1, t.shape[2])  # noqa: E731
+    share = lambda t: rows(t.reshape(B, kv, 1, -1, tk).expand(B, kv, G, t.shape[1] // kv, tk).reshape(B, -1, tk))  # noqa: E731
+    s = bmm(share(k), rows(q), trans_a=True, alpha=scale)
+    if table is not None:
+        t = table.float()
+        barred = t <= -1e30
+        s = relative_bias(s, t.masked_fill(barred, -1e30), buckets, heads)
+        mask_s = s.detach() > -5e29  # (barred pairs: weight zero, like masked keys)
+    else:
+        mask_s = None
+    if mask is not None:
+        m = mask[:, None, :, None].expand(B, heads, tk, tq).reshape(B * heads, tk, tq)
+        mask_s = m if mask_s is None else m & mask_s
+        s = s.masked_fill(~m, -1e30)
+    p = softmax_dim1(s)
+    if mask_s is not None:
+        p = p * mask_s
+    return bmm(share(v), p).reshape(B, heads * dv, tq)
+
+
+class _Attention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, mask, cfg, keep):
+        a = _attention_desc(q, k, v, mask, table, cfg)
+        out = torch.empty((q.shape[0], v.shape[1] // cfg[1] * cfg[0], q.shape[2]), device=q.device, dtype=q.dtype)
+        lse = torch.empty((q.shape[0], cfg[0], q.shape[2]), device=q.device, dtype=torch.float32) if keep else None
+        rest = torch.empty_like(out) if keep and _bf(q) else None
+        with _on(q):
+            nbytes = _lib.load().eeggan_attention_fwd_workspace(ctypes.byref(a))
+            ws = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
+            call("eeggan_attention_fwd", ctypes.byref(a), out.data_ptr(), _p(rest), _p(lse), ws.data_ptr(), nbytes, _stream())
+        ctx.cfg = cfg
+        ctx.save_for_backward(q, k, v, table, mask, out, rest, lse)
+        return out
+
+    @staticmethod
+    def backward(ctx, g):
+        q, k, v, table, mask, out, rest, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        want_table = table is not None and need[3] and not _input_grad_only
+        if torch.is_grad_enabled():
+            # a graph for second derivatives is being built: the pass is made of operators that have them
+            ins = [q, k, v, table]
+            wanted = [i for i in range(4) if need[i] and (i < 3 or want_table)]
+            with torch.enable_grad():
+                again = _attention_stored(q, k, v, table, mask, ctx.cfg)
+                got = torch.autograd.grad(again, [ins[i] for i in wanted], g.float(), create_graph=True)
+            grads = dict(zip(wanted, got))
+            return tuple(grads.get(i) for i in range(4)) + (None, None, None)
+        g = g.to(q.dtype).contiguous()
+        a = _attention_desc(q, k, v, mask, table, ctx.cfg)
+        gq, gk, gv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        gt = torch.empty(table.shape, device=table.device, dtype=table.dtype) if want_table else None
+        with _on(q):
+            nbytes = _lib.load().eeggan_attention_bwd_workspace(ctypes.byref(a), int(want_table))
+            ws = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
+            call("eeggan_attention_bwd", ctypes.byref(a), out.data_ptr(), _p(rest), lse.data_ptr(), g.data_ptr(),
+                 gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _p(gt), ws.data_ptr(), nbytes, _stream())
+        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, gt, None, None, None
+
+
+def attention(q, k, v, *, heads: int = 1, kv_heads: Optional[int] = None, scale: float = 1.0, mask=None, bias=None,
+              buckets: Optional[RelativeBuckets] = None):
+    """out[c, t] = sum_s v[c, s] softmax_s(scale * sum_d k[d, s] q[d, t] + bias)[s, t] per sample and head, without the
+    [Tk, Tq] map ever being stored: the backward pass forms it again.
+
+    q [B, heads * Dk, Tq], k [B, kv_heads * Dk, Tk], v [B, kv_heads * Dv, Tk], all float32 or all bfloat16 -> out
+    [B, heads * Dv, Tq]; Dk and Dv up to 128, any lengths from one step, any strides with unit stride in time (other
+    layouts are copied).  ``kv_heads`` (default ``heads``): query head h reads key head h // (heads // kv_heads).
+    ``mask``: bool [B, Tk], True = this key may be attended; what masked keys hold is never used.  A query with no key
+    left has zeros and no gradient.  ``bias`` [buckets.num_buckets, heads] (the operands' type or float32): learned bias
+    by relative position; entries <= -1e30 bar their pairs.
+
+    Gradients of q, k, v and the table come from kernels with a fixed order of summation.  Under ``create_graph=True``
+    the backward pass is made of the operators with stored scores instead (float32), which are twice differentiable."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise RuntimeError(f"attention {name}: expected a HIP device tensor, got {t.device}; this package has no CPU path")
+        if t.dim() != 3 or 0 in t.shape:
+            raise RuntimeError(f"attention {name}: expected [B, channels, T] without empty axes, got {tuple(t.shape)}")
+        if t.dtype != q.dtype or t.dtype not in (torch.float32, torch.bfloat16):
+            raise RuntimeError(f"attention {name}: expected float32 or bfloat16 for q, k and v alike, got {t.dtype}")
+        if t.device != q.device:
+            raise RuntimeError(f"attention {name}: on {t.device}, q on {q.device}")
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise RuntimeError(f"attention: {heads} query heads cannot share {kv_heads} key heads")
+    B, tk = q.shape[0], k.shape[2]
+    if q.shape[1] % heads or k.shape[1] != q.shape[1] // heads * kv_heads or v.shape[1] % kv_heads:
+        raise RuntimeError(f"attention: channels {q.shape[1]}, {k.shape[1]}, {v.shape[1]} do not fit {heads} query and "
+                           f"{kv_heads} key heads")
+    if k.shape[0] != B or v.shape[0] != B or v.shape[2] != tk:
+        raise RuntimeError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    if max(q.shape[1] // heads, v.shape[1] // kv_heads) > 128:
+        raise RuntimeError("attention: heads of up to 128 channels are supported")
+    if mask is not None:
+        if mask.dtype != torch.bool or tuple(mask.shape) != (B, tk) or mask.device != q.device:
+            raise RuntimeError(f"attention: mask must be a bool tensor of shape {(B, tk)} on {q.device}, got "
+                               f"{mask.dtype} {tuple(mask.shape)} on {mask.device}")
+        mask = mask.contiguous()
+    if bias is not None:
+        if bias.dtype not in (q.dtype, torch.float32):
+            raise RuntimeError(f"attention: table of {bias.dtype}, expected float32 or {q.dtype}")
+        _table_chk(bias, buckets, heads, q.device, "attention")
+        bias = bias.contiguous()
+    elif buckets is not None:
+        raise RuntimeError("attention: buckets without a table")
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias))
+    return _Attention.apply(_rows(q), _rows(k), _rows(v), bias, mask, (int(heads), int(kv_heads), float(scale), buckets),
+                            keep)
+
+
 # --------------------------------------------------------------------------------------- minibatch stddev
 # ``segments``: the batch is a concatenation of that many independent minibatches (e.g. reals and
 # fakes stacked into one critic pass); the group statistics never mix samples of two segments, so

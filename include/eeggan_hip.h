@@ -388,6 +388,58 @@ int eeggan_maxpool_select(const float* src, const unsigned char* idx, float* dst
 size_t eeggan_dot_workspace(void);
 int eeggan_dot(const float* a, const float* b, float* out, size_t n, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention over time without stored probabilities, with learned relative positions ---------------
+ * The products of SelfAttention (layers.py:56-64), for any number of heads, key masks and position biases:
+ *   S[s,t] = scale * sum_d k[d,s] q[d,t] + bias(s,t);  P = softmax over the attended s;  out[c,t] = sum_s v[c,s] P[s,t]
+ * q is [B, H Dk, Tq], k [B, KV Dk, Tk], v [B, KV Dv, Tk], channels-first with time contiguous; the sample and channel
+ * strides are given in elements.  H = KV * (query heads that share a key head): query head h reads key head h / (H / KV).
+ * mask: [B, Tk] bytes, zero = key not attended by any query of the sample (its k and v are never used, whatever they
+ * hold); NULL: all attended.  A query without any key to attend has a zero column in `out` and zero gradients.
+ * All of q, k, v, out and the gradients are float32 (products exact to float32 rounding) or, with bf16 = 1, bfloat16
+ * (P and dS are rounded to bfloat16 for their products; sums and statistics are float32).  Dk, Dv <= 128; any
+ * alignment of the elements' own size.
+ * Positions: query t lies at t, key s at step * s + offset; distance rel = step * s + offset - t.  table is
+ * [count, H], float32 or (table_bf16) bfloat16; bias(s,t) = table[bucket(rel), h].  Entries <= -1e30 bar their pairs. */
+typedef struct {
+    int count;         /* buckets: 2 .. 128 */
+    int bidirectional; /* 1: keys ahead of the query (rel > 0) take the second half of the buckets (count even);
+                          0: they count as distance 0 */
+    int step, offset;  /* position of key s: 1 <= step <= 16 */
+    int edges[64];     /* smallest distance of every bucket of one side, strictly increasing from 0, last one <= 1024;
+                          count / 2 (bidirectional) or count of them, at most 64 */
+} eeggan_buckets;
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_batch, q_channel, k_batch, k_channel, v_batch, v_channel; /* strides in elements */
+    const unsigned char* mask;
+    const void* table;             /* NULL: no position bias */
+    const eeggan_buckets* buckets; /* HOST pointer, read during the call */
+    int bf16, table_bf16;
+    int B, H, KV, Dk, Dv, Tq, Tk;
+    float scale;
+} eeggan_attention;
+/* out [B, H Dv, Tq]; lse [B, H, Tq] (float32, log2 of the softmax sums) and, for bfloat16, rest (like out: what the
+ * rounding of out left over, so that sum_c out dO, from which dS is subtracted, is formed from 16 bits instead of 8);
+ * both NULL when no backward pass follows, rest NULL for float32.
+ * workspace: device memory of the size the _workspace function returns (0 for a rejected descriptor). */
+size_t eeggan_attention_fwd_workspace(const eeggan_attention* a);
+int eeggan_attention_fwd(const eeggan_attention* a, void* out, void* rest, float* lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
+/* Gradients for the cotangent g of `out` (dense, like out): gq, gk, gv dense in their inputs' shapes and types,
+ * g_table [count, H] in the table's type (NULL: not wanted).  Sums over samples, queries and shared heads run in a
+ * fixed order: equal inputs give equal bits. */
+size_t eeggan_attention_bwd_workspace(const eeggan_attention* a, int want_table);
+int eeggan_attention_bwd(const eeggan_attention* a, const void* out, const void* rest, const float* lse, const void* g,
+                         void* gq, void* gk, void* gv, void* g_table, void* workspace, size_t workspace_bytes, void* stream);
+/* The same bias on stored scores [B * H, Tk, Tq] (float32): out = scores + table[bucket(rel), h]; scores NULL: the bias
+ * alone.  Its gradient: g_table[j, h] = sum over samples and pairs of bucket j of g (table and g_table float32).  Both
+ * are linear and each other's transposes. */
+int eeggan_relative_bias(const float* scores, const float* table, const eeggan_buckets* buckets, float* out, int B, int H,
+                         int Tk, int Tq, void* stream);
+size_t eeggan_relative_bias_grad_workspace(const eeggan_buckets* buckets, int B, int H, int Tk, int Tq);
+int eeggan_relative_bias_grad(const float* g, const eeggan_buckets* buckets, float* g_table, int B, int H, int Tk, int Tq,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 /* out[0] = scale * mean(v[0..n))  (generator loss -mean(d_fake): scale = -1). */
 int eeggan_mean_scale(const float* v, float* out, int n, float scale, void* stream);
 /* out[i] = gl[0] * scale / n  for i in [0,n): backward of eeggan_mean_scale. */
@@ -406,6 +458,20 @@ typedef struct {
 } eeggan_adam_tensor;
 int eeggan_adam_step(const eeggan_adam_tensor* table, int ntensors,
                      float lr, float beta1, float beta2, float eps, float grad_scale, void* stream);
+/* ---- global gradient norm and clipping ----------------------------------------------------------------
+ * norm[0] = |scale| * sqrt(sum over the table's tensors of g^2) (squares and sums in double, fixed order) and norm[1] =
+ * scale * min(1, max_norm / (norm[0] + 1e-6)), the multiplier that bounds scale * g; max_norm > 0, infinity: no bound.
+ * Of the table only g and n are read.  norm: two floats of device memory; workspace: device memory, 8-byte aligned, of
+ * the size the _workspace function returns (0 for a rejected table). */
+size_t eeggan_grad_norm_workspace(const eeggan_adam_tensor* table, int ntensors);
+int eeggan_grad_norm(const eeggan_adam_tensor* table, int ntensors, float scale, double max_norm, float* norm,
+                     void* workspace, size_t workspace_bytes, void* stream);
+/* g *= norm[1] in place for every tensor of the table (each listed once); a multiplier of exactly one touches nothing. */
+int eeggan_grad_scale(const eeggan_adam_tensor* table, int ntensors, const float* norm, void* stream);
+/* eeggan_adam_step on norm[1] * g, the multiplier read from device memory by the launch: clipped gradients are never
+ * written.  workspace: 8 bytes per tensor at least (the one of eeggan_grad_norm serves). */
+int eeggan_adam_step_clipped(const eeggan_adam_tensor* table, int ntensors, double lr, double beta1, double beta2,
+                             double eps, const float* norm, void* workspace, size_t workspace_bytes, void* stream);
 /* p[k] = g[k] for every tensor of the table (m, v, step unused): packs gradients into the slices
  * of one flat bucket for a single all-reduce. */
 int eeggan_multi_copy(const eeggan_adam_tensor* table, int ntensors, void* stream);
