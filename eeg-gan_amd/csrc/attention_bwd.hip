@@ -64,23 +64,30 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     float delta = 0.f;
     {
         const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc + t;
-        fq.fill(h, [&](int d) {
-            const float v = live && d < a.Dk ? ld1(q + d * a.qsc) : 0.f;
-            return NP == 3 ? v * c : v;
-        });
         const T* g = reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq + t;
         const T* o = reinterpret_cast<const T*>(a.out) + row * a.Dv * a.Tq + t;
-        const T* rest = reinterpret_cast<const T*>(a.rest) + row * a.Dv * a.Tq + t;
-        fg.fill(h, [&](int d) {
-            const bool ok = live && d < a.Dv;
-            const float v = ok ? ld1(g + (long long)d * a.Tq) : 0.f;
-            if (ok) {
-                float x = ld1(o + (long long)d * a.Tq);
-                if (NP == 1) x += ld1(rest + (long long)d * a.Tq);
-                delta = __builtin_fmaf(v, x, delta);
-            }
-            return v;
-        });
+        typedef SFrag<NP, DK> FK;
+        typedef SFrag<NP, DV> FV;
+        float x[FK::VALUES], y[FV::VALUES], z[FV::VALUES];
+        FK::read(q, a.qsc, a.Dk, h, x);
+        FV::read(g, a.Tq, a.Dv, h, y);
+        FV::read(o, a.Tq, a.Dv, h, z);
+        if constexpr (NP == 1) {
+            float w[FV::VALUES];
+            FV::read(reinterpret_cast<const T*>(a.rest) + row * a.Dv * a.Tq + t, a.Tq, a.Dv, h, w);
+#pragma unroll
+            for (int i = 0; i < FV::VALUES; ++i) z[i] += w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < FK::VALUES; ++i) x[i] = live && FK::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < FV::VALUES; ++i) {
+            const bool ok = live && FV::channel(i, h) < a.Dv;
+            y[i] = ok ? y[i] : 0.f;
+            delta = ok ? __builtin_fmaf(y[i], z[i], delta) : delta;
+        }
+        fq.fill(h, x);
+        fg.fill(h, y);
         delta = half_sum(delta);
         if (inside && h == 0) a.delta[row * a.Tq + t] = delta;
     }
@@ -105,25 +112,24 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
 
     Block<T, DK, XT> kblk;
     Block<T, DV, XT> vblk;
-    unsigned long long word64 = 0;
+    Steps<XT> ahead;
     auto fetch = [&](int s0) {
-        kblk.load(kb, a.ksc, a.Dk, s0, a.Tk, mask, tid);
-        vblk.load(vb, a.vsc, a.Dv, s0, a.Tk, mask, tid);
-        const int s = s0 + lane;
-        word64 = __ballot(lane < XT && s < a.Tk && (!mask || mask[s]));
+        kblk.load(kb, a.ksc, a.Dk, s0, a.Tk, tid);
+        vblk.load(vb, a.vsc, a.Dv, s0, a.Tk, tid);
+        ahead.find(s0, a.Tk, mask, lane);
     };
     fetch(0);
     for (int s0 = 0; s0 < a.Tk; s0 += XT) {
         __syncthreads();
-        kblk.template store<true, true>(kt, kn, mask != nullptr, tid);
-        vblk.template store<true, false>(vt, nullptr, mask != nullptr, tid);
-        const unsigned long long now = word64;
+        const Steps<XT> now = ahead;
+        kblk.template store<true, true>(kt, kn, a.Dk, now, tid);
+        vblk.template store<true, false>(vt, nullptr, a.Dv, now, tid);
         __syncthreads();
         if (s0 + XT < a.Tk) fetch(s0 + XT);
 #pragma unroll
         for (int u = 0; u < XT / 32; ++u) {
             const int x0 = 32 * u;
-            const unsigned word = (unsigned)(now >> x0);
+            const unsigned word = now.tile(x0);
             if (word == 0) continue;
             const int s = s0 + x0;
             f32x16 acc;
@@ -135,12 +141,10 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[r] = bias;
                 } else {
-                    const float* r0 = rel + (long long)a.pos.step * (s + 4 * h);
+                    const int first = min(s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
+                    const float* r0 = rel + (long long)a.pos.step * first;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = (r & 3) + 8 * (r >> 2);
-                        acc[r] = (s + 4 * h + i < a.Tk ? r0[a.pos.step * i] : 0.f) - lse;
-                    }
+                    for (int r = 0; r < 16; ++r) acc[r] = r0[a.pos.step * min((r & 3) + 8 * (r >> 2), last)] - lse;
                 }
             } else {
 #pragma unroll
@@ -254,12 +258,18 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     SFrag<NP, DV> fv;
     {
         const T* k = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc + (live ? s : 0);
-        fk.fill(h, [&](int d) {
-            const float v = live && d < a.Dk ? ld1(k + d * a.ksc) : 0.f;
-            return NP == 3 ? v * c : v;
-        });
         const T* v = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc + (live ? s : 0);
-        fv.fill(h, [&](int d) { return live && d < a.Dv ? ld1(v + d * a.vsc) : 0.f; });
+        typedef SFrag<NP, DK> FK;
+        typedef SFrag<NP, DV> FV;
+        float x[FK::VALUES], y[FV::VALUES];
+        FK::read(k, a.ksc, a.Dk, h, x);
+        FV::read(v, a.vsc, a.Dv, h, y);
+#pragma unroll
+        for (int i = 0; i < FK::VALUES; ++i) x[i] = live && FK::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < FV::VALUES; ++i) y[i] = live && FV::channel(i, h) < a.Dv ? y[i] : 0.f;
+        fk.fill(h, x);
+        fv.fill(h, y);
     }
     f32x16 dk[QN::GROUPS], dv[GN::GROUPS];
 #pragma unroll
@@ -274,24 +284,27 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     Block<T, DK, XT> qblk;
     Block<T, DV, XT> gblk;
     float stat = 0.f;
+    Steps<XT> ahead;
     auto fetch = [&](int stage) {
         const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
         const int head = kvh * a.G + g;
         const long long row = (long long)b * H + head;
         qblk.load(reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc, a.qsc, a.Dk, t0, a.Tq,
-                  nullptr, tid);
-        gblk.load(reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq, a.Tq, a.Dv, t0, a.Tq, nullptr, tid);
+                  tid);
+        gblk.load(reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq, a.Tq, a.Dv, t0, a.Tq, tid);
+        ahead.find(t0, a.Tq, nullptr, lane);
         if (tid < 2 * XT) {
             const int t = t0 + tid % XT;
             const float* p = (tid < XT ? a.lse : a.delta) + row * a.Tq;
-            stat = t < a.Tq ? -p[t] : tid < XT ? -INFINITY : 0.f;
+            const float x = -p[min(t, a.Tq - 1)];
+            stat = t < a.Tq ? x : tid < XT ? -INFINITY : 0.f;
         }
     };
     if (first < last) fetch(first);
     for (int stage = first; stage < last; ++stage) {
         __syncthreads();
-        qblk.template store<true, true>(qt, qn, false, tid);
-        gblk.template store<true, true>(gt, gn, false, tid);
+        qblk.template store<true, true>(qt, qn, a.Dk, ahead, tid);
+        gblk.template store<true, true>(gt, gn, a.Dv, ahead, tid);
         if (tid < 2 * XT) stats[tid] = stat;
         __syncthreads();
         if (stage + 1 < last) fetch(stage + 1);
@@ -322,10 +335,7 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
                     for (int r = 0; r < 16; ++r) acc[r] += bias;
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = acc_row(r, h);
-                        acc[r] += t + i < a.Tq ? r0[-i] : 0.f;
-                    }
+                    for (int r = 0; r < 16; ++r) acc[r] += r0[-min(acc_row(r, h), a.Tq - 1 - t)];
                 }
             }
             const f32x16 raw = mma_scores<NP, DK, XT>(qt + (x0 + l31) * QT::RS, h, fk, zero16());

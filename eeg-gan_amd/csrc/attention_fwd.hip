@@ -62,10 +62,12 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
     {
         const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc + t;
         // (float32: the scale goes into the split operand; bfloat16 operands stay exact and the scores are scaled)
-        fq.fill(h, [&](int d) {
-            const float v = live && d < a.Dk ? ld1(q + d * a.qsc) : 0.f;
-            return NP == 3 ? v * c : v;
-        });
+        typedef SFrag<NP, DK> F;
+        float x[F::VALUES];
+        F::read(q, a.qsc, a.Dk, h, x);
+#pragma unroll
+        for (int i = 0; i < F::VALUES; ++i) x[i] = live && F::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
+        fq.fill(h, x);
     }
     const T* const kb = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc;
     const T* const vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc;
@@ -87,32 +89,25 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
 
     Block<T, DK, XT> kblk;
     Block<T, DV, XT> vblk;
-    unsigned long long words[(XT + 63) / 64];  // which keys of the stage are attended
+    Steps<XT> ahead;  // which keys of the stage are attended
     auto fetch = [&](int s0) {
-        kblk.load(kb, a.ksc, a.Dk, s0, s_end, mask, tid);
-        vblk.load(vb, a.vsc, a.Dv, s0, s_end, mask, tid);
-#pragma unroll
-        for (int i = 0; i < (XT + 63) / 64; ++i) {
-            const int s = s0 + 64 * i + lane;
-            words[i] = __ballot(64 * i + lane < XT && s < s_end && (!mask || mask[s]));
-        }
+        kblk.load(kb, a.ksc, a.Dk, s0, s_end, tid);
+        vblk.load(vb, a.vsc, a.Dv, s0, s_end, tid);
+        ahead.find(s0, s_end, mask, lane);
     };
     if (s_begin < s_end) fetch(s_begin);
     for (int s0 = s_begin; s0 < s_end; s0 += XT) {
         __syncthreads();
-        kblk.template store<true, false>(kt, nullptr, mask != nullptr, tid);
-        vblk.template store<false, true>(nullptr, vt, mask != nullptr, tid);
-        unsigned long long now[(XT + 63) / 64];
-#pragma unroll
-        for (int i = 0; i < (XT + 63) / 64; ++i) now[i] = words[i];
+        const Steps<XT> now = ahead;
+        kblk.template store<true, false>(kt, nullptr, a.Dk, now, tid);
+        vblk.template store<false, true>(nullptr, vt, a.Dv, now, tid);
         __syncthreads();
         if (s0 + XT < s_end) fetch(s0 + XT);
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {
             const int sub = KW == 1 ? u : ksub;
             const int x0 = 32 * sub;
-            unsigned word = (unsigned)(now[0] >> (x0 & 32));
-            if (XT > 64 && x0 >= 64) word = (unsigned)(now[(XT + 63) / 64 - 1] >> (x0 & 32));
+            const unsigned word = now.tile(x0);
             if (word == 0) continue;  // (the same for every lane of the wave)
             f32x16 acc;
             if constexpr (BIAS) {
@@ -122,11 +117,12 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[r] = cinit[r] + bias;
                 } else {
-                    const float* r0 = rel + a.pos.step * (s + 4 * h);
+                    const int first = min((int)s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
+                    const float* r0 = rel + (long long)a.pos.step * first;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int i = (r & 3) + 8 * (r >> 2);
-                        acc[r] = cinit[r] + (s + 4 * h + i < a.Tk ? r0[a.pos.step * i] : 0.f);
+                        acc[r] = cinit[r] + r0[a.pos.step * min(i, last)];
                     }
                 }
             } else {

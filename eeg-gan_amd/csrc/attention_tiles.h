@@ -47,19 +47,14 @@ __device__ __forceinline__ u32x2 load4(const __bf16* p) {
     o[1] = v[1];
     return o;
 }
-// the first n (1 .. 3) of four values, the rest zero
-__device__ __forceinline__ f32x4 load_few(const float* p, int n) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    v[0] = p[0];
-    if (n > 1) v[1] = p[1];
-    if (n > 2) v[2] = p[2];
+__device__ __forceinline__ f32x4 gather4(const float* p, int i0, int i1, int i2, int i3) {
+    const f32x4 v = {p[i0], p[i1], p[i2], p[i3]};
     return v;
 }
-__device__ __forceinline__ u32x2 load_few(const __bf16* q, int n) {
+__device__ __forceinline__ u32x2 gather4(const __bf16* q, int i0, int i1, int i2, int i3) {
     const unsigned short* p = reinterpret_cast<const unsigned short*>(q);
-    u32x2 v = {p[0], 0u};
-    if (n > 1) v[0] |= (unsigned)p[1] << 16;
-    if (n > 2) v[1] = p[2];
+    const unsigned a = p[i0], b = p[i1], c = p[i2], d = p[i3];
+    const u32x2 v = {a | b << 16, c | d << 16};
     return v;
 }
 
@@ -95,9 +90,27 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// the two lane halves' values combined
-__device__ __forceinline__ float half_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
-__device__ __forceinline__ float half_sum(float v) { return v + __shfl_xor(v, 32, 64); }
+// The two lane halves' values combined: one exchange of register halves, no trip through LDS.  (The second operand is
+// hidden from the compiler: given the same value twice, it takes both results for one.)
+__device__ __forceinline__ void halves(float v, float& lo, float& hi) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    unsigned w = u;
+    asm("" : "+v"(w));
+    const auto r = __builtin_amdgcn_permlane32_swap(u, w, false, false);
+    const unsigned a = r[0], b = r[1];
+    lo = __builtin_bit_cast(float, a);
+    hi = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float half_max(float v) {
+    float lo, hi;
+    halves(v, lo, hi);
+    return fmaxf(lo, hi);
+}
+__device__ __forceinline__ float half_sum(float v) {
+    float lo, hi;
+    halves(v, lo, hi);
+    return lo + hi;
+}
 
 // ---- tiles --------------------------------------------------------------------------------------------------
 // Eight channels in three pieces: the pieces share the reduction axis (see SFrag), one row holds all of them.
@@ -124,81 +137,96 @@ struct NTile {
 // byte offset of time index x (a multiple of 4) in a row of an N tile
 __device__ __forceinline__ int n_off(int x) { return 2 * ((x & ~31) + (x & 16) + ((x & 4) << 1) + ((x & 8) >> 1)); }
 
+// Which steps of a stage count, one bit each (the same in every lane).
+template <int XT>
+struct Steps {
+    unsigned long long w[(XT + 63) / 64];
+    // steps [x0, x0 + XT) of `len`, less the masked ones (mask: nonzero bytes count; null: all)
+    __device__ __forceinline__ void find(int x0, int len, const unsigned char* mask, int lane) {
+#pragma unroll
+        for (int i = 0; i < (XT + 63) / 64; ++i) {
+            const int x = x0 + 64 * i + lane;
+            const bool in = 64 * i + lane < XT && x < len;
+            w[i] = __ballot(mask ? in && mask[x < len ? x : len - 1] : in);
+        }
+    }
+    __device__ __forceinline__ bool all() const {
+        bool a = true;
+#pragma unroll
+        for (int i = 0; i < (XT + 63) / 64; ++i) a = a && w[i] == (XT >= 64 ? ~0ull : (1ull << (XT & 63)) - 1);
+        return a;
+    }
+    __device__ __forceinline__ unsigned tile(int x0) const {  // the 32 steps from x0
+        return (unsigned)(w[XT > 64 && x0 >= 64 ? (XT + 63) / 64 - 1 : 0] >> (x0 & 32));
+    }
+    __device__ __forceinline__ unsigned quad(int kq) const {  // the four steps from 4 kq
+        return (unsigned)((XT > 64 && kq >= 16 ? w[(XT + 63) / 64 - 1] : w[0]) >> (4 * (kq & 15))) & 15u;
+    }
+};
+
 // A [D, XT] block of a channels-first matrix on its way from memory into LDS: 4 x 4 units (four channels, four time
-// steps), neighbouring threads on neighbouring steps.  Units past the matrix are zero, and so are masked steps: what
-// lies there (NaN included) never meets a product.
+// steps), neighbouring threads on neighbouring steps.  Loads never branch (the compiler would wait at every join):
+// whatever lies past the matrix is read at its last row or step.  Such values and those of masked steps become zeros on
+// their way into LDS, so what they hold (NaN included) never meets a product.
 template <class T, int D, int XT>
 struct Block {
     static constexpr int NP = Elem<T>::NP;
     static constexpr int XQ = XT / 4, UNITS = (D / 4) * XQ, U = (UNITS + THREADS - 1) / THREADS;
     typename Elem<T>::raw4 r[U][4];
-    unsigned keep[U];
 
-    // base: channel 0, step 0 of the head; steps [x0, x0 + XT) of `len`; mask: this sample's key mask or null
-    __device__ __forceinline__ void load(const T* base, long long stride, int channels, int x0, int len,
-                                         const unsigned char* mask, int tid) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int unit = tid + THREADS * u;
-            const int kq = unit % XQ, db = unit / XQ;
-            const int x = x0 + 4 * kq;
-            const T* p = base + (long long)(4 * db) * stride + x;
-            const bool in = UNITS % THREADS == 0 || unit < UNITS;
-            keep[u] = 0x01010101u;
-            if (mask && in && x < len) {
-                if (x + 3 < len) {
-                    typedef unsigned int u32u __attribute__((aligned(1)));
-                    keep[u] = *reinterpret_cast<const u32u*>(mask + x);
-                } else {
-                    keep[u] = mask[x] | (x + 1 < len ? (unsigned)mask[x + 1] << 8 : 0u) |
-                              (x + 2 < len ? (unsigned)mask[x + 2] << 16 : 0u);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                typename Elem<T>::raw4 z = {};
-                r[u][i] = z;
-                if (in && 4 * db + i < channels) {
-                    if (x + 3 < len) r[u][i] = load4(p + i * stride);
-                    else if (x < len) r[u][i] = load_few(p + i * stride, len - x);
-                }
-            }
-        }
-    }
-
-    // WT / WN: write the T tile / the N tile
-    template <bool WT, bool WN>
-    __device__ __forceinline__ void store(char* tt, char* nt, bool masked, int tid) {
-        typedef TTile<NP, D, XT> TL;
-        typedef NTile<NP, D, XT> NL;
+    // base: channel 0, step 0 of the head; steps [x0, x0 + XT) of `len`
+    __device__ __forceinline__ void load(const T* base, long long stride, int channels, int x0, int len, int tid) {
+        const bool whole = x0 + XT <= len;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int unit = tid + THREADS * u;
             if (UNITS % THREADS != 0 && unit >= UNITS) continue;
             const int kq = unit % XQ, db = unit / XQ;
+            const int x = x0 + 4 * kq, last = len - 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const T* p = base + (long long)min(4 * db + i, channels - 1) * stride;
+                if (whole) r[u][i] = load4(p + x);
+                else r[u][i] = gather4(p, min(x, last), min(x + 1, last), min(x + 2, last), min(x + 3, last));
+            }
+        }
+    }
+
+    // WT / WN: write the T tile / the N tile.  steps: which count.
+    template <bool WT, bool WN>
+    __device__ __forceinline__ void store(char* tt, char* nt, int channels, const Steps<XT>& steps, int tid) {
+        typedef TTile<NP, D, XT> TL;
+        typedef NTile<NP, D, XT> NL;
+        const bool clean = steps.all() && channels == D;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int unit = tid + THREADS * u;
+            if (UNITS % THREADS != 0 && unit >= UNITS) continue;
+            const int kq = unit % XQ, db = unit / XQ;
+            if (!clean) {
+                const unsigned keep = steps.quad(kq);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned k = 4 * db + i < channels ? keep : 0u;
+                    if constexpr (NP == 3) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) r[u][i][e] = (k >> e) & 1u ? r[u][i][e] : 0.f;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            r[u][i][e] &= ((k >> (2 * e)) & 1u ? 0xffffu : 0u) | ((k >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+                    }
+                }
+            }
             unsigned w[4][2][NP];  // [channel][pair of steps][piece]
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (NP == 3) {
-                    f32x4 v = r[u][i];
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = (keep[u] >> (8 * e)) & 0xffu ? v[e] : 0.f;
-                    }
-                    pieces2<NP>(v[0], v[1], w[i][0]);
-                    pieces2<NP>(v[2], v[3], w[i][1]);
+                    pieces2<NP>(r[u][i][0], r[u][i][1], w[i][0]);
+                    pieces2<NP>(r[u][i][2], r[u][i][3], w[i][1]);
                 } else {
-                    u32x2 v = r[u][i];
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const unsigned lo = (keep[u] >> (16 * e)) & 0xffu ? 0xffffu : 0u;
-                            const unsigned hi = (keep[u] >> (16 * e + 8)) & 0xffu ? 0xffff0000u : 0u;
-                            v[e] &= lo | hi;
-                        }
-                    }
-                    w[i][0][0] = v[0];
-                    w[i][1][0] = v[1];
+                    w[i][0][0] = r[u][i][0];
+                    w[i][1][0] = r[u][i][1];
                 }
             }
 #pragma unroll
@@ -235,15 +263,24 @@ struct SFrag {
     static constexpr int N = packed8<NP, D>() ? 2 : NP * D / 16;
     bf16x8 f[N];
 
-    // value(d) -> the (already scaled) value of channel d, zero past the matrix
-    template <class F>
-    __device__ __forceinline__ void fill(int h, F value) {
+    static constexpr int VALUES = packed8<NP, D>() ? 8 : D / 2;  // channels of a lane (half)
+    static __device__ __forceinline__ int channel(int i, int h) {
+        return packed8<NP, D>() ? i : 16 * (i / 8) + 8 * h + i % 8;
+    }
+    // the lane's channels of a column (p: channel 0 of it); past the matrix the last channel again, to be zeroed
+    template <class T>
+    static __device__ __forceinline__ void read(const T* p, long long stride, int channels, int h, float (&v)[VALUES]) {
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) v[i] = ld1(p + (long long)min(channel(i, h), channels - 1) * stride);
+    }
+    // v: the (already scaled) values, zero past the matrix
+    __device__ __forceinline__ void fill(int h, const float (&v)[VALUES]) {
         if constexpr (packed8<NP, D>()) {
             u32x4 w0, w1, w2;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 unsigned w[3];
-                pieces2<3>(value(2 * i), value(2 * i + 1), w);
+                pieces2<3>(v[2 * i], v[2 * i + 1], w);
                 w0[i] = w[0];
                 w1[i] = w[1];
                 w2[i] = w[2];
@@ -257,8 +294,7 @@ struct SFrag {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     unsigned w[NP];
-                    const int d = 16 * j + 8 * h + 2 * i;
-                    pieces2<NP>(value(d), value(d + 1), w);
+                    pieces2<NP>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1], w);
 #pragma unroll
                     for (int p = 0; p < NP; ++p) ws[p][i] = w[p];
                 }

@@ -8,6 +8,15 @@ namespace {
 
 constexpr int MAX_T = 1 << 27;  // time steps of one call
 
+// the first n (1 .. 3) of four values, the rest zero
+__device__ __forceinline__ f32x4 load_few(const float* p, int n) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    v[0] = p[0];
+    if (n > 1) v[1] = p[1];
+    if (n > 2) v[2] = p[2];
+    return v;
+}
+
 // rel[head][i] = log2(e) * table[bucket(first + i)][head]; entries at or below -1e30 (a mask written into the table, the
 // type's lowest value among them) bar the pair.
 template <class T>
