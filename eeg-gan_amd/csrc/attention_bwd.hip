@@ -32,23 +32,29 @@ struct BwdArgs {
     float scale;
 };
 
+template <class T, int DK, int DV, int XT>
+struct DqCut {
+    static constexpr int NP = Elem<T>::NP;
+    static constexpr int STAGE = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES + TTile<NP, DV, XT>::BYTES;
+    static constexpr int BUFS = 2 * STAGE <= 64 * 1024 ? 2 : 1;  // (two workgroups to a CU, with room for histograms)
+    static constexpr int LDS = BUFS * STAGE;
+};
 template <class T, int DK, int DV, int XT, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
+    typedef DqCut<T, DK, DV, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     typedef TTile<NP, DK, XT> KT;
     typedef NTile<NP, DK, XT> KN;
     typedef TTile<NP, DV, XT> VT;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char* const kt = smem;
-    char* const kn = kt + KT::BYTES;
-    char* const vt = kn + KN::BYTES;
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tile = blockIdx.x % a.coltiles;
-    const int bh = blockIdx.x / a.coltiles;
     const int H = a.KV * a.G;
-    const int b = bh / H, head = bh - b * H, kvh = head / a.G;
+    int group, part_of;
+    place(blockIdx.x, a.B * a.KV, a.G * a.coltiles, group, part_of);
+    const int b = group / a.KV, kvh = group - b * a.KV;
+    const int tile = part_of % a.coltiles, head = kvh * a.G + part_of / a.coltiles;
 
     const int t0 = (tile * 4 + wave) * 32;
     const bool inside = t0 + l31 < a.Tq;
@@ -59,8 +65,8 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     if (!live) lse = INFINITY;
 
     const float c = a.scale * LOG2E;
-    SFrag<NP, DK> fq;
-    SFrag<NP, DV> fg;
+    SFrag<NP, DK> fq[1];
+    SFrag<NP, DV> fg[1];
     float delta = 0.f;
     {
         const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc + t;
@@ -86,8 +92,8 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
             y[i] = ok ? y[i] : 0.f;
             delta = ok ? __builtin_fmaf(y[i], z[i], delta) : delta;
         }
-        fq.fill(h, x);
-        fg.fill(h, y);
+        fq[0].fill(h, x);
+        fg[0].fill(h, y);
         delta = half_sum(delta);
         if (inside && h == 0) a.delta[row * a.Tq + t] = delta;
     }
@@ -99,12 +105,12 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     f32x16 dinit;
 #pragma unroll
     for (int r = 0; r < 16; ++r) dinit[r] = -delta;
-    f32x16 dq[KN::GROUPS];
+    f32x16 dq[1][KN::GROUPS];
 #pragma unroll
-    for (int i = 0; i < KN::GROUPS; ++i) dq[i] = zero16();
+    for (int i = 0; i < KN::GROUPS; ++i) dq[0][i] = zero16();
 
     double beyond[2] = {0.0, 0.0};  // sums of dS over far tiles, behind / ahead of the query (thousands of terms)
-    float* const hist = BIAS ? reinterpret_cast<float*>(vt + VT::BYTES) + wave * a.nhist : nullptr;
+    float* const hist = BIAS ? reinterpret_cast<float*>(smem + Cut::LDS) + wave * a.nhist : nullptr;
     const bool want = BIAS && a.hist != nullptr;
     const int width = a.nhist / 2;  // (distances -width .. width)
     if (want)
@@ -112,20 +118,34 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
 
     Block<T, DK, XT> kblk;
     Block<T, DV, XT> vblk;
-    Steps<XT> ahead;
+    kblk.init(a.ksc, a.Dk, tid);
+    vblk.init(a.vsc, a.Dv, tid);
+    Steps<XT> ahead, now;
     auto fetch = [&](int s0) {
-        kblk.load(kb, a.ksc, a.Dk, s0, a.Tk, tid);
-        vblk.load(vb, a.vsc, a.Dv, s0, a.Tk, tid);
+        kblk.load(kb, s0, a.Tk, tid);
+        vblk.load(vb, s0, a.Tk, tid);
         ahead.find(s0, a.Tk, mask, lane);
     };
+    auto put = [&](int buf) {
+        char* const kt = smem + buf * Cut::STAGE;
+        kblk.template store<true, true>(kt, kt + KT::BYTES, a.Dk, ahead, tid);
+        vblk.template store<true, false>(kt + KT::BYTES + KN::BYTES, nullptr, a.Dv, ahead, tid);
+    };
+    int buf = 0;
     fetch(0);
+    put(0);
+    now = ahead;
+    if (XT < a.Tk) fetch(XT);
+    __syncthreads();
     for (int s0 = 0; s0 < a.Tk; s0 += XT) {
-        __syncthreads();
-        const Steps<XT> now = ahead;
-        kblk.template store<true, true>(kt, kn, a.Dk, now, tid);
-        vblk.template store<true, false>(vt, nullptr, a.Dv, now, tid);
-        __syncthreads();
-        if (s0 + XT < a.Tk) fetch(s0 + XT);
+        const Steps<XT> next = ahead;
+        if (Cut::BUFS == 2 && s0 + XT < a.Tk) {
+            put(buf ^ 1);
+            if (s0 + 2 * XT < a.Tk) fetch(s0 + 2 * XT);
+        }
+        const char* const kt = smem + buf * Cut::STAGE;
+        const char* const kn = kt + KT::BYTES;
+        const char* const vt = kn + KN::BYTES;
 #pragma unroll
         for (int u = 0; u < XT / 32; ++u) {
             const int x0 = 32 * u;
@@ -152,15 +172,17 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
             }
             // (the scores accumulate from zero and meet lse once: on top of -lse every partial sum would be rounded at
             // its magnitude)
-            const f32x16 raw = mma_scores<NP, DK, XT>(kt + (x0 + l31) * KT::RS, h, fq, zero16());
+            f32x16 raw[1] = {zero16()}, dsv[1] = {dinit};
+            mma_scores<NP, DK, XT, 1>(kt + (x0 + l31) * KT::RS, h, fq, raw);
+            mma_scores<NP, DV, XT, 1>(vt + (x0 + l31) * VT::RS, h, fg, dsv);
+            f32x16& ds = dsv[0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[r] + acc[r] : __builtin_fmaf(raw[r], c, acc[r]);
+            for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[0][r] + acc[r] : __builtin_fmaf(raw[0][r], c, acc[r]);
             if (word != 0xffffffffu) {
                 const unsigned w = word >> (4 * h);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[r] = (w >> ((r & 3) + 8 * (r >> 2))) & 1u ? acc[r] : -INFINITY;
             }
-            f32x16 ds = mma_scores<NP, DV, XT>(vt + (x0 + l31) * VT::RS, h, fg, dinit);
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(acc[r]);
             if constexpr (BIAS) {
@@ -186,27 +208,38 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
                     }
                 }
             }
-            PFrag<NP> p;
-            p.fill(ds);
-            mma_values<NP, DK, XT>(kn, x0, l31, h, p, dq);
+            PFrag<NP> p[1];
+            p[0].fill(ds);
+            mma_values<NP, DK, XT, 1>(kn, x0, l31, h, p, dq);
+        }
+        if (s0 + XT < a.Tk) {
+            __syncthreads();
+            if (Cut::BUFS == 1) {
+                put(0);
+                if (s0 + 2 * XT < a.Tk) fetch(s0 + 2 * XT);
+                __syncthreads();
+            } else {
+                buf ^= 1;
+            }
+            now = next;
         }
     }
     if (inside) {
-        eight_rows<NP, DK>(dq[0]);
+        eight_rows<NP, DK>(dq[0][0]);
         T* out = reinterpret_cast<T*>(a.gq) + row * a.Dk * a.Tq + t;
 #pragma unroll
         for (int i = 0; i < KN::GROUPS; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * i + acc_row(r, h);
-                if (d < a.Dk && (!KN::P8 || r < 4)) st1(out + (long long)d * a.Tq, live ? dq[i][r] * a.scale : 0.f);
+                if (d < a.Dk && (!KN::P8 || r < 4)) st1(out + (long long)d * a.Tq, live ? dq[0][i][r] * a.scale : 0.f);
             }
     }
     if constexpr (BIAS) {
         if (want) {
             float* const part = a.hist + ((long long)head * a.B * a.coltiles + (long long)b * a.coltiles + tile) * (a.nhist + 2);
             __syncthreads();
-            const float* const all = reinterpret_cast<const float*>(vt + VT::BYTES);
+            const float* const all = reinterpret_cast<const float*>(smem + Cut::LDS);
             for (int i = tid; i < a.nhist; i += THREADS)
                 part[i] = (all[i] + all[a.nhist + i]) + (all[2 * a.nhist + i] + all[3 * a.nhist + i]);
             float* const sums = reinterpret_cast<float*>(smem);
@@ -222,8 +255,19 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
 }
 
 // WK waves along the keys, WT = 4 / WK along the queries of a stage (their sums are joined through LDS at the end).
+template <class T, int DK, int DV, int WK, int XT>
+struct DkvCut {
+    static constexpr int NP = Elem<T>::NP;
+    static constexpr int Q = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES;
+    static constexpr int STAGE = Q + TTile<NP, DV, XT>::BYTES + NTile<NP, DV, XT>::BYTES + 2 * XT * (int)sizeof(float);
+    static constexpr int BUFS = 2 * STAGE <= 80 * 1024 ? 2 : 1;
+    static constexpr int WORDS = (NTile<NP, DK, XT>::GROUPS + NTile<NP, DV, XT>::GROUPS) * 16 * 64;  // a wave's sums
+    static constexpr int JOIN = (4 / WK - 1) * WK * WORDS * (int)sizeof(float);
+    static constexpr int LDS = BUFS * STAGE > JOIN ? BUFS * STAGE : JOIN;
+};
 template <class T, int DK, int DV, int WK, int XT, bool BIAS>
 __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 2) void attn_dkv_kernel(BwdArgs a) {
+    typedef DkvCut<T, DK, DV, WK, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     constexpr int WT = 4 / WK, SUBS = XT / (32 * WT);
     typedef TTile<NP, DK, XT> QT;
@@ -231,20 +275,14 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     typedef TTile<NP, DV, XT> GT;
     typedef NTile<NP, DV, XT> GN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char* const qt = smem;
-    char* const qn = qt + QT::BYTES;
-    char* const gt = qn + QN::BYTES;
-    char* const gn = gt + GT::BYTES;
-    float* const stats = reinterpret_cast<float*>(gn + GN::BYTES);  // -lse, then -delta, of the stage's queries
+    // a stage: q transposed and as it is, dO likewise, then -lse and -delta of its queries
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wk = wave % WK, wt = wave / WK;
-    int blk = blockIdx.x;
-    const int tile = blk % a.coltiles;
-    blk /= a.coltiles;
-    const int split = blk % a.nsplit;
-    const int bkv = blk / a.nsplit;
+    int bkv, part;
+    place(blockIdx.x, a.B * a.KV, a.coltiles * a.nsplit, bkv, part);
+    const int tile = part % a.coltiles, split = part / a.coltiles;
     const int b = bkv / a.KV, kvh = bkv - b * a.KV;
     const int H = a.KV * a.G;
 
@@ -254,8 +292,8 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     const bool live = inside && (!a.mask || a.mask[(long long)b * a.Tk + s]);
 
     const float c = a.scale * LOG2E;
-    SFrag<NP, DK> fk;
-    SFrag<NP, DV> fv;
+    SFrag<NP, DK> fk[1];
+    SFrag<NP, DV> fv[1];
     {
         const T* k = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc + (live ? s : 0);
         const T* v = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc + (live ? s : 0);
@@ -268,14 +306,14 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
         for (int i = 0; i < FK::VALUES; ++i) x[i] = live && FK::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
 #pragma unroll
         for (int i = 0; i < FV::VALUES; ++i) y[i] = live && FV::channel(i, h) < a.Dv ? y[i] : 0.f;
-        fk.fill(h, x);
-        fv.fill(h, y);
+        fk[0].fill(h, x);
+        fv[0].fill(h, y);
     }
-    f32x16 dk[QN::GROUPS], dv[GN::GROUPS];
+    f32x16 dk[1][QN::GROUPS], dv[1][GN::GROUPS];
 #pragma unroll
-    for (int i = 0; i < QN::GROUPS; ++i) dk[i] = zero16();
+    for (int i = 0; i < QN::GROUPS; ++i) dk[0][i] = zero16();
 #pragma unroll
-    for (int i = 0; i < GN::GROUPS; ++i) dv[i] = zero16();
+    for (int i = 0; i < GN::GROUPS; ++i) dv[0][i] = zero16();
 
     const int per_head = (a.Tq + XT - 1) / XT;
     const int stages = a.G * per_head;
@@ -283,15 +321,16 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
 
     Block<T, DK, XT> qblk;
     Block<T, DV, XT> gblk;
+    qblk.init(a.qsc, a.Dk, tid);
+    gblk.init(a.Tq, a.Dv, tid);
     float stat = 0.f;
     Steps<XT> ahead;
     auto fetch = [&](int stage) {
         const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
         const int head = kvh * a.G + g;
         const long long row = (long long)b * H + head;
-        qblk.load(reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc, a.qsc, a.Dk, t0, a.Tq,
-                  tid);
-        gblk.load(reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq, a.Tq, a.Dv, t0, a.Tq, tid);
+        qblk.load(reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc, t0, a.Tq, tid);
+        gblk.load(reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq, t0, a.Tq, tid);
         ahead.find(t0, a.Tq, nullptr, lane);
         if (tid < 2 * XT) {
             const int t = t0 + tid % XT;
@@ -300,14 +339,30 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
             stat = t < a.Tq ? x : tid < XT ? -INFINITY : 0.f;
         }
     };
-    if (first < last) fetch(first);
+    auto put = [&](int buf) {
+        char* const qt = smem + buf * Cut::STAGE;
+        char* const gt = qt + Cut::Q;
+        qblk.template store<true, true>(qt, qt + QT::BYTES, a.Dk, ahead, tid);
+        gblk.template store<true, true>(gt, gt + GT::BYTES, a.Dv, ahead, tid);
+        if (tid < 2 * XT) reinterpret_cast<float*>(gt + GT::BYTES + GN::BYTES)[tid] = stat;
+    };
+    int buf = 0;
+    if (first < last) {
+        fetch(first);
+        put(0);
+        if (first + 1 < last) fetch(first + 1);
+        __syncthreads();
+    }
     for (int stage = first; stage < last; ++stage) {
-        __syncthreads();
-        qblk.template store<true, true>(qt, qn, a.Dk, ahead, tid);
-        gblk.template store<true, true>(gt, gn, a.Dv, ahead, tid);
-        if (tid < 2 * XT) stats[tid] = stat;
-        __syncthreads();
-        if (stage + 1 < last) fetch(stage + 1);
+        if (Cut::BUFS == 2 && stage + 1 < last) {
+            put(buf ^ 1);
+            if (stage + 2 < last) fetch(stage + 2);
+        }
+        const char* const qt = smem + buf * Cut::STAGE;
+        const char* const qn = qt + QT::BYTES;
+        const char* const gt = qt + Cut::Q;
+        const char* const gn = gt + GT::BYTES;
+        const float* const stats = reinterpret_cast<const float*>(gn + GN::BYTES);
         const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
         const float* rel = nullptr;
         if constexpr (BIAS) rel = a.pos.rel + (long long)(kvh * a.G + g) * a.pos.nrel + (a.Tq - 1);
@@ -315,7 +370,8 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
         for (int u = 0; u < SUBS; ++u) {
             const int x0 = 32 * (u * WT + wt);
             if (t0 + x0 >= a.Tq) continue;  // (the same for every lane of the wave)
-            f32x16 acc, ds;
+            f32x16 acc, raw[1] = {zero16()}, dsv[1];
+            f32x16& ds = dsv[0];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 e = *reinterpret_cast<const f32x4*>(stats + x0 + 8 * i + 4 * h);
@@ -338,24 +394,34 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
                     for (int r = 0; r < 16; ++r) acc[r] += r0[-min(acc_row(r, h), a.Tq - 1 - t)];
                 }
             }
-            const f32x16 raw = mma_scores<NP, DK, XT>(qt + (x0 + l31) * QT::RS, h, fk, zero16());
+            mma_scores<NP, DK, XT, 1>(qt + (x0 + l31) * QT::RS, h, fk, raw);
+            mma_scores<NP, DV, XT, 1>(gt + (x0 + l31) * GT::RS, h, fv, dsv);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[r] + acc[r] : __builtin_fmaf(raw[r], c, acc[r]);
+            for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[0][r] + acc[r] : __builtin_fmaf(raw[0][r], c, acc[r]);
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[r] = __builtin_amdgcn_exp2f(acc[r]);
-            ds = mma_scores<NP, DV, XT>(gt + (x0 + l31) * GT::RS, h, fv, ds);
+            PFrag<NP> p[1];
+            p[0].fill(acc);
+            mma_values<NP, DV, XT, 1>(gn, x0, l31, h, p, dv);
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] *= acc[r];
-            PFrag<NP> p;
-            p.fill(acc);
-            mma_values<NP, DV, XT>(gn, x0, l31, h, p, dv);
-            p.fill(ds);
-            mma_values<NP, DK, XT>(qn, x0, l31, h, p, dk);
+            p[0].fill(ds);
+            mma_values<NP, DK, XT, 1>(qn, x0, l31, h, p, dk);
+        }
+        if (stage + 1 < last) {
+            __syncthreads();
+            if (Cut::BUFS == 1) {
+                put(0);
+                if (stage + 2 < last) fetch(stage + 2);
+                __syncthreads();
+            } else {
+                buf ^= 1;
+            }
         }
     }
     if constexpr (WT > 1) {
         // the sums of the waves wt = 1 .. WT - 1 are added to those of wave wt = 0, in that order
-        constexpr int WORDS = (QN::GROUPS + GN::GROUPS) * 16 * 64;
+        constexpr int WORDS = Cut::WORDS;
         float* const buf = reinterpret_cast<float*>(smem);
         __syncthreads();
         if (wt > 0) {
@@ -363,9 +429,9 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
 #pragma unroll
-                for (int i = 0; i < QN::GROUPS; ++i) mine[(16 * i + r) * 64] = dk[i][r];
+                for (int i = 0; i < QN::GROUPS; ++i) mine[(16 * i + r) * 64] = dk[0][i][r];
 #pragma unroll
-                for (int i = 0; i < GN::GROUPS; ++i) mine[(16 * (QN::GROUPS + i) + r) * 64] = dv[i][r];
+                for (int i = 0; i < GN::GROUPS; ++i) mine[(16 * (QN::GROUPS + i) + r) * 64] = dv[0][i][r];
             }
         }
         __syncthreads();
@@ -375,28 +441,28 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
 #pragma unroll
-                for (int i = 0; i < QN::GROUPS; ++i) dk[i][r] += other[(16 * i + r) * 64];
+                for (int i = 0; i < QN::GROUPS; ++i) dk[0][i][r] += other[(16 * i + r) * 64];
 #pragma unroll
-                for (int i = 0; i < GN::GROUPS; ++i) dv[i][r] += other[(16 * (QN::GROUPS + i) + r) * 64];
+                for (int i = 0; i < GN::GROUPS; ++i) dv[0][i][r] += other[(16 * (QN::GROUPS + i) + r) * 64];
             }
         }
     }
     if (!inside) return;
-    eight_rows<NP, DK>(dk[0]);
+    eight_rows<NP, DK>(dk[0][0]);
     auto each = [&](auto&& put_k, auto&& put_v) {
 #pragma unroll
         for (int i = 0; i < QN::GROUPS; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * i + acc_row(r, h);
-                if (d < a.Dk && (!QN::P8 || r < 4)) put_k(d, live ? dk[i][r] * a.scale : 0.f);
+                if (d < a.Dk && (!QN::P8 || r < 4)) put_k(d, live ? dk[0][i][r] * a.scale : 0.f);
             }
 #pragma unroll
         for (int i = 0; i < GN::GROUPS; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * i + acc_row(r, h);
-                if (d < a.Dv) put_v(d, live ? dv[i][r] : 0.f);
+                if (d < a.Dv) put_v(d, live ? dv[0][i][r] : 0.f);
             }
     };
     if (a.part == nullptr) {
@@ -473,8 +539,8 @@ BwdPlan plan_of(const eeggan_attention& a, bool want_table) {
 
 template <class T, int DK, int DV, bool BIAS>
 int launch_dq(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
-    constexpr int NP = Elem<T>::NP, XT = Cut<T, DK, DV>::DQ_XT;
-    constexpr size_t tiles = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES + TTile<NP, DV, XT>::BYTES;
+    constexpr int XT = Cut<T, DK, DV>::DQ_XT;
+    constexpr size_t tiles = DqCut<T, DK, DV, XT>::LDS;
     constexpr size_t most = tiles + (BIAS ? 4 * (2 * (1024 + 31 * 16 + 31) + 1) * sizeof(float) : 0);
     static_assert(most <= 160 * 1024, "LDS");
     auto kernel = &attn_dq_kernel<T, DK, DV, XT, BIAS>;
@@ -491,11 +557,7 @@ int launch_dq(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
 
 template <class T, int DK, int DV, int WK, int XT, bool BIAS>
 int launch_dkv(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
-    constexpr int NP = Elem<T>::NP;
-    constexpr size_t tiles = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES + TTile<NP, DV, XT>::BYTES +
-                             NTile<NP, DV, XT>::BYTES + 2 * XT * sizeof(float);
-    constexpr size_t join = (4 / WK - 1) * WK * (NTile<NP, DK, XT>::GROUPS + NTile<NP, DV, XT>::GROUPS) * 16 * 64 * sizeof(float);
-    constexpr size_t lds = tiles > join ? tiles : join;
+    constexpr size_t lds = DkvCut<T, DK, DV, WK, XT>::LDS;
     static_assert(lds <= 160 * 1024 && 2 * XT <= THREADS, "LDS");
     auto kernel = &attn_dkv_kernel<T, DK, DV, WK, XT, BIAS>;
     static LdsReady ready;

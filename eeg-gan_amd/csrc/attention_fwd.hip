@@ -29,219 +29,306 @@ struct FwdArgs {
     float scale;
 };
 
-template <class T, int DK, int DV, int KW, int XT, bool BIAS>
+// KW waves share the columns and split a stage's keys; CB: column blocks of a wave (its LDS operands serve all of them).
+template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS>
+struct FwdCut {
+    static constexpr int NP = Elem<T>::NP;
+    static constexpr int STAGE = TTile<NP, DK, XT>::BYTES + NTile<NP, DV, XT>::BYTES;
+    static constexpr int BUFS = 2 * STAGE <= 80 * 1024 ? 2 : 1;  // (two workgroups to a CU)
+    static constexpr int LDS = BUFS * STAGE;
+};
+template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
+    typedef FwdCut<T, DK, DV, KW, XT, CB, BIAS> Cut;
     constexpr int NP = Elem<T>::NP;
-    constexpr int WC = 4 / KW;                 // column tiles of a workgroup
-    constexpr int SUBS = XT / (32 * KW);       // key tiles a wave takes of a stage
+    constexpr int WC = 4 / KW;                  // waves along the columns
+    constexpr int SUBS = XT / (32 * KW);        // key tiles a wave takes of a stage
+    constexpr int J = CB == 1 && SUBS % 2 == 0 ? 2 : 1;  // ... of them at once: independent chains to overlap
     typedef TTile<NP, DK, XT> KT;
     typedef NTile<NP, DV, XT> VT;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    char* const kt = smem;
-    char* const vt = smem + KT::BYTES;
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ksub = wave % KW;
-    int blk = blockIdx.x;
-    const int tile = blk % a.coltiles;
-    blk /= a.coltiles;
-    const int split = blk % a.nsplit;
-    const int bkv = blk / a.nsplit;
+    int bkv, part;
+    place(blockIdx.x, a.B * a.KV, a.coltiles * a.nsplit, bkv, part);
+    const int tile = part % a.coltiles, split = part / a.coltiles;
     const int b = bkv / a.KV, kvh = bkv - b * a.KV;
 
     const int ncols = a.G * a.Tq;
-    const int col0 = (tile * WC + wave / KW) * 32;
-    const int n = col0 + l31;
-    const bool live = n < ncols;
-    const int g = live ? n / a.Tq : 0, t = live ? n - g * a.Tq : 0;
-    const int head = kvh * a.G + g;
-
+    const int col0 = (tile * WC + wave / KW) * 32 * CB;
     const float c = a.scale * LOG2E;
-    SFrag<NP, DK> fq;
-    {
-        const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc + t;
+    // per column block: its lane's query and head
+    bool live[CB];
+    int t[CB], head[CB];
+    SFrag<NP, DK> fq[CB];
+    const float* rel[CB];  // position bias: rel[step * s], relative to this lane's query
+    bool one_head[CB];     // (a block of columns of several heads is always near)
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const int n0 = col0 + 32 * i, n = n0 + l31;
+        live[i] = n < ncols;
+        const int g = live[i] ? n / a.Tq : 0;
+        t[i] = live[i] ? n - g * a.Tq : 0;
+        head[i] = kvh * a.G + g;
+        const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head[i] * a.Dk * a.qsc + t[i];
         // (float32: the scale goes into the split operand; bfloat16 operands stay exact and the scores are scaled)
         typedef SFrag<NP, DK> F;
         float x[F::VALUES];
         F::read(q, a.qsc, a.Dk, h, x);
 #pragma unroll
-        for (int i = 0; i < F::VALUES; ++i) x[i] = live && F::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
-        fq.fill(h, x);
+        for (int e = 0; e < F::VALUES; ++e)
+            x[e] = live[i] && F::channel(e, h) < a.Dk ? (NP == 3 ? x[e] * c : x[e]) : 0.f;
+        fq[i].fill(h, x);
+        rel[i] = BIAS ? a.pos.rel + (long long)head[i] * a.pos.nrel + (a.Tq - 1 - t[i]) : nullptr;
+        one_head[i] = n0 < ncols && n0 / a.Tq == min(n0 + 31, ncols - 1) / a.Tq;
     }
     const T* const kb = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc;
     const T* const vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc;
     const unsigned char* const mask = a.mask ? a.mask + (long long)b * a.Tk : nullptr;
-    // position bias: rel[step * s] relative to this lane's query
-    const float* const rel = BIAS ? a.pos.rel + (long long)head * a.pos.nrel + (a.Tq - 1 - t) : nullptr;
-    // (a tile of columns of several heads is always near)
-    const bool one_head = col0 / a.Tq == min(col0 + 31, ncols - 1) / a.Tq;
-    const int t_tile = col0 % a.Tq;
 
     const int s_begin = split * a.split_keys;
     const int s_end = min(a.Tk, s_begin + a.split_keys);
 
-    float m = 0.f, l = 0.f, threshold = -INFINITY;  // threshold -inf: no key seen yet
-    f32x16 cinit = zero16();                        // -m in every register: the scores accumulate on top of it
-    f32x16 o[VT::GROUPS];
+    float m[CB], l[CB], threshold[CB];  // threshold -inf: no key seen yet
+    f32x16 o[CB][VT::GROUPS];
 #pragma unroll
-    for (int i = 0; i < VT::GROUPS; ++i) o[i] = zero16();
+    for (int i = 0; i < CB; ++i) {
+        m[i] = l[i] = 0.f;
+        threshold[i] = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < VT::GROUPS; ++e) o[i][e] = zero16();
+    }
 
     Block<T, DK, XT> kblk;
     Block<T, DV, XT> vblk;
-    Steps<XT> ahead;  // which keys of the stage are attended
+    kblk.init(a.ksc, a.Dk, tid);
+    vblk.init(a.vsc, a.Dv, tid);
+    Steps<XT> ahead, now;  // which keys of the stage are attended
     auto fetch = [&](int s0) {
-        kblk.load(kb, a.ksc, a.Dk, s0, s_end, tid);
-        vblk.load(vb, a.vsc, a.Dv, s0, s_end, tid);
+        kblk.load(kb, s0, s_end, tid);
+        vblk.load(vb, s0, s_end, tid);
         ahead.find(s0, s_end, mask, lane);
     };
-    if (s_begin < s_end) fetch(s_begin);
+    auto put = [&](int buf) {
+        char* const kt = smem + buf * Cut::STAGE;
+        kblk.template store<true, false>(kt, nullptr, a.Dk, ahead, tid);
+        vblk.template store<false, true>(nullptr, kt + KT::BYTES, a.Dv, ahead, tid);
+    };
+    int buf = 0;
+    if (s_begin < s_end) {
+        fetch(s_begin);
+        put(0);
+        now = ahead;
+        if (s_begin + XT < s_end) fetch(s_begin + XT);
+        __syncthreads();
+    }
     for (int s0 = s_begin; s0 < s_end; s0 += XT) {
-        __syncthreads();
-        const Steps<XT> now = ahead;
-        kblk.template store<true, false>(kt, nullptr, a.Dk, now, tid);
-        vblk.template store<false, true>(nullptr, vt, a.Dv, now, tid);
-        __syncthreads();
-        if (s0 + XT < s_end) fetch(s0 + XT);
+        // two buffers: the next stage goes into the other one before this one is worked on
+        const Steps<XT> next = ahead;
+        if (Cut::BUFS == 2 && s0 + XT < s_end) {
+            put(buf ^ 1);
+            if (s0 + 2 * XT < s_end) fetch(s0 + 2 * XT);
+        }
+        const char* const kt = smem + buf * Cut::STAGE;
+        const char* const vt = kt + KT::BYTES;
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u) {
-            const int sub = KW == 1 ? u : ksub;
-            const int x0 = 32 * sub;
-            const unsigned word = now.tile(x0);
-            if (word == 0) continue;  // (the same for every lane of the wave)
-            f32x16 acc;
-            if constexpr (BIAS) {
-                const long long s = s0 + x0;
-                if (one_head && tile_side(a.pos, s, t_tile) != 0) {
-                    const float bias = rel[a.pos.step * s];
+        for (int u = 0; u < SUBS; u += J) {
+            unsigned word[J], any = 0;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[r] = cinit[r] + bias;
-                } else {
-                    const int first = min((int)s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
-                    const float* r0 = rel + (long long)a.pos.step * first;
+            for (int j = 0; j < J; ++j) {
+                word[j] = now.tile(32 * (KW == 1 ? u + j : ksub));
+                any |= word[j];
+            }
+            if (any == 0) continue;  // (the same for every lane of the wave)
+            f32x16 acc[J][CB];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = (r & 3) + 8 * (r >> 2);
-                        acc[r] = cinit[r] + r0[a.pos.step * min(i, last)];
+            for (int j = 0; j < J; ++j) {
+                const int x0 = 32 * (KW == 1 ? u + j : ksub);
+#pragma unroll
+                for (int i = 0; i < CB; ++i) acc[j][i] = zero16();
+                mma_scores<NP, DK, XT, CB>(kt + (x0 + l31) * KT::RS, h, fq, acc[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < CB; ++i) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const int x0 = 32 * (KW == 1 ? u + j : ksub);
+                    if constexpr (BIAS) {
+                        const int s = min(s0 + x0, a.Tk - 1);
+                        if (one_head[i] && tile_side(a.pos, s0 + x0, (col0 + 32 * i) % a.Tq) != 0) {
+                            const float base = rel[i][(long long)a.pos.step * s] - m[i];
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c, base);
+                        } else {
+                            const int first = min(s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
+                            const float* r0 = rel[i] + (long long)a.pos.step * first;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c,
+                                                              r0[a.pos.step * min((r & 3) + 8 * (r >> 2), last)] - m[i]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            acc[j][i][r] = NP == 3 ? acc[j][i][r] - m[i] : __builtin_fmaf(acc[j][i][r], c, -m[i]);
+                    }
+                    if (word[j] != 0xffffffffu) {
+                        const unsigned w = word[j] >> (4 * h);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            acc[j][i][r] = (w >> ((r & 3) + 8 * (r >> 2))) & 1u ? acc[j][i][r] : -INFINITY;
                     }
                 }
-            } else {
-                acc = cinit;
-            }
-            if constexpr (NP == 3) {
-                acc = mma_scores<NP, DK, XT>(kt + (x0 + l31) * KT::RS, h, fq, acc);
-            } else {
-                const f32x16 raw = mma_scores<NP, DK, XT>(kt + (x0 + l31) * KT::RS, h, fq, zero16());
+                float top = acc[0][i][0];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[r] = __builtin_fmaf(raw[r], c, acc[r]);
-            }
-            if (word != 0xffffffffu) {
-                const unsigned w = word >> (4 * h);
+                for (int j = 0; j < J; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[r] = (w >> ((r & 3) + 8 * (r >> 2))) & 1u ? acc[r] : -INFINITY;
-            }
-            float top = acc[0];
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[j][i][r]);
+                top = half_max(top);
+                const bool move = top > threshold[i];
+                if (__any(move)) {
+                    const float d = move ? top : 0.f;
+                    const float f = move && threshold[i] > 0.f ? __builtin_amdgcn_exp2f(-d) : 1.f;
+                    if (move) threshold[i] = 8.f;
+                    m[i] += d;
+                    l[i] *= f;
 #pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, acc[r]);
-            top = half_max(top);
-            const bool move = top > threshold;
-            if (__any(move)) {
-                const float d = move ? top : 0.f;
-                const float f = move && threshold > 0.f ? __builtin_amdgcn_exp2f(-d) : 1.f;
-                if (move) threshold = 8.f;
-                m += d;
-                l *= f;
+                    for (int e = 0; e < VT::GROUPS; ++e)
 #pragma unroll
-                for (int i = 0; i < VT::GROUPS; ++i)
+                        for (int r = 0; r < 16; ++r) o[i][e][r] *= f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[i][r] *= f;
+                    for (int j = 0; j < J; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    acc[r] -= d;
-                    cinit[r] = -m;
+                        for (int r = 0; r < 16; ++r) acc[j][i][r] -= d;
                 }
-            }
-            float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                acc[r] = __builtin_amdgcn_exp2f(acc[r]);
-                s4[r & 3] += acc[r];
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        acc[j][i][r] = __builtin_amdgcn_exp2f(acc[j][i][r]);
+                        s4[r & 3] += acc[j][i][r];
+                    }
+                l[i] += (s4[0] + s4[1]) + (s4[2] + s4[3]);
             }
-            l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            PFrag<NP> p;
-            p.fill(acc);
-            mma_values<NP, DV, XT>(vt, x0, l31, h, p, o);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                PFrag<NP> p[CB];
+#pragma unroll
+                for (int i = 0; i < CB; ++i) p[i].fill(acc[j][i]);
+                mma_values<NP, DV, XT, CB>(vt, 32 * (KW == 1 ? u + j : ksub), l31, h, p, o);
+            }
+        }
+        if (s0 + XT < s_end) {
+            __syncthreads();
+            if (Cut::BUFS == 1) {
+                put(0);
+                if (s0 + 2 * XT < s_end) fetch(s0 + 2 * XT);
+                __syncthreads();
+            } else {
+                buf ^= 1;
+            }
+            now = next;
         }
     }
 
-    l = half_sum(l);
-    if (!live) return;
-    if (a.part == nullptr) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // (no key: a column of zeros)
-        const long long row = (long long)b * a.KV * a.G + head;
-        if (a.lse && h == 0) a.lse[row * a.Tq + t] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
-        T* out = reinterpret_cast<T*>(a.out) + row * a.Dv * a.Tq + t;
 #pragma unroll
-        for (int i = 0; i < VT::GROUPS; ++i)
+    for (int i = 0; i < CB; ++i) {
+        const float sum = half_sum(l[i]);
+        if (!live[i]) continue;
+        if (a.part == nullptr) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (no key: a column of zeros)
+            const long long row = (long long)b * a.KV * a.G + head[i];
+            if (a.lse && h == 0) a.lse[row * a.Tq + t[i]] = sum == 0.f ? INFINITY : m[i] + __builtin_amdgcn_logf(sum);
+            T* out = reinterpret_cast<T*>(a.out) + row * a.Dv * a.Tq + t[i];
+            T* rest = NP == 1 && a.rest ? reinterpret_cast<T*>(a.rest) + row * a.Dv * a.Tq + t[i] : nullptr;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int d = 32 * i + acc_row(r, h);
-                if (d < a.Dv) {
-                    const float v = o[i][r] * inv;
-                    st1(out + (long long)d * a.Tq, v);
-                    if (NP == 1 && a.rest) {
-                        T* rest = reinterpret_cast<T*>(a.rest) + row * a.Dv * a.Tq + t;
-                        st1(rest + (long long)d * a.Tq, v - (float)(T)v);
+            for (int e = 0; e < VT::GROUPS; ++e)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = 32 * e + acc_row(r, h);
+                    if (d < a.Dv) {
+                        const float v = o[i][e][r] * inv;
+                        st1(out + (long long)d * a.Tq, v);
+                        if (NP == 1 && rest) st1(rest + (long long)d * a.Tq, v - (float)(T)v);
                     }
                 }
-            }
-    } else {
-        const long long nparts = (long long)a.nsplit * KW;
-        const long long part = ((long long)bkv * nparts + split * KW + ksub);
-        float* po = a.part + part * a.Dv * ncols + n;
+        } else {
+            const long long nparts = (long long)a.nsplit * KW;
+            const long long at = (long long)bkv * nparts + split * KW + ksub;
+            float* po = a.part + at * a.Dv * ncols + col0 + 32 * i + l31;
 #pragma unroll
-        for (int i = 0; i < VT::GROUPS; ++i)
+            for (int e = 0; e < VT::GROUPS; ++e)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int d = 32 * i + acc_row(r, h);
-                if (d < a.Dv) po[(long long)d * ncols] = o[i][r];
+                for (int r = 0; r < 16; ++r) {
+                    const int d = 32 * e + acc_row(r, h);
+                    if (d < a.Dv) po[(long long)d * ncols] = o[i][e][r];
+                }
+            if (h == 0) {
+                const long long total = (long long)a.B * a.KV * nparts;
+                float* pm = a.part + total * a.Dv * ncols + at * ncols + col0 + 32 * i + l31;
+                pm[0] = m[i];
+                pm[total * ncols] = sum;
             }
-        if (h == 0) {
-            const long long total = (long long)a.B * a.KV * nparts;
-            float* pm = a.part + total * a.Dv * ncols + part * ncols + n;
-            pm[0] = m;
-            pm[total * ncols] = l;
         }
     }
 }
 
 // Parts of a split over the keys -> output: M = max m, O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i; parts that saw
-// no key (l = 0) are left out.
+// no key (l = 0) are left out.  `lanes` threads share an output's parts, joined in LDS in a
+// fixed order: there are few outputs and up to hundreds of parts, and a thread that walked them alone would wait for one
+// load after the other.
 template <class T>
-__global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a, int nparts, long long items) {
-    const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
-    if (i >= items) return;
+__global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a, int nparts, int lanes, long long items) {
+    __shared__ float red[3][THREADS];
+    const int tid = threadIdx.x, per = THREADS / lanes;  // outputs of the workgroup
+    const int lane = tid / per;
+    const long long i = (long long)blockIdx.x * per + tid % per;
     const int ncols = a.G * a.Tq;
+    float top = -INFINITY, l = 0.f, o = 0.f;
+    if (i < items) {
+        const int n = (int)(i % ncols);
+        const long long j = i / ncols;
+        const int d = (int)(j % a.Dv);
+        const long long bkv = j / a.Dv;
+        const long long total = (long long)a.B * a.KV * nparts;
+        const float* po = a.part + (bkv * nparts * a.Dv + d) * ncols + n;
+        const float* pm = a.part + total * a.Dv * ncols + bkv * nparts * ncols + n;
+        const float* pl = pm + total * ncols;
+        for (int p = lane; p < nparts; p += lanes) {
+            const float lp = pl[(long long)p * ncols], mp = pm[(long long)p * ncols], op = po[(long long)p * a.Dv * ncols];
+            if (lp != 0.f) {
+                const float t = fmaxf(top, mp);
+                const float f = __builtin_amdgcn_exp2f(top - t), e = __builtin_amdgcn_exp2f(mp - t);
+                l = l * f + lp * e;
+                o = o * f + op * e;
+                top = t;
+            }
+        }
+    }
+    if (lanes > 1) {
+        red[0][tid] = top, red[1][tid] = l, red[2][tid] = o;
+        __syncthreads();
+        if (lane != 0) return;
+        for (int w = 1; w < lanes; ++w) {
+            const float mp = red[0][tid + w * per], lp = red[1][tid + w * per], op = red[2][tid + w * per];
+            if (lp != 0.f) {
+                const float t = fmaxf(top, mp);
+                const float f = __builtin_amdgcn_exp2f(top - t), e = __builtin_amdgcn_exp2f(mp - t);
+                l = l * f + lp * e;
+                o = o * f + op * e;
+                top = t;
+            }
+        }
+    }
+    if (i >= items) return;
     const int n = (int)(i % ncols);
     const long long j = i / ncols;
     const int d = (int)(j % a.Dv);
     const long long bkv = j / a.Dv;
-    const long long total = (long long)a.B * a.KV * nparts;
-    const float* po = a.part + (bkv * nparts * a.Dv + d) * ncols + n;
-    const float* pm = a.part + total * a.Dv * ncols + bkv * nparts * ncols + n;
-    const float* pl = pm + total * ncols;
-    float top = -INFINITY;
-    for (int p = 0; p < nparts; ++p)
-        if (pl[(long long)p * ncols] != 0.f) top = fmaxf(top, pm[(long long)p * ncols]);
-    float l = 0.f, o = 0.f;
-    for (int p = 0; p < nparts; ++p) {
-        const float lp = pl[(long long)p * ncols];
-        if (lp != 0.f) {
-            const float f = __builtin_amdgcn_exp2f(pm[(long long)p * ncols] - top);
-            l += f * lp;
-            o += f * po[(long long)p * a.Dv * ncols];
-        }
-    }
     const int g = n / a.Tq, t = n - g * a.Tq;
     const long long row = bkv * a.G + g;
     const float v = l == 0.f ? 0.f : o / l;
@@ -262,27 +349,31 @@ namespace {
 // How the forward pass is cut.  Up to 32 query columns per key head: the waves split every stage's keys.  Beyond that
 // each wave has columns of its own.  Keys are split over workgroups until there are `WANTED` of them.
 struct FwdPlan {
-    int kw, xt, coltiles, nsplit, split_keys, nparts;
+    int kw, xt, cb, coltiles, nsplit, split_keys, nparts;
 };
 constexpr int WANTED = 512;
 
 template <class T, int DK, int DV>
-constexpr int stage_keys(bool few) {
-    constexpr bool f32 = Elem<T>::NP == 3;
-    return few ? (f32 && DK + DV > 128 ? 64 : 128) : (f32 && DK + DV > 160 ? 32 : 64);
-}
+struct Cuts {
+    static constexpr bool F32 = Elem<T>::NP == 3;
+    static constexpr int FEW_XT = F32 && DK + DV > 128 ? 64 : 128;  // keys of a stage: few columns / many
+    static constexpr int XT = F32 && DK + DV > 96 ? 32 : 64;
+    static constexpr int CB = DK + DV <= (F32 ? 64 : 128) ? 2 : 1;  // column blocks of a wave, where there are enough
+};
 
 template <class T, int DK, int DV>
 FwdPlan plan_of(const eeggan_attention& a) {
+    typedef Cuts<T, DK, DV> C;
     FwdPlan p;
-    const long long ncols = (long long)(a.H / a.KV) * a.Tq;
+    const long long ncols = (long long)(a.H / a.KV) * a.Tq, heads = (long long)a.B * a.KV;
     const bool few = ncols <= 32;
-    p.xt = stage_keys<T, DK, DV>(few);
+    p.xt = few ? C::FEW_XT : C::XT;
     p.kw = few ? p.xt / 32 : 1;
-    p.coltiles = few ? 1 : (int)((ncols + 127) / 128);
-    const long long blocks = (long long)a.B * a.KV * p.coltiles;
+    p.cb = !few && C::CB == 2 && heads * ((ncols + 255) / 256) >= WANTED ? 2 : 1;
+    p.coltiles = few ? 1 : (int)((ncols + 128 * p.cb - 1) / (128 * p.cb));
+    const long long blocks = heads * p.coltiles;
     const long long stages = (a.Tk + p.xt - 1) / p.xt;
-    long long n = blocks >= WANTED ? 1 : (WANTED + blocks - 1) / blocks;
+    long long n = blocks >= WANTED / 2 ? 1 : (WANTED + blocks - 1) / blocks;
     const long long most = few ? stages : stages / 4 > 0 ? stages / 4 : 1;
     if (n > most) n = most;
     const long long per = (stages + n - 1) / n;
@@ -298,18 +389,27 @@ size_t part_bytes(const eeggan_attention& a, const FwdPlan& p) {
     return (size_t)a.B * a.KV * p.nparts * ncols * (a.Dv + 2) * sizeof(float);
 }
 
-template <class T, int DK, int DV, int KW, int XT, bool BIAS>
+template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS>
 int launch(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
-    constexpr int NP = Elem<T>::NP;
-    constexpr size_t lds = TTile<NP, DK, XT>::BYTES + NTile<NP, DV, XT>::BYTES;
+    constexpr size_t lds = FwdCut<T, DK, DV, KW, XT, CB, BIAS>::LDS;
     static_assert(lds <= 160 * 1024, "LDS");
-    auto kernel = &attn_fwd_kernel<T, DK, DV, KW, XT, BIAS>;
+    auto kernel = &attn_fwd_kernel<T, DK, DV, KW, XT, CB, BIAS>;
     static LdsReady ready;
     if (ready.reserve("attention", reinterpret_cast<const void*>(kernel), lds)) return 1;
     const long long grid = (long long)f.B * f.KV * p.nsplit * p.coltiles;
     EEGGAN_REQUIRE(grid < (1ll << 31), "attention: too many workgroups");
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), lds, st, f);
     return check_launch("attention");
+}
+
+template <class T, int DK, int DV, bool BIAS>
+int launch_cut(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
+    typedef Cuts<T, DK, DV> C;
+    if (p.kw > 1) return launch<T, DK, DV, C::FEW_XT / 32, C::FEW_XT, 1, BIAS>(f, p, st);
+    if constexpr (C::CB == 2) {
+        if (p.cb == 2) return launch<T, DK, DV, 1, C::XT, 2, BIAS>(f, p, st);
+    }
+    return launch<T, DK, DV, 1, C::XT, 1, BIAS>(f, p, st);
 }
 
 template <class T, int DK, int DV>
@@ -325,17 +425,14 @@ int forward(const eeggan_attention& a, void* out, void* rest, float* lse, void* 
     f.B = a.B, f.KV = a.KV, f.G = a.H / a.KV, f.Dk = a.Dk, f.Dv = a.Dv, f.Tq = a.Tq, f.Tk = a.Tk;
     f.coltiles = p.coltiles, f.nsplit = p.nsplit, f.split_keys = p.split_keys, f.scale = a.scale;
     if (positions(a, reinterpret_cast<float*>(ws), &f.pos, st)) return 1;
-    int rc;
-    constexpr int XF = stage_keys<T, DK, DV>(true), XN = stage_keys<T, DK, DV>(false);
-    if (p.kw > 1)
-        rc = a.table ? launch<T, DK, DV, XF / 32, XF, true>(f, p, st) : launch<T, DK, DV, XF / 32, XF, false>(f, p, st);
-    else
-        rc = a.table ? launch<T, DK, DV, 1, XN, true>(f, p, st) : launch<T, DK, DV, 1, XN, false>(f, p, st);
-    if (rc || p.nparts == 1) return rc;
+    if (a.table ? launch_cut<T, DK, DV, true>(f, p, st) : launch_cut<T, DK, DV, false>(f, p, st)) return 1;
+    if (p.nparts == 1) return 0;
     const long long items = (long long)a.B * a.KV * a.Dv * f.G * a.Tq;
-    EEGGAN_REQUIRE((items + THREADS - 1) / THREADS < (1ll << 31), "attention: too many outputs");
-    hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)((items + THREADS - 1) / THREADS)), dim3(THREADS), 0, st, f,
-                       p.nparts, items);
+    int lanes = 1;  // threads that share an output's parts: at least four parts each
+    while (lanes < 16 && lanes * 8 <= p.nparts) lanes *= 2;
+    const long long blocks = (items * lanes + THREADS - 1) / THREADS;
+    EEGGAN_REQUIRE(blocks < (1ll << 31), "attention: too many outputs");
+    hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)blocks), dim3(THREADS), 0, st, f, p.nparts, lanes, items);
     return check_launch("attention (join)");
 }
 

@@ -165,29 +165,56 @@ struct Steps {
 };
 
 // A [D, XT] block of a channels-first matrix on its way from memory into LDS: 4 x 4 units (four channels, four time
-// steps), neighbouring threads on neighbouring steps.  Loads never branch (the compiler would wait at every join):
-// whatever lies past the matrix is read at its last row or step.  Such values and those of masked steps become zeros on
-// their way into LDS, so what they hold (NaN included) never meets a product.
+// steps).  A wave takes 8 x 8 units where the block has them (its transposed writes then fall on all LDS banks: rows of
+// units lie 16 banks apart, neighbouring channel groups 2), else neighbouring steps first.  Loads never branch per value
+// (the compiler would wait at every join): whatever lies past the matrix is read at its last row or step.  Such values and
+// those of masked steps become zeros on their way into LDS, so what they hold (NaN included) never meets a product.
 template <class T, int D, int XT>
 struct Block {
     static constexpr int NP = Elem<T>::NP;
-    static constexpr int XQ = XT / 4, UNITS = (D / 4) * XQ, U = (UNITS + THREADS - 1) / THREADS;
+    static constexpr int XQ = XT / 4, DB = D / 4, UNITS = DB * XQ, U = (UNITS + THREADS - 1) / THREADS;
+    static constexpr bool SQUARE = XQ % 8 == 0 && DB % 8 == 0;
     typename Elem<T>::raw4 r[U][4];
+    unsigned off[U][4];  // byte offsets of the unit's rows from (channel 0, first step of the stage)
 
-    // base: channel 0, step 0 of the head; steps [x0, x0 + XT) of `len`
-    __device__ __forceinline__ void load(const T* base, long long stride, int channels, int x0, int len, int tid) {
-        const bool whole = x0 + XT <= len;
+    static __device__ __forceinline__ int unit_kq(int unit) {
+        return SQUARE ? 8 * ((unit >> 6) % (XQ / 8)) + (unit & 7) : unit % XQ;
+    }
+    static __device__ __forceinline__ int unit_db(int unit) {
+        return SQUARE ? 8 * ((unit >> 6) / (XQ / 8)) + ((unit >> 3) & 7) : unit / XQ;
+    }
+
+    // stride (channels, in elements) times 128 fits 32 bits in bytes: checked on the host
+    __device__ __forceinline__ void init(long long stride, int channels, int tid) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int unit = tid + THREADS * u;
-            if (UNITS % THREADS != 0 && unit >= UNITS) continue;
-            const int kq = unit % XQ, db = unit / XQ;
-            const int x = x0 + 4 * kq, last = len - 1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const T* p = base + (long long)min(4 * db + i, channels - 1) * stride;
-                if (whole) r[u][i] = load4(p + x);
-                else r[u][i] = gather4(p, min(x, last), min(x + 1, last), min(x + 2, last), min(x + 3, last));
+            for (int i = 0; i < 4; ++i)
+                off[u][i] = (unsigned)((min(4 * unit_db(unit) + i, channels - 1) * (unsigned)stride + 4 * unit_kq(unit)) * sizeof(T));
+        }
+    }
+
+    // base: channel 0, step 0 of the head; steps [x0, x0 + XT) of `len`
+    __device__ __forceinline__ void load(const T* base, int x0, int len, int tid) {
+        if (x0 + XT <= len) {
+            const char* p = reinterpret_cast<const char*>(base + x0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (UNITS % THREADS != 0 && tid + THREADS * u >= UNITS) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[u][i] = load4(reinterpret_cast<const T*>(p + off[u][i]));
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int unit = tid + THREADS * u;
+                if (UNITS % THREADS != 0 && unit >= UNITS) continue;
+                const int kq = unit_kq(unit), x = x0 + 4 * kq, last = len - 1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    r[u][i] = gather4(reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off[u][i]) - 4 * kq,
+                                      min(x, last), min(x + 1, last), min(x + 2, last), min(x + 3, last));
             }
         }
     }
@@ -202,7 +229,7 @@ struct Block {
         for (int u = 0; u < U; ++u) {
             const int unit = tid + THREADS * u;
             if (UNITS % THREADS != 0 && unit >= UNITS) continue;
-            const int kq = unit % XQ, db = unit / XQ;
+            const int kq = unit_kq(unit), db = unit_db(unit);
             if (!clean) {
                 const unsigned keep = steps.quad(kq);
 #pragma unroll
@@ -305,14 +332,19 @@ struct SFrag {
     }
 };
 
-// acc[x, column] += sum_d tile[x, d] frag[d, column] for the 32 rows from `row` (= tile + (first row + lane & 31) * RS)
-template <int NP, int D, int XT>
-__device__ __forceinline__ f32x16 mma_scores(const char* row, int h, const SFrag<NP, D>& s, f32x16 acc) {
+// acc[b][x, column] += sum_d tile[x, d] frag[b][d, column] for the 32 rows from `row` (= tile + (first row + lane & 31)
+// * RS) and CB column blocks: every operand read from LDS serves all of them.
+template <int NP, int D, int XT, int CB>
+__device__ __forceinline__ void mma_scores(const char* row, int h, const SFrag<NP, D> (&s)[CB], f32x16 (&acc)[CB]) {
     typedef TTile<NP, D, XT> TL;
     if constexpr (packed8<NP, D>()) {
-        acc = mfma(lds8(row + 32 * h), s.f[1], acc);  // p1 q3 | p3 q1
-        acc = mfma(lds8(row + 16), s.f[0], acc);      // p2 q1 | p2 q2
-        acc = mfma(lds8(row), s.f[0], acc);           // p1 q1 | p1 q2
+        const bf16x8 a0 = lds8(row + 32 * h), a1 = lds8(row + 16), a2 = lds8(row);
+#pragma unroll
+        for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[1], acc[b]);  // p1 q3 | p3 q1
+#pragma unroll
+        for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[0], acc[b]);  // p2 q1 | p2 q2
+#pragma unroll
+        for (int b = 0; b < CB; ++b) acc[b] = mfma(a2, s[b].f[0], acc[b]);  // p1 q1 | p1 q2
     } else {
         constexpr int J = D / 16;
 #pragma unroll
@@ -321,16 +353,21 @@ __device__ __forceinline__ f32x16 mma_scores(const char* row, int h, const SFrag
             const bf16x8 a0 = lds8(p);
             if constexpr (NP == 3) {
                 const bf16x8 a1 = lds8(p + TL::PIECE), a2 = lds8(p + 2 * TL::PIECE);
-                acc = mfma(a2, s.f[j], acc);
-                acc = mfma(a0, s.f[2 * J + j], acc);
-                acc = mfma(a1, s.f[J + j], acc);
-                acc = mfma(a1, s.f[j], acc);
-                acc = mfma(a0, s.f[J + j], acc);
+#pragma unroll
+                for (int b = 0; b < CB; ++b) acc[b] = mfma(a2, s[b].f[j], acc[b]);
+#pragma unroll
+                for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[2 * J + j], acc[b]);
+#pragma unroll
+                for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[J + j], acc[b]);
+#pragma unroll
+                for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[j], acc[b]);
+#pragma unroll
+                for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[J + j], acc[b]);
             }
-            acc = mfma(a0, s.f[j], acc);
+#pragma unroll
+            for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[j], acc[b]);
         }
     }
-    return acc;
 }
 
 // The result registers of a scores-like product as the operand of a values-like one.
@@ -354,31 +391,39 @@ struct PFrag {
     }
 };
 
-// acc[g][row, column] += sum_x tile[32 g + row, x] frag[x, column] over the 32 steps from x0.
+// acc[b][g][row, column] += sum_x tile[32 g + row, x] frag[b][x, column] over the 32 steps from x0.
 // Eight rows in three pieces: the pieces lie one after the other in the rows of ONE instruction (rows 8 p + d), three
 // instructions instead of six; eight_rows() sums the pieces' results.
-template <int NP, int D, int XT>
-__device__ __forceinline__ void mma_values(const char* tile, int x0, int l31, int h, const PFrag<NP>& b,
-                                           f32x16 (&acc)[NTile<NP, D, XT>::GROUPS]) {
+template <int NP, int D, int XT, int CB>
+__device__ __forceinline__ void mma_values(const char* tile, int x0, int l31, int h, const PFrag<NP> (&f)[CB],
+                                           f32x16 (&acc)[CB][NTile<NP, D, XT>::GROUPS]) {
     typedef NTile<NP, D, XT> NL;
 #pragma unroll
-    for (int g = 0; g < NL::GROUPS; ++g) {
-        const char* row = tile + (32 * g + l31) * NL::RS + 2 * x0 + 16 * h;
+    for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const bf16x8 a0 = lds8(row + 32 * kk);
-            if constexpr (NL::P8) {
-                acc[g] = mfma(a0, b.f[kk][2], acc[g]);
-                acc[g] = mfma(a0, b.f[kk][1], acc[g]);
-            } else if constexpr (NP == 3) {
-                const bf16x8 a1 = lds8(row + 32 * kk + NL::PIECE), a2 = lds8(row + 32 * kk + 2 * NL::PIECE);
-                acc[g] = mfma(a2, b.f[kk][0], acc[g]);
-                acc[g] = mfma(a0, b.f[kk][2], acc[g]);
-                acc[g] = mfma(a1, b.f[kk][1], acc[g]);
-                acc[g] = mfma(a1, b.f[kk][0], acc[g]);
-                acc[g] = mfma(a0, b.f[kk][1], acc[g]);
+        for (int g = 0; g < NL::GROUPS; ++g) {
+            const char* row = tile + (32 * g + l31) * NL::RS + 2 * x0 + 16 * h + 32 * kk;
+            const bf16x8 a0 = lds8(row);
+            bf16x8 a1 = a0, a2 = a0;
+            if constexpr (NP == 3 && !NL::P8) {
+                a1 = lds8(row + NL::PIECE);
+                a2 = lds8(row + 2 * NL::PIECE);
             }
-            acc[g] = mfma(a0, b.f[kk][0], acc[g]);
+#pragma unroll
+            for (int b = 0; b < CB; ++b) {
+                f32x16 c = acc[b][g];
+                if constexpr (NL::P8) {
+                    c = mfma(a0, f[b].f[kk][2], c);
+                    c = mfma(a0, f[b].f[kk][1], c);
+                } else if constexpr (NP == 3) {
+                    c = mfma(a2, f[b].f[kk][0], c);
+                    c = mfma(a0, f[b].f[kk][2], c);
+                    c = mfma(a1, f[b].f[kk][1], c);
+                    c = mfma(a1, f[b].f[kk][0], c);
+                    c = mfma(a0, f[b].f[kk][1], c);
+                }
+                acc[b][g] = mfma(a0, f[b].f[kk][0], c);
+            }
         }
     }
 }
@@ -391,6 +436,20 @@ __device__ __forceinline__ void eight_rows(f32x16& a) {
     }
 }
 __device__ __forceinline__ int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+// Workgroup -> (head, part of it).  Workgroups are dealt to the eight XCDs in turn, each with an L2 of its own: the parts
+// of a head go to one of them, so that what its parts share (keys and values, or queries) is read into one L2.
+__device__ __forceinline__ void place(int blk, int heads, int parts, int& head, int& part) {
+    const int spread = heads / 8 * 8 * parts;
+    if (blk < spread) {
+        const int i = blk >> 3;
+        head = (blk & 7) + 8 * (i / parts);
+        part = i % parts;
+    } else {
+        head = blk / parts;
+        part = blk - head * parts;
+    }
+}
 
 // ---- positions ----------------------------------------------------------------------------------------------
 // Key s lies at position step * s + offset, query t at position t; the bias of the pair depends on their difference

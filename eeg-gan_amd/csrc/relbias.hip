@@ -202,6 +202,10 @@ int check_attention(const char* what, const eeggan_attention* a) {
     EEGGAN_REQUIRE(a->q_batch >= 0 && a->q_channel >= 0 && a->k_batch >= 0 && a->k_channel >= 0 && a->v_batch >= 0 &&
                        a->v_channel >= 0,
                    "%s: negative stride", what);
+    // (a head's rows are addressed with 32-bit byte offsets)
+    const int64_t reach = (1ll << 31) / (128 * (a->bf16 ? 2 : 4));
+    EEGGAN_REQUIRE(a->q_channel <= reach && a->k_channel <= reach && a->v_channel <= reach && a->Tq <= reach,
+                   "%s: channel strides beyond %lld elements", what, (long long)reach);
     const uintptr_t odd = a->bf16 ? 1 : 3;
     EEGGAN_REQUIRE(((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
                      reinterpret_cast<uintptr_t>(a->v)) & odd) == 0, "%s: misaligned tensor", what);
