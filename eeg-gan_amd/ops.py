@@ -1718,9 +1718,18 @@ class RelativeBuckets:
         return side + (self.num_buckets // 2 if self.bidirectional and rel > 0 else 0)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(t):
-    """Launches for ``t``: its device made current (restored afterwards)."""
-    return torch.cuda.device(t.device)
+    """Launches for ``t``: its device made current (and restored) if it is not already."""
+    index = t.device.index
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _stream_of(t) -> int:
+    """Handle of the current stream of ``t``'s device, without building a Stream object (4 us per launch)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
 def _table_chk(table, buckets, heads, device, what):
@@ -1742,7 +1751,7 @@ class _RelBias(Function):
         out = torch.empty(shape, device=table.device, dtype=torch.float32)
         with _on(table):
             call("eeggan_relative_bias", _p(scores), table.data_ptr(), buckets._ptr(), out.data_ptr(), shape[0] // heads,
-                 heads, shape[1], shape[2], _stream())
+                 heads, shape[1], shape[2], _stream_of(table))
         return out
 
     @staticmethod
@@ -1762,7 +1771,7 @@ class _RelBiasSum(Function):
             nbytes = _lib.load().eeggan_relative_bias_grad_workspace(buckets._ptr(), *dims)
             ws = torch.empty(max(nbytes, 16), device=g.device, dtype=torch.uint8)
             call("eeggan_relative_bias_grad", g.data_ptr(), buckets._ptr(), out.data_ptr(), *dims, ws.data_ptr(), nbytes,
-                 _stream())
+                 _stream_of(g))
         return out
 
     @staticmethod
@@ -1802,23 +1811,21 @@ def get_attention() -> str:
 
 def _rows(t):
     """A [B, C, T] tensor the attention kernels can read: unit stride in time, any strides otherwise (a slice of the
-    channels of a wider tensor, an expanded batch); else a copy."""
-    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+    channels of a wider tensor, an expanded batch) that 32-bit row offsets reach; else a copy."""
+    if t.is_contiguous():
+        return t
+    return t if (t.stride(2) == 1 or t.shape[2] == 1) and t.stride(1) < 1 << 22 else t.contiguous()
 
 
 def _attention_desc(q, k, v, mask, table, cfg):
     heads, kv_heads, scale, buckets = cfg
-    a = _AttentionDesc()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_batch, a.q_channel, a.k_batch, a.k_channel = q.stride(0), q.stride(1), k.stride(0), k.stride(1)
-    a.v_batch, a.v_channel = v.stride(0), v.stride(1)
-    a.mask, a.table = _p(mask), _p(table)
-    a.buckets = buckets._ptr() if table is not None else None
-    a.bf16, a.table_bf16 = _bf(q), _bf(table)
-    a.B, a.H, a.KV = q.shape[0], heads, kv_heads
-    a.Dk, a.Dv, a.Tq, a.Tk = q.shape[1] // heads, v.shape[1] // kv_heads, q.shape[2], k.shape[2]
-    a.scale = scale
-    return a
+    B, cq, tq = q.shape
+    (kb, kc, _), (vb, vc, _), (qb, qc, _) = k.stride(), v.stride(), q.stride()
+    return _AttentionDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, qc, kb, kc, vb, vc,
+                          None if mask is None else mask.data_ptr(), None if table is None else table.data_ptr(),
+                          None if table is None else buckets._ptr(), q.dtype is torch.bfloat16,
+                          table is not None and table.dtype is torch.bfloat16, B, heads, kv_heads, cq // heads,
+                          v.shape[1] // kv_heads, tq, k.shape[2], scale)
 
 
 def _attention_stored(q, k, v, table, mask, cfg):
@@ -1850,17 +1857,22 @@ def _attention_stored(q, k, v, table, mask, cfg):
 
 class _Attention(Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, mask, cfg, keep):
-        a = _attention_desc(q, k, v, mask, table, cfg)
-        out = torch.empty((q.shape[0], v.shape[1] // cfg[1] * cfg[0], q.shape[2]), device=q.device, dtype=q.dtype)
-        lse = torch.empty((q.shape[0], cfg[0], q.shape[2]), device=q.device, dtype=torch.float32) if keep else None
-        rest = torch.empty_like(out) if keep and _bf(q) else None
+    def forward(ctx, q, k, v, table, cfg):
+        mask, keep, heads = cfg[4], cfg[5], cfg[0]
+        desc = _attention_desc(q, k, v, mask, table, cfg[:4])
+        a = ctypes.addressof(desc)
+        B, _, tq = q.shape
+        out = q.new_empty((B, v.shape[1] // cfg[1] * heads, tq))
+        rest = torch.empty_like(out) if keep and q.dtype is torch.bfloat16 else None
+        lse = torch.empty((B, heads, tq), device=q.device, dtype=torch.float32) if keep else None
         with _on(q):
-            nbytes = _lib.load().eeggan_attention_fwd_workspace(ctypes.byref(a))
-            ws = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
-            call("eeggan_attention_fwd", ctypes.byref(a), out.data_ptr(), _p(rest), _p(lse), ws.data_ptr(), nbytes, _stream())
-        ctx.cfg = cfg
-        ctx.save_for_backward(q, k, v, table, mask, out, rest, lse)
+            nbytes = _lib.load().eeggan_attention_fwd_workspace(a)
+            ws = torch.empty(nbytes or 16, device=q.device, dtype=torch.uint8)
+            call("eeggan_attention_fwd", a, out.data_ptr(), None if rest is None else rest.data_ptr(),
+                 None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, _stream_of(q))
+        if keep:
+            ctx.cfg, ctx.desc = cfg[:4], desc  # (the descriptor points to tensors that are saved below)
+            ctx.save_for_backward(q, k, v, table, mask, out, rest, lse)
         return out
 
     @staticmethod
@@ -1876,17 +1888,49 @@ class _Attention(Function):
                 again = _attention_stored(q, k, v, table, mask, ctx.cfg)
                 got = torch.autograd.grad(again, [ins[i] for i in wanted], g.float(), create_graph=True)
             grads = dict(zip(wanted, got))
-            return tuple(grads.get(i) for i in range(4)) + (None, None, None)
-        g = g.to(q.dtype).contiguous()
-        a = _attention_desc(q, k, v, mask, table, ctx.cfg)
+            return tuple(grads.get(i) for i in range(4)) + (None,)
+        if g.dtype is not q.dtype or not g.is_contiguous():
+            g = g.to(q.dtype).contiguous()
+        a = ctypes.addressof(ctx.desc)
         gq, gk, gv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
         gt = torch.empty(table.shape, device=table.device, dtype=table.dtype) if want_table else None
         with _on(q):
-            nbytes = _lib.load().eeggan_attention_bwd_workspace(ctypes.byref(a), int(want_table))
-            ws = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
-            call("eeggan_attention_bwd", ctypes.byref(a), out.data_ptr(), _p(rest), lse.data_ptr(), g.data_ptr(),
-                 gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _p(gt), ws.data_ptr(), nbytes, _stream())
-        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, gt, None, None, None
+            nbytes = _lib.load().eeggan_attention_bwd_workspace(a, want_table)
+            ws = torch.empty(nbytes or 16, device=q.device, dtype=torch.uint8)
+            call("eeggan_attention_bwd", a, out.data_ptr(), None if rest is None else rest.data_ptr(), lse.data_ptr(),
+                 g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), None if gt is None else gt.data_ptr(),
+                 ws.data_ptr(), nbytes, _stream_of(q))
+        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, gt, None
+
+
+def _attention_check(q, k, v, heads, kv_heads, mask, bias, buckets):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not t.is_cuda:
+            raise RuntimeError(f"attention {name}: expected a HIP device tensor, got {t.device}; this package has no CPU path")
+        if t.dim() != 3 or 0 in t.shape:
+            raise RuntimeError(f"attention {name}: expected [B, channels, T] without empty axes, got {tuple(t.shape)}")
+        if t.dtype != q.dtype or t.dtype not in (torch.float32, torch.bfloat16):
+            raise RuntimeError(f"attention {name}: expected float32 or bfloat16 for q, k and v alike, got {t.dtype}")
+        if t.device != q.device:
+            raise RuntimeError(f"attention {name}: on {t.device}, q on {q.device}")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise RuntimeError(f"attention: {heads} query heads cannot share {kv_heads} key heads")
+    (B, cq, _), (bk, ck, tk), (bv, cv, tv) = q.shape, k.shape, v.shape
+    if cq % heads or ck != cq // heads * kv_heads or cv % kv_heads:
+        raise RuntimeError(f"attention: channels {cq}, {ck}, {cv} do not fit {heads} query and {kv_heads} key heads")
+    if bk != B or bv != B or tv != tk:
+        raise RuntimeError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
+    if cq // heads > 128 or cv // kv_heads > 128:
+        raise RuntimeError("attention: heads of up to 128 channels are supported")
+    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (B, tk) or mask.device != q.device):
+        raise RuntimeError(f"attention: mask must be a bool tensor of shape {(B, tk)} on {q.device}, got "
+                           f"{mask.dtype} {tuple(mask.shape)} on {mask.device}")
+    if bias is not None:
+        if bias.dtype not in (q.dtype, torch.float32):
+            raise RuntimeError(f"attention: table of {bias.dtype}, expected float32 or {q.dtype}")
+        _table_chk(bias, buckets, heads, q.device, "attention")
+    elif buckets is not None:
+        raise RuntimeError("attention: buckets without a table")
 
 
 def attention(q, k, v, *, heads: int = 1, kv_heads: Optional[int] = None, scale: float = 1.0, mask=None, bias=None,
@@ -1903,41 +1947,16 @@ def attention(q, k, v, *, heads: int = 1, kv_heads: Optional[int] = None, scale:
 
     Gradients of q, k, v and the table come from kernels with a fixed order of summation.  Under ``create_graph=True``
     the backward pass is made of the operators with stored scores instead (float32), which are twice differentiable."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not t.is_cuda:
-            raise RuntimeError(f"attention {name}: expected a HIP device tensor, got {t.device}; this package has no CPU path")
-        if t.dim() != 3 or 0 in t.shape:
-            raise RuntimeError(f"attention {name}: expected [B, channels, T] without empty axes, got {tuple(t.shape)}")
-        if t.dtype != q.dtype or t.dtype not in (torch.float32, torch.bfloat16):
-            raise RuntimeError(f"attention {name}: expected float32 or bfloat16 for q, k and v alike, got {t.dtype}")
-        if t.device != q.device:
-            raise RuntimeError(f"attention {name}: on {t.device}, q on {q.device}")
     kv_heads = heads if kv_heads is None else kv_heads
-    if heads < 1 or kv_heads < 1 or heads % kv_heads:
-        raise RuntimeError(f"attention: {heads} query heads cannot share {kv_heads} key heads")
-    B, tk = q.shape[0], k.shape[2]
-    if q.shape[1] % heads or k.shape[1] != q.shape[1] // heads * kv_heads or v.shape[1] % kv_heads:
-        raise RuntimeError(f"attention: channels {q.shape[1]}, {k.shape[1]}, {v.shape[1]} do not fit {heads} query and "
-                           f"{kv_heads} key heads")
-    if k.shape[0] != B or v.shape[0] != B or v.shape[2] != tk:
-        raise RuntimeError(f"attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
-    if max(q.shape[1] // heads, v.shape[1] // kv_heads) > 128:
-        raise RuntimeError("attention: heads of up to 128 channels are supported")
-    if mask is not None:
-        if mask.dtype != torch.bool or tuple(mask.shape) != (B, tk) or mask.device != q.device:
-            raise RuntimeError(f"attention: mask must be a bool tensor of shape {(B, tk)} on {q.device}, got "
-                               f"{mask.dtype} {tuple(mask.shape)} on {mask.device}")
-        mask = mask.contiguous()
-    if bias is not None:
-        if bias.dtype not in (q.dtype, torch.float32):
-            raise RuntimeError(f"attention: table of {bias.dtype}, expected float32 or {q.dtype}")
-        _table_chk(bias, buckets, heads, q.device, "attention")
+    _attention_check(q, k, v, heads, kv_heads, mask, bias, buckets)
+    keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                        or (bias is not None and bias.requires_grad))
+    if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    elif buckets is not None:
-        raise RuntimeError("attention: buckets without a table")
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias))
-    return _Attention.apply(_rows(q), _rows(k), _rows(v), bias, mask, (int(heads), int(kv_heads), float(scale), buckets),
-                            keep)
+    if mask is not None and not mask.is_contiguous():
+        mask = mask.contiguous()
+    return _Attention.apply(_rows(q), _rows(k), _rows(v), bias,
+                            (int(heads), int(kv_heads), float(scale), buckets, mask, keep))
 
 
 # --------------------------------------------------------------------------------------- minibatch stddev

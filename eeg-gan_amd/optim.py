@@ -25,10 +25,7 @@ DESC_BYTES = ctypes.sizeof(_Desc)
 
 def build_table(rows):
     """rows: list of (p_ptr, g_ptr, m_ptr, v_ptr, step_ptr, n).  Returns a host ctypes array."""
-    arr = (_Desc * len(rows))()
-    for i, (p, g, m, v, s, n) in enumerate(rows):
-        arr[i].p, arr[i].g, arr[i].m, arr[i].v, arr[i].step, arr[i].n = p, g, m, v, s, n
-    return arr
+    return (_Desc * len(rows))(*rows)
 
 
 def _grad_rows(grads, what):
@@ -51,7 +48,8 @@ def _grad_rows(grads, what):
 
 
 def _norm_into(rows, out, scale, max_norm):
-    """out[0] = the norm, out[1] = the multiplier; returns the workspace (the clipped Adam step uses it again)."""
+    """out[0] = the norm, out[1] = the multiplier; returns the table and the workspace (the clipped Adam step uses them
+    again)."""
     table = build_table(rows)
     nbytes = _lib.load().eeggan_grad_norm_workspace(table, len(rows))
     ws = torch.empty(max(nbytes, 16), device=out.device, dtype=torch.uint8)
@@ -152,7 +150,8 @@ class Adam(torch.optim.Optimizer):
                     continue
                 if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
                     raise RuntimeError("Adam: parameters must be contiguous float32 device tensors")
-                g = g if g.is_contiguous() else g.contiguous()
+                if not g.is_contiguous():
+                    g = g.contiguous()
                 st = self._init_state(p)
                 rows.append((p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
                              st["step"].data_ptr(), p.numel()))
@@ -179,11 +178,12 @@ class Adam(torch.optim.Optimizer):
         if self._norm is None or self._norm.device != device:
             self._norm = torch.zeros(2, device=device, dtype=torch.float32)
         with torch.cuda.device(device):
-            # (one norm over the gradients of all groups)
-            _table, ws = _norm_into([row for _, rows in work for row in rows], self._norm, self.grad_scale,
-                                    self.max_grad_norm)
+            # (one norm over the gradients of all groups, whose tensors lie one group after the other in the table)
+            table, ws = _norm_into([row for _, rows in work for row in rows], self._norm, self.grad_scale,
+                                   self.max_grad_norm)
+            first, stream = ctypes.addressof(table), torch.cuda.current_stream().cuda_stream
             for group, rows in work:
                 b1, b2 = group["betas"]
-                call("eeggan_adam_step_clipped", build_table(rows), len(rows), float(group["lr"]), float(b1), float(b2),
-                     float(group["eps"]), self._norm.data_ptr(), ws.data_ptr(), ws.numel(),
-                     torch.cuda.current_stream().cuda_stream)
+                call("eeggan_adam_step_clipped", first, len(rows), float(group["lr"]), float(b1), float(b2),
+                     float(group["eps"]), self._norm.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+                first += len(rows) * DESC_BYTES
