@@ -9,8 +9,9 @@
 // (attention_tiles.h), so nothing crosses lanes.  -delta is the initial accumulator of dP.
 //
 // The position table's gradient rides on attn_dq_kernel: tiles whose distances all lie beyond the last bucket's edge
-// add to one register; a near tile adds its dS to a histogram by distance in LDS, private to the wave, one lane half
-// at a time (no two lanes of an addition share a distance): a fixed order, no races.
+// add to one register; a near tile goes through LDS, every lane adds up the pairs of one distance, and the sums go to a
+// histogram by distance that belongs to the wave: a fixed order, no races.  (LDS float atomics in the place of that took
+// ~300 cycles per instruction: 73 us of 167 at 4 x 6 heads over 1537 steps.)
 #include "attention_host.h"
 
 namespace eeggan {
@@ -39,6 +40,7 @@ struct DqCut {
     static constexpr int BUFS = 2 * STAGE <= 64 * 1024 ? 2 : 1;  // (two workgroups to a CU, with room for histograms)
     static constexpr int LDS = BUFS * STAGE;
 };
+constexpr int SQUARE = 32 * 33;  // a wave's tile of dS on its way into the histogram by distance
 template <class T, int DK, int DV, int XT, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     typedef DqCut<T, DK, DV, XT> Cut;
@@ -100,7 +102,15 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     const T* const kb = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc;
     const T* const vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc;
     const unsigned char* const mask = a.mask ? a.mask + (long long)b * a.Tk : nullptr;
-    const float* const rel = BIAS ? a.pos.rel + (long long)head * a.pos.nrel + (a.Tq - 1 - t) : nullptr;
+    // position bias: one value per side beyond the last edge, near tiles from LDS
+    const float* const rel = BIAS ? a.pos.rel + (long long)head * a.pos.nrel : nullptr;
+    float* const band = reinterpret_cast<float*>(smem + Cut::LDS);
+    float side_bias[2] = {0.f, 0.f};
+    if constexpr (BIAS) {
+        side_bias[0] = rel_at(a.pos, rel, a.Tq, -a.pos.far) - lse;
+        side_bias[1] = rel_at(a.pos, rel, a.Tq, a.pos.far) - lse;
+        fill_band(band, a.pos, rel, a.Tq, tid, THREADS);
+    }
 
     f32x16 dinit;
 #pragma unroll
@@ -110,8 +120,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     for (int i = 0; i < KN::GROUPS; ++i) dq[0][i] = zero16();
 
     double beyond[2] = {0.0, 0.0};  // sums of dS over far tiles, behind / ahead of the query (thousands of terms)
-    float* const hist = BIAS ? reinterpret_cast<float*>(smem + Cut::LDS) + wave * a.nhist : nullptr;
+    float* const hist = BIAS ? band + (2 * a.pos.width + 1) + wave * a.nhist : nullptr;
     const bool want = BIAS && a.hist != nullptr;
+    float* const square = band + (2 * a.pos.width + 1) + 4 * a.nhist + wave * SQUARE;
     const int width = a.nhist / 2;  // (distances -width .. width)
     if (want)
         for (int i = lane; i < a.nhist; i += 64) hist[i] = 0.f;
@@ -120,28 +131,33 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     Block<T, DV, XT> vblk;
     kblk.init(a.ksc, a.Dk, tid);
     vblk.init(a.vsc, a.Dv, tid);
-    Steps<XT> ahead, now;
+    int s_begin = 0, s_end = a.Tk;
+    if (mask) attended_range(mask, s_begin, s_end, reinterpret_cast<int*>(smem));
+    StepsAhead<XT> ahead;
+    Steps<XT> now, next;
     auto fetch = [&](int s0) {
-        kblk.load(kb, s0, a.Tk, tid);
-        vblk.load(vb, s0, a.Tk, tid);
-        ahead.find(s0, a.Tk, mask, lane);
+        ahead.load(s0, s_end, mask, lane);
+        kblk.load(kb, s0, s_end, tid);
+        vblk.load(vb, s0, s_end, tid);
     };
     auto put = [&](int buf) {
         char* const kt = smem + buf * Cut::STAGE;
-        kblk.template store<true, true>(kt, kt + KT::BYTES, a.Dk, ahead, tid);
-        vblk.template store<true, false>(kt + KT::BYTES + KN::BYTES, nullptr, a.Dv, ahead, tid);
+        next.find(ahead.x0, s_end, ahead.raw, lane);
+        kblk.template store<true, true>(kt, kt + KT::BYTES, a.Dk, next, tid);
+        vblk.template store<true, false>(kt + KT::BYTES + KN::BYTES, nullptr, a.Dv, next, tid);
     };
     int buf = 0;
-    fetch(0);
-    put(0);
-    now = ahead;
-    if (XT < a.Tk) fetch(XT);
+    if (s_begin < s_end) {
+        fetch(s_begin);
+        put(0);
+        now = next;
+        if (s_begin + XT < s_end) fetch(s_begin + XT);
+    }
     __syncthreads();
-    for (int s0 = 0; s0 < a.Tk; s0 += XT) {
-        const Steps<XT> next = ahead;
-        if (Cut::BUFS == 2 && s0 + XT < a.Tk) {
+    for (int s0 = s_begin; s0 < s_end; s0 += XT) {
+        if (Cut::BUFS == 2 && s0 + XT < s_end) {
             put(buf ^ 1);
-            if (s0 + 2 * XT < a.Tk) fetch(s0 + 2 * XT);
+            if (s0 + 2 * XT < s_end) fetch(s0 + 2 * XT);
         }
         const char* const kt = smem + buf * Cut::STAGE;
         const char* const kn = kt + KT::BYTES;
@@ -152,32 +168,25 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
             const unsigned word = now.tile(x0);
             if (word == 0) continue;
             const int s = s0 + x0;
-            f32x16 acc;
-            int side = 0;
-            if constexpr (BIAS) {
-                side = tile_side(a.pos, s, t0);
-                if (side != 0) {
-                    const float bias = rel[(long long)a.pos.step * s] - lse;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[r] = bias;
-                } else {
-                    const int first = min(s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
-                    const float* r0 = rel + (long long)a.pos.step * first;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[r] = r0[a.pos.step * min((r & 3) + 8 * (r >> 2), last)] - lse;
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[r] = -lse;
-            }
             // (the scores accumulate from zero and meet lse once: on top of -lse every partial sum would be rounded at
             // its magnitude)
             f32x16 raw[1] = {zero16()}, dsv[1] = {dinit};
-            mma_scores<NP, DK, XT, 1>(kt + (x0 + l31) * KT::RS, h, fq, raw);
-            mma_scores<NP, DV, XT, 1>(vt + (x0 + l31) * VT::RS, h, fg, dsv);
-            f32x16& ds = dsv[0];
+            two_scores<NP, DK, DV, XT>(kt + (x0 + l31) * KT::RS, fq, raw, vt + (x0 + l31) * VT::RS, fg, dsv, h);
+            f32x16 &acc = raw[0], &ds = dsv[0];
+            const float k1 = NP == 3 ? 1.f : c;
+            int side = 0;
+            if constexpr (BIAS) side = tile_side(a.pos, s, t0);
+            if (BIAS && side == 0) {
+                const float* const r0 = band + (int)((long long)a.pos.step * s + a.pos.offset - t0 + a.pos.width) +
+                                        a.pos.step * 4 * h - l31;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[0][r] + acc[r] : __builtin_fmaf(raw[0][r], c, acc[r]);
+                for (int r = 0; r < 16; ++r)
+                    acc[r] = __builtin_fmaf(acc[r], k1, r0[a.pos.step * ((r & 3) + 8 * (r >> 2))] - lse);
+            } else {
+                const float base = !BIAS ? -lse : side < 0 ? side_bias[0] : side_bias[1];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[r] = __builtin_fmaf(acc[r], k1, base);
+            }
             if (word != 0xffffffffu) {
                 const unsigned w = word >> (4 * h);
 #pragma unroll
@@ -191,20 +200,27 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
                         float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int r = 0; r < 16; ++r) s4[r & 3] += ds[r];
-                        const float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
-                        if (side < 0) beyond[0] += (double)sum;
-                        else beyond[1] += (double)sum;
+                        beyond[side > 0] += (double)((s4[0] + s4[1]) + (s4[2] + s4[3]));
                     } else {
-                        // (distances of a near tile stay within the histogram: tile_side)
-                        float* const hp = hist + width + a.pos.offset + a.pos.step * (s + 4 * h) - (t0 + l31);
+                        // the tile goes through LDS and every lane adds up one distance's pairs (row i, column
+                        // step i - distance, of the tile), 64 distances at a time
 #pragma unroll
-                        for (int half = 0; half < 2; ++half)
-                            if (h == half && live) {
-#pragma unroll
-                                for (int r = 0; r < 16; ++r)
-                                    __hip_atomic_fetch_add(hp + a.pos.step * ((r & 3) + 8 * (r >> 2)), ds[r],
-                                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                        for (int r = 0; r < 16; ++r) square[acc_row(r, h) * 33 + l31] = ds[r];
+                        const int step = a.pos.step, span = 31 * step + 32, most = (32 + step - 1) / step;
+                        float* const hp = hist + (int)((long long)step * s + a.pos.offset - t0 + width) - 31;
+                        for (int d0 = 0; d0 < span; d0 += 64) {
+                            const int e = d0 + lane - 31;          // distance relative to the tile's first pair
+                            const int i0 = e <= 0 ? 0 : (e + step - 1) / step;  // first row with a column >= 0
+                            float sum = 0.f;
+#pragma unroll 8
+                            for (int i = 0; i < most; ++i) {
+                                const int row = i0 + i, col = step * row - e;
+                                const bool ok = row < 32 && col >= 0 && col < 32;
+                                const float v = square[ok ? row * 33 + col : 0];
+                                sum += ok ? v : 0.f;
                             }
+                            if (d0 + lane < span) hp[d0 + lane] += sum;
+                        }
                     }
                 }
             }
@@ -212,11 +228,11 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
             p[0].fill(ds);
             mma_values<NP, DK, XT, 1>(kn, x0, l31, h, p, dq);
         }
-        if (s0 + XT < a.Tk) {
+        if (s0 + XT < s_end) {
             __syncthreads();
             if (Cut::BUFS == 1) {
                 put(0);
-                if (s0 + 2 * XT < a.Tk) fetch(s0 + 2 * XT);
+                if (s0 + 2 * XT < s_end) fetch(s0 + 2 * XT);
                 __syncthreads();
             } else {
                 buf ^= 1;
@@ -239,7 +255,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
         if (want) {
             float* const part = a.hist + ((long long)head * a.B * a.coltiles + (long long)b * a.coltiles + tile) * (a.nhist + 2);
             __syncthreads();
-            const float* const all = reinterpret_cast<const float*>(smem + Cut::LDS);
+            const float* const all = band + (2 * a.pos.width + 1);
             for (int i = tid; i < a.nhist; i += THREADS)
                 part[i] = (all[i] + all[a.nhist + i]) + (all[2 * a.nhist + i] + all[3 * a.nhist + i]);
             float* const sums = reinterpret_cast<float*>(smem);
@@ -291,6 +307,8 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     const bool inside = s < a.Tk;
     const bool live = inside && (!a.mask || a.mask[(long long)b * a.Tk + s]);
 
+    const bool any_live = __any(live);
+
     const float c = a.scale * LOG2E;
     SFrag<NP, DK> fk[1];
     SFrag<NP, DV> fv[1];
@@ -324,14 +342,14 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     qblk.init(a.qsc, a.Dk, tid);
     gblk.init(a.Tq, a.Dv, tid);
     float stat = 0.f;
-    Steps<XT> ahead;
+    int ahead = 0;  // first query of the stage that is on its way
     auto fetch = [&](int stage) {
         const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
         const int head = kvh * a.G + g;
         const long long row = (long long)b * H + head;
         qblk.load(reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc, t0, a.Tq, tid);
         gblk.load(reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq, t0, a.Tq, tid);
-        ahead.find(t0, a.Tq, nullptr, lane);
+        ahead = t0;
         if (tid < 2 * XT) {
             const int t = t0 + tid % XT;
             const float* p = (tid < XT ? a.lse : a.delta) + row * a.Tq;
@@ -342,14 +360,29 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     auto put = [&](int buf) {
         char* const qt = smem + buf * Cut::STAGE;
         char* const gt = qt + Cut::Q;
-        qblk.template store<true, true>(qt, qt + QT::BYTES, a.Dk, ahead, tid);
-        gblk.template store<true, true>(gt, gt + GT::BYTES, a.Dv, ahead, tid);
+        Steps<XT> steps;
+        unsigned char all[(XT + 63) / 64];
+#pragma unroll
+        for (int i = 0; i < (XT + 63) / 64; ++i) all[i] = 1;
+        steps.find(ahead, a.Tq, all, lane);
+        qblk.template store<true, true>(qt, qt + QT::BYTES, a.Dk, steps, tid);
+        gblk.template store<true, true>(gt, gt + GT::BYTES, a.Dv, steps, tid);
         if (tid < 2 * XT) reinterpret_cast<float*>(gt + GT::BYTES + GN::BYTES)[tid] = stat;
     };
+    // position bias: near tiles read the stage's head's band in LDS, two of them so that the next head's can be filled
+    // while the last one's is in use
+    float* const bands = reinterpret_cast<float*>(smem + Cut::LDS);
+    float side_bias[2] = {0.f, 0.f};
+    auto band_of = [&](int g) { return bands + (g & 1) * (2 * a.pos.width + 1); };
+    auto put_band = [&](int g) {
+        fill_band(band_of(g), a.pos, a.pos.rel + (long long)(kvh * a.G + g) * a.pos.nrel, a.Tq, tid, THREADS);
+    };
+    int head_now = -1;
     int buf = 0;
     if (first < last) {
         fetch(first);
         put(0);
+        if (BIAS) put_band(first / per_head);
         if (first + 1 < last) fetch(first + 1);
         __syncthreads();
     }
@@ -358,18 +391,23 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
             put(buf ^ 1);
             if (stage + 2 < last) fetch(stage + 2);
         }
+        if (BIAS && stage + 1 < last && (stage + 1) / per_head != stage / per_head) put_band((stage + 1) / per_head);
         const char* const qt = smem + buf * Cut::STAGE;
         const char* const qn = qt + QT::BYTES;
         const char* const gt = qt + Cut::Q;
         const char* const gn = gt + GT::BYTES;
         const float* const stats = reinterpret_cast<const float*>(gn + GN::BYTES);
         const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
-        const float* rel = nullptr;
-        if constexpr (BIAS) rel = a.pos.rel + (long long)(kvh * a.G + g) * a.pos.nrel + (a.Tq - 1);
+        if (BIAS && g != head_now) {
+            head_now = g;
+            const float* const rel = a.pos.rel + (long long)(kvh * a.G + g) * a.pos.nrel;
+            side_bias[0] = rel_at(a.pos, rel, a.Tq, -a.pos.far);
+            side_bias[1] = rel_at(a.pos, rel, a.Tq, a.pos.far);
+        }
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {
             const int x0 = 32 * (u * WT + wt);
-            if (t0 + x0 >= a.Tq) continue;  // (the same for every lane of the wave)
+            if (t0 + x0 >= a.Tq || !any_live) continue;  // (the same for every lane of the wave)
             f32x16 acc, raw[1] = {zero16()}, dsv[1];
             f32x16& ds = dsv[0];
 #pragma unroll
@@ -383,19 +421,20 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
                 }
             }
             if constexpr (BIAS) {
-                const int t = t0 + x0;
-                const float* r0 = rel + (long long)a.pos.step * (inside ? s : 0) - t;
-                if (tile_side(a.pos, s_tile, t) != 0) {
-                    const float bias = r0[0];
+                const int t = t0 + x0, side = tile_side(a.pos, s_tile, t);
+                if (side != 0) {
+                    const float bias = side < 0 ? side_bias[0] : side_bias[1];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[r] += bias;
                 } else {
+                    const float* const r0 = band_of(g) +
+                                            (int)((long long)a.pos.step * s_tile + a.pos.offset - t + a.pos.width) +
+                                            a.pos.step * l31;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[r] += r0[-min(acc_row(r, h), a.Tq - 1 - t)];
+                    for (int r = 0; r < 16; ++r) acc[r] += r0[-acc_row(r, h)];
                 }
             }
-            mma_scores<NP, DK, XT, 1>(qt + (x0 + l31) * QT::RS, h, fk, raw);
-            mma_scores<NP, DV, XT, 1>(gt + (x0 + l31) * GT::RS, h, fv, dsv);
+            two_scores<NP, DK, DV, XT>(qt + (x0 + l31) * QT::RS, fk, raw, gt + (x0 + l31) * GT::RS, fv, dsv, h);
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[0][r] + acc[r] : __builtin_fmaf(raw[0][r], c, acc[r]);
 #pragma unroll
@@ -520,14 +559,14 @@ BwdPlan plan_of(const eeggan_attention& a, bool want_table) {
     BwdPlan p;
     p.qtiles = (a.Tq + 127) / 128;
     const long long heads = (long long)a.B * a.KV;
-    p.narrow = C::NARROW && heads * ((a.Tk + 127) / 128) < WANTED;
+    p.narrow = C::NARROW && a.Tk <= 64;
     const int keys = p.narrow ? 64 : 128, xt = p.narrow ? 64 : C::WIDE_XT;
     p.ktiles = (a.Tk + keys - 1) / keys;
     const long long blocks = heads * p.ktiles, stages = (long long)(a.H / a.KV) * ((a.Tq + xt - 1) / xt);
     long long n = blocks >= WANTED ? 1 : WANTED / blocks;
     if (n > stages / 2) n = stages / 2 > 0 ? stages / 2 : 1;
     p.nsplit = (int)n;
-    p.nhist = a.table && want_table ? 2 * (bucket_far(*a.buckets) + 31 * a.buckets->step + 31) + 1 : 0;
+    p.nhist = a.table && want_table ? 2 * band_width(*a.buckets) + 1 : 0;
     auto up = [](size_t x) { return (x + 15) / 16 * 16; };
     p.rel = positions_bytes(a);
     p.delta = up((size_t)a.B * a.H * a.Tq * sizeof(float));
@@ -541,7 +580,7 @@ template <class T, int DK, int DV, bool BIAS>
 int launch_dq(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
     constexpr int XT = Cut<T, DK, DV>::DQ_XT;
     constexpr size_t tiles = DqCut<T, DK, DV, XT>::LDS;
-    constexpr size_t most = tiles + (BIAS ? 4 * (2 * (1024 + 31 * 16 + 31) + 1) * sizeof(float) : 0);
+    constexpr size_t most = tiles + (BIAS ? (5 * MAX_BAND + 4 * SQUARE) * sizeof(float) : 0);
     static_assert(most <= 160 * 1024, "LDS");
     auto kernel = &attn_dq_kernel<T, DK, DV, XT, BIAS>;
     static LdsReady ready;
@@ -551,17 +590,19 @@ int launch_dq(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
     BwdArgs a = f;
     a.coltiles = p.qtiles;
     a.nhist = p.nhist;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), tiles + 4 * (size_t)p.nhist * sizeof(float), st, a);
+    const size_t lds = tiles + (BIAS ? (2 * (size_t)f.pos.width + 1 + (p.nhist ? 4 * (size_t)(p.nhist + SQUARE) : 0)) * sizeof(float) : 0);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), lds, st, a);
     return check_launch("attention backward (queries)");
 }
 
 template <class T, int DK, int DV, int WK, int XT, bool BIAS>
 int launch_dkv(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
-    constexpr size_t lds = DkvCut<T, DK, DV, WK, XT>::LDS;
-    static_assert(lds <= 160 * 1024 && 2 * XT <= THREADS, "LDS");
+    constexpr size_t tiles = DkvCut<T, DK, DV, WK, XT>::LDS, most = tiles + (BIAS ? 2 * MAX_BAND * sizeof(float) : 0);
+    const size_t lds = tiles + (BIAS ? 2 * (2 * (size_t)f.pos.width + 1) * sizeof(float) : 0);
+    static_assert(most <= 160 * 1024 && 2 * XT <= THREADS, "LDS");
     auto kernel = &attn_dkv_kernel<T, DK, DV, WK, XT, BIAS>;
     static LdsReady ready;
-    if (ready.reserve("attention backward", reinterpret_cast<const void*>(kernel), lds)) return 1;
+    if (ready.reserve("attention backward", reinterpret_cast<const void*>(kernel), most)) return 1;
     const long long grid = (long long)f.B * f.KV * p.ktiles * p.nsplit;
     EEGGAN_REQUIRE(grid < (1ll << 31), "attention backward: too many workgroups");
     BwdArgs a = f;

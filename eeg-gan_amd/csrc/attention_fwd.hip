@@ -30,7 +30,7 @@ struct FwdArgs {
 };
 
 // KW waves share the columns and split a stage's keys; CB: column blocks of a wave (its LDS operands serve all of them).
-template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS>
+template <class T, int DK, int DV, int XT>
 struct FwdCut {
     static constexpr int NP = Elem<T>::NP;
     static constexpr int STAGE = TTile<NP, DK, XT>::BYTES + NTile<NP, DV, XT>::BYTES;
@@ -39,7 +39,7 @@ struct FwdCut {
 };
 template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
-    typedef FwdCut<T, DK, DV, KW, XT, CB, BIAS> Cut;
+    typedef FwdCut<T, DK, DV, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     constexpr int WC = 4 / KW;                  // waves along the columns
     constexpr int SUBS = XT / (32 * KW);        // key tiles a wave takes of a stage
@@ -63,8 +63,12 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
     bool live[CB];
     int t[CB], head[CB];
     SFrag<NP, DK> fq[CB];
-    const float* rel[CB];  // position bias: rel[step * s], relative to this lane's query
-    bool one_head[CB];     // (a block of columns of several heads is always near)
+    // position bias: beyond the last edge (behind, ahead) one value per lane; near tiles read band[distance + width] in LDS,
+    // or, where the block's columns belong to several heads (which never count as far), rel[step * s] in memory
+    float beyond[CB][2];
+    const float* rel[CB];
+    bool one_head[CB];
+    float* const bands = reinterpret_cast<float*>(smem + Cut::LDS) + wave * CB * (2 * a.pos.width + 1);
 #pragma unroll
     for (int i = 0; i < CB; ++i) {
         const int n0 = col0 + 32 * i, n = n0 + l31;
@@ -81,15 +85,24 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
         for (int e = 0; e < F::VALUES; ++e)
             x[e] = live[i] && F::channel(e, h) < a.Dk ? (NP == 3 ? x[e] * c : x[e]) : 0.f;
         fq[i].fill(h, x);
-        rel[i] = BIAS ? a.pos.rel + (long long)head[i] * a.pos.nrel + (a.Tq - 1 - t[i]) : nullptr;
-        one_head[i] = n0 < ncols && n0 / a.Tq == min(n0 + 31, ncols - 1) / a.Tq;
+        if constexpr (BIAS) {
+            const float* const mine = a.pos.rel + (long long)head[i] * a.pos.nrel;
+            rel[i] = mine + (a.Tq - 1 - t[i]);
+            one_head[i] = n0 < ncols && n0 / a.Tq == min(n0 + 31, ncols - 1) / a.Tq;
+            beyond[i][0] = rel_at(a.pos, mine, a.Tq, -a.pos.far);
+            beyond[i][1] = rel_at(a.pos, mine, a.Tq, a.pos.far);
+            if (one_head[i])  // (the whole wave is of one head: lane 0's)
+                fill_band(bands + i * (2 * a.pos.width + 1), a.pos,
+                          a.pos.rel + (long long)(kvh * a.G + n0 / a.Tq) * a.pos.nrel, a.Tq, lane, 64);
+        }
     }
     const T* const kb = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc;
     const T* const vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc;
     const unsigned char* const mask = a.mask ? a.mask + (long long)b * a.Tk : nullptr;
 
-    const int s_begin = split * a.split_keys;
-    const int s_end = min(a.Tk, s_begin + a.split_keys);
+    int s_begin = split * a.split_keys;
+    int s_end = min(a.Tk, s_begin + a.split_keys);
+    if (mask && s_begin < s_end) attended_range(mask, s_begin, s_end, reinterpret_cast<int*>(smem));
 
     float m[CB], l[CB], threshold[CB];  // threshold -inf: no key seen yet
     f32x16 o[CB][VT::GROUPS];
@@ -105,28 +118,29 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
     Block<T, DV, XT> vblk;
     kblk.init(a.ksc, a.Dk, tid);
     vblk.init(a.vsc, a.Dv, tid);
-    Steps<XT> ahead, now;  // which keys of the stage are attended
+    StepsAhead<XT> ahead;
+    Steps<XT> now, next;  // which keys of the stage are attended
     auto fetch = [&](int s0) {
+        ahead.load(s0, s_end, mask, lane);
         kblk.load(kb, s0, s_end, tid);
         vblk.load(vb, s0, s_end, tid);
-        ahead.find(s0, s_end, mask, lane);
     };
     auto put = [&](int buf) {
         char* const kt = smem + buf * Cut::STAGE;
-        kblk.template store<true, false>(kt, nullptr, a.Dk, ahead, tid);
-        vblk.template store<false, true>(nullptr, kt + KT::BYTES, a.Dv, ahead, tid);
+        next.find(ahead.x0, s_end, ahead.raw, lane);
+        kblk.template store<true, false>(kt, nullptr, a.Dk, next, tid);
+        vblk.template store<false, true>(nullptr, kt + KT::BYTES, a.Dv, next, tid);
     };
     int buf = 0;
     if (s_begin < s_end) {
         fetch(s_begin);
         put(0);
-        now = ahead;
+        now = next;
         if (s_begin + XT < s_end) fetch(s_begin + XT);
         __syncthreads();
     }
     for (int s0 = s_begin; s0 < s_end; s0 += XT) {
         // two buffers: the next stage goes into the other one before this one is worked on
-        const Steps<XT> next = ahead;
         if (Cut::BUFS == 2 && s0 + XT < s_end) {
             put(buf ^ 1);
             if (s0 + 2 * XT < s_end) fetch(s0 + 2 * XT);
@@ -141,7 +155,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
                 word[j] = now.tile(32 * (KW == 1 ? u + j : ksub));
                 any |= word[j];
             }
-            if (any == 0) continue;  // (the same for every lane of the wave)
+            if (any == 0 || col0 >= ncols) continue;  // (the same for every lane of the wave)
             f32x16 acc[J][CB];
 #pragma unroll
             for (int j = 0; j < J; ++j) {
@@ -156,12 +170,21 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
                 for (int j = 0; j < J; ++j) {
                     const int x0 = 32 * (KW == 1 ? u + j : ksub);
                     if constexpr (BIAS) {
-                        const int s = min(s0 + x0, a.Tk - 1);
-                        if (one_head[i] && tile_side(a.pos, s0 + x0, (col0 + 32 * i) % a.Tq) != 0) {
-                            const float base = rel[i][(long long)a.pos.step * s] - m[i];
+                        const int s = s0 + x0, n0 = col0 + 32 * i, t0 = n0 % a.Tq;
+                        const int side = one_head[i] ? tile_side(a.pos, s, t0) : 0;
+                        if (side != 0) {
+                            const float base = (side < 0 ? beyond[i][0] : beyond[i][1]) - m[i];
 #pragma unroll
                             for (int r = 0; r < 16; ++r)
                                 acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c, base);
+                        } else if (one_head[i]) {
+                            const float* const r0 = bands + i * (2 * a.pos.width + 1) +
+                                                    (int)((long long)a.pos.step * s + a.pos.offset - t0 + a.pos.width) +
+                                                    a.pos.step * 4 * h - l31;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c,
+                                                              r0[a.pos.step * ((r & 3) + 8 * (r >> 2))] - m[i]);
                         } else {
                             const int first = min(s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
                             const float* r0 = rel[i] + (long long)a.pos.step * first;
@@ -356,7 +379,7 @@ constexpr int WANTED = 512;
 template <class T, int DK, int DV>
 struct Cuts {
     static constexpr bool F32 = Elem<T>::NP == 3;
-    static constexpr int FEW_XT = F32 && DK + DV > 128 ? 64 : 128;  // keys of a stage: few columns / many
+    static constexpr int FEW_XT = F32 && DK + DV > 160 ? 32 : 64;  // keys of a stage: few columns / many
     static constexpr int XT = F32 && DK + DV > 96 ? 32 : 64;
     static constexpr int CB = DK + DV <= (F32 ? 64 : 128) ? 2 : 1;  // column blocks of a wave, where there are enough
 };
@@ -391,11 +414,12 @@ size_t part_bytes(const eeggan_attention& a, const FwdPlan& p) {
 
 template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS>
 int launch(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
-    constexpr size_t lds = FwdCut<T, DK, DV, KW, XT, CB, BIAS>::LDS;
-    static_assert(lds <= 160 * 1024, "LDS");
+    constexpr size_t tiles = FwdCut<T, DK, DV, XT>::LDS, most = tiles + (BIAS ? 4 * CB * MAX_BAND * sizeof(float) : 0);
+    static_assert(most <= 160 * 1024, "LDS");
+    const size_t lds = tiles + (BIAS ? 4 * CB * (2 * (size_t)f.pos.width + 1) * sizeof(float) : 0);
     auto kernel = &attn_fwd_kernel<T, DK, DV, KW, XT, CB, BIAS>;
     static LdsReady ready;
-    if (ready.reserve("attention", reinterpret_cast<const void*>(kernel), lds)) return 1;
+    if (ready.reserve("attention", reinterpret_cast<const void*>(kernel), most)) return 1;
     const long long grid = (long long)f.B * f.KV * p.nsplit * p.coltiles;
     EEGGAN_REQUIRE(grid < (1ll << 31), "attention: too many workgroups");
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(THREADS), lds, st, f);
@@ -405,7 +429,9 @@ int launch(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
 template <class T, int DK, int DV, bool BIAS>
 int launch_cut(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
     typedef Cuts<T, DK, DV> C;
-    if (p.kw > 1) return launch<T, DK, DV, C::FEW_XT / 32, C::FEW_XT, 1, BIAS>(f, p, st);
+    if constexpr (C::FEW_XT == 64) {
+        if (p.kw == 2) return launch<T, DK, DV, 2, 64, 1, BIAS>(f, p, st);
+    }
     if constexpr (C::CB == 2) {
         if (p.cb == 2) return launch<T, DK, DV, 1, C::XT, 2, BIAS>(f, p, st);
     }

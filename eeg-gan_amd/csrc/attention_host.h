@@ -24,6 +24,8 @@ struct LdsReady {
     }
 };
 
+constexpr size_t MAX_BAND = 2 * (1024 + 31 * 16 + 31) + 1;  // 2 width + 1 at the widest buckets
+
 int check_attention(const char* what, const eeggan_attention* a);
 // rel table of a call: entries per head, bytes (a multiple of 16), and the launch that fills it (nothing without a bias)
 inline long long positions_entries(const eeggan_attention& a) {

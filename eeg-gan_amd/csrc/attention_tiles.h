@@ -141,14 +141,11 @@ __device__ __forceinline__ int n_off(int x) { return 2 * ((x & ~31) + (x & 16) +
 template <int XT>
 struct Steps {
     unsigned long long w[(XT + 63) / 64];
-    // steps [x0, x0 + XT) of `len`, less the masked ones (mask: nonzero bytes count; null: all)
-    __device__ __forceinline__ void find(int x0, int len, const unsigned char* mask, int lane) {
+    // steps [x0, x0 + XT) of `len`, less the masked ones: `raw` is what StepsAhead read for them
+    __device__ __forceinline__ void find(int x0, int len, const unsigned char (&raw)[(XT + 63) / 64], int lane) {
 #pragma unroll
-        for (int i = 0; i < (XT + 63) / 64; ++i) {
-            const int x = x0 + 64 * i + lane;
-            const bool in = 64 * i + lane < XT && x < len;
-            w[i] = __ballot(mask ? in && mask[x < len ? x : len - 1] : in);
-        }
+        for (int i = 0; i < (XT + 63) / 64; ++i)
+            w[i] = __ballot(64 * i + lane < XT && x0 + 64 * i + lane < len && raw[i] != 0);
     }
     __device__ __forceinline__ bool all() const {
         bool a = true;
@@ -163,6 +160,43 @@ struct Steps {
         return (unsigned)((XT > 64 && kq >= 16 ? w[(XT + 63) / 64 - 1] : w[0]) >> (4 * (kq & 15))) & 15u;
     }
 };
+
+// The mask bytes of a stage on their way: read with the stage's data and looked at only when that is stored (a vote right
+// behind the loads would wait for all of them).
+template <int XT>
+struct StepsAhead {
+    unsigned char raw[(XT + 63) / 64];
+    int x0;
+    // mask: nonzero bytes count; null: all
+    __device__ __forceinline__ void load(int first, int len, const unsigned char* mask, int lane) {
+        x0 = first;
+#pragma unroll
+        for (int i = 0; i < (XT + 63) / 64; ++i) raw[i] = mask ? mask[min(first + 64 * i + lane, len - 1)] : 1;
+    }
+};
+
+// The attended keys of [begin, end) lie in the range this leaves (end <= begin: none); all threads, ends in a barrier.
+__device__ __forceinline__ void attended_range(const unsigned char* mask, int& begin, int& end, int* lds) {
+    int lo = end, hi = begin;
+    for (int x = begin + (int)threadIdx.x; x < end; x += THREADS)
+        if (mask[x]) {
+            lo = min(lo, x);
+            hi = x + 1;
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o, 64));
+        hi = max(hi, __shfl_xor(hi, o, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        lds[2 * (threadIdx.x >> 6)] = lo;
+        lds[2 * (threadIdx.x >> 6) + 1] = hi;
+    }
+    __syncthreads();
+    begin = __builtin_amdgcn_readfirstlane(min(min(lds[0], lds[2]), min(lds[4], lds[6])));
+    end = __builtin_amdgcn_readfirstlane(max(max(lds[1], lds[3]), max(lds[5], lds[7])));
+    __syncthreads();
+}
 
 // A [D, XT] block of a channels-first matrix on its way from memory into LDS: 4 x 4 units (four channels, four time
 // steps).  A wave takes 8 x 8 units where the block has them (its transposed writes then fall on all LDS banks: rows of
@@ -332,41 +366,82 @@ struct SFrag {
     }
 };
 
-// acc[b][x, column] += sum_d tile[x, d] frag[b][d, column] for the 32 rows from `row` (= tile + (first row + lane & 31)
-// * RS) and CB column blocks: every operand read from LDS serves all of them.
+// The operands of a scores-like product for the 32 rows from `row` (= tile + (first row + lane & 31) * RS).
+template <int NP, int D, int XT>
+struct SRead {
+    static constexpr int N = packed8<NP, D>() ? 3 : NP * D / 16;
+    bf16x8 a[N];
+    __device__ __forceinline__ void load(const char* row, int h) {
+        if constexpr (packed8<NP, D>()) {
+            a[0] = lds8(row + 32 * h);
+            a[1] = lds8(row + 16);
+            a[2] = lds8(row);
+        } else {
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                for (int p = 0; p < NP; ++p) a[NP * j + p] = lds8(row + 32 * j + 16 * h + p * TTile<NP, D, XT>::PIECE);
+        }
+    }
+    // acc[b][x, column] += sum_d tile[x, d] frag[b][d, column] for CB column blocks: every operand serves all of them
+    template <int CB>
+    __device__ __forceinline__ void mma(const SFrag<NP, D> (&s)[CB], f32x16 (&acc)[CB]) const {
+        if constexpr (packed8<NP, D>()) {
+#pragma unroll
+            for (int b = 0; b < CB; ++b) acc[b] = mfma(a[0], s[b].f[1], acc[b]);  // p1 q3 | p3 q1
+#pragma unroll
+            for (int b = 0; b < CB; ++b) acc[b] = mfma(a[1], s[b].f[0], acc[b]);  // p2 q1 | p2 q2
+#pragma unroll
+            for (int b = 0; b < CB; ++b) acc[b] = mfma(a[2], s[b].f[0], acc[b]);  // p1 q1 | p1 q2
+        } else {
+            constexpr int J = D / 16;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                if constexpr (NP == 3) {
+                    const bf16x8 &a0 = a[3 * j], &a1 = a[3 * j + 1], &a2 = a[3 * j + 2];
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) acc[b] = mfma(a2, s[b].f[j], acc[b]);
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[2 * J + j], acc[b]);
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[J + j], acc[b]);
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[j], acc[b]);
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[J + j], acc[b]);
+                }
+#pragma unroll
+                for (int b = 0; b < CB; ++b) acc[b] = mfma(a[NP * j], s[b].f[j], acc[b]);
+            }
+        }
+    }
+};
+// Whether a tile's operands are all read before the first product: up to this many (the compiler reads each one right
+// before its product and waits for it; past that the registers do not hold them).
+constexpr int READ_AHEAD = 9;
+
 template <int NP, int D, int XT, int CB>
 __device__ __forceinline__ void mma_scores(const char* row, int h, const SFrag<NP, D> (&s)[CB], f32x16 (&acc)[CB]) {
-    typedef TTile<NP, D, XT> TL;
-    if constexpr (packed8<NP, D>()) {
-        const bf16x8 a0 = lds8(row + 32 * h), a1 = lds8(row + 16), a2 = lds8(row);
-#pragma unroll
-        for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[1], acc[b]);  // p1 q3 | p3 q1
-#pragma unroll
-        for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[0], acc[b]);  // p2 q1 | p2 q2
-#pragma unroll
-        for (int b = 0; b < CB; ++b) acc[b] = mfma(a2, s[b].f[0], acc[b]);  // p1 q1 | p1 q2
+    SRead<NP, D, XT> r;
+    r.load(row, h);
+    if constexpr (SRead<NP, D, XT>::N <= READ_AHEAD) __builtin_amdgcn_sched_barrier(0);
+    r.template mma<CB>(s, acc);
+}
+// scores and dP of a tile
+template <int NP, int DK, int DV, int XT>
+__device__ __forceinline__ void two_scores(const char* k, const SFrag<NP, DK> (&fk)[1], f32x16 (&s)[1], const char* v,
+                                           const SFrag<NP, DV> (&fv)[1], f32x16 (&dp)[1], int h) {
+    if constexpr (SRead<NP, DK, XT>::N + SRead<NP, DV, XT>::N <= READ_AHEAD) {
+        SRead<NP, DK, XT> rk;
+        SRead<NP, DV, XT> rv;
+        rk.load(k, h);
+        rv.load(v, h);
+        __builtin_amdgcn_sched_barrier(0);
+        rk.template mma<1>(fk, s);
+        rv.template mma<1>(fv, dp);
     } else {
-        constexpr int J = D / 16;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const char* p = row + 32 * j + 16 * h;
-            const bf16x8 a0 = lds8(p);
-            if constexpr (NP == 3) {
-                const bf16x8 a1 = lds8(p + TL::PIECE), a2 = lds8(p + 2 * TL::PIECE);
-#pragma unroll
-                for (int b = 0; b < CB; ++b) acc[b] = mfma(a2, s[b].f[j], acc[b]);
-#pragma unroll
-                for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[2 * J + j], acc[b]);
-#pragma unroll
-                for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[J + j], acc[b]);
-#pragma unroll
-                for (int b = 0; b < CB; ++b) acc[b] = mfma(a1, s[b].f[j], acc[b]);
-#pragma unroll
-                for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[J + j], acc[b]);
-            }
-#pragma unroll
-            for (int b = 0; b < CB; ++b) acc[b] = mfma(a0, s[b].f[j], acc[b]);
-        }
+        mma_scores<NP, DK, XT, 1>(k, h, fk, s);
+        mma_scores<NP, DV, XT, 1>(v, h, fv, dp);
     }
 }
 
@@ -459,12 +534,24 @@ struct Positions {
     const float* rel;  // null: no bias
     int nrel;          // entries per head
     int step, offset, far;
+    int width;  // near tiles hold distances -width .. width: far + 31 step + 31
 };
 
 // -1 / +1: every pair of the 32 x 32 tile lies beyond `far` on that side; 0: near.  s: first key, t: first query.
-__device__ __forceinline__ int tile_side(const Positions& p, long long s, long long t) {
-    const long long lo = p.step * s + p.offset - (t + 31), hi = p.step * (s + 31) + p.offset - t;
+__device__ __forceinline__ int tile_side(const Positions& p, int s, int t) {
+    const long long base = (long long)p.step * s + p.offset - t;
+    const long long lo = base - 31, hi = base + 31 * p.step;
     return lo >= p.far ? 1 : hi <= -p.far ? -1 : 0;
+}
+// entry of a head's table for a distance (clamped: a value past the table belongs to no pair)
+__device__ __forceinline__ float rel_at(const Positions& p, const float* head, int tq, long long distance) {
+    const long long i = distance - p.offset + (tq - 1);
+    return head[i < 0 ? 0 : i >= p.nrel ? p.nrel - 1 : i];
+}
+// The near distances' values in LDS (2 width + 1 floats): read from memory inside the loop over the tiles they cost a
+// trip to the L2 per tile, which nothing hides at two waves per SIMD.
+__device__ __forceinline__ void fill_band(float* band, const Positions& p, const float* head, int tq, int first, int stride) {
+    for (int i = first; i <= 2 * p.width; i += stride) band[i] = rel_at(p, head, tq, i - p.width);
 }
 
 }  // namespace attn

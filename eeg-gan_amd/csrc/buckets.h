@@ -11,6 +11,9 @@ inline __host__ __device__ int bucket_far(const eeggan_buckets& b) {
     return last > 1 ? last : 1;
 }
 
+// a 32 x 32 tile of pairs with one within `far` holds distances up to this
+inline __host__ __device__ int band_width(const eeggan_buckets& b) { return bucket_far(b) + 31 * b.step + 31; }
+
 __device__ __forceinline__ int bucket_of(const eeggan_buckets& b, long long rel) {
     const int side = bucket_side(b);
     long long dist = rel < 0 ? -rel : rel;

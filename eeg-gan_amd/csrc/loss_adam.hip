@@ -542,7 +542,7 @@ namespace {
 // Squares and sums are formed in double (one pass over the gradients, bound by reading them: the double-rate fma keeps
 // up with four bytes per element), so no gradient overflows or vanishes on the way and the result does not depend on the
 // cut.  Every workgroup leaves one partial sum and one workgroup adds those up in a fixed order: two launches, no atomics.
-constexpr int64_t NCHUNK = 256 * 4 * 8;
+constexpr int64_t NCHUNK = 256 * 4 * 8;  // elements of a step: eight 16-byte loads per thread in flight
 constexpr int NMAXT = 160;
 
 struct NormPack {
@@ -550,7 +550,9 @@ struct NormPack {
     int64_t n[NMAXT];
     int first[NMAXT];  // first chunk of the tensor
     int count;
+    int chunks;
 };
+constexpr int NORM_BLOCKS = 2048;  // eight workgroups to a CU: each walks the chunks at this distance
 
 // index of the tensor that owns workgroup `blk` (chunk counts ascend)
 template <class P>
@@ -566,29 +568,30 @@ __device__ __forceinline__ int owner(const P& pk, int blk) {
 
 __global__ __launch_bounds__(256) void grad_square_kernel(NormPack pk, double* __restrict__ part) {
     __shared__ double red[4];
-    const int ti = owner(pk, blockIdx.x);
-    const float* g = pk.g[ti];
-    const int64_t start = (int64_t)(blockIdx.x - pk.first[ti]) * NCHUNK;
-    const int64_t left = pk.n[ti] - start;
-    const int n = (int)(left < NCHUNK ? left : NCHUNK);
-    g += start;
     double s = 0.0;
-    const int n4 = n / 4;
-    if (n4 == (int)(NCHUNK / 4)) {
-        f32x4 v[8];
+    int ti = owner(pk, blockIdx.x);
+    for (int chunk = blockIdx.x; chunk < pk.chunks; chunk += gridDim.x) {
+        while (ti + 1 < pk.count && pk.first[ti + 1] <= chunk) ++ti;
+        const int64_t start = (int64_t)(chunk - pk.first[ti]) * NCHUNK;
+        const float* g = pk.g[ti] + start;
+        const int64_t left = pk.n[ti] - start;
+        if (left >= NCHUNK) {
+            f32x4 v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4u*>(g + 4 * (threadIdx.x + 256 * u));
+            for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4u*>(g + 4 * (threadIdx.x + 256 * u));
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+            for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_fma((double)v[u][e], (double)v[u][e], s);
-    } else {
-        for (int i = threadIdx.x; i < n4; i += 256) {
-            const f32x4 v = *reinterpret_cast<const f32x4u*>(g + 4 * i);
+                for (int e = 0; e < 4; ++e) s = __builtin_fma((double)v[u][e], (double)v[u][e], s);
+        } else {
+            const int n = (int)left, n4 = n / 4;
+            for (int i = threadIdx.x; i < n4; i += 256) {
+                const f32x4 v = *reinterpret_cast<const f32x4u*>(g + 4 * i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = __builtin_fma((double)v[e], (double)v[e], s);
+                for (int e = 0; e < 4; ++e) s = __builtin_fma((double)v[e], (double)v[e], s);
+            }
+            for (int i = 4 * n4 + threadIdx.x; i < n; i += 256) s = __builtin_fma((double)g[i], (double)g[i], s);
         }
-        for (int i = 4 * n4 + threadIdx.x; i < n; i += 256) s = __builtin_fma((double)g[i], (double)g[i], s);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -638,12 +641,10 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(NormPack pk, const floa
     const float c = norm[1];
     if (c == 1.f) return;
     const int ti = owner(pk, blockIdx.x);
-    float* g = const_cast<float*>(pk.g[ti]);
     const int64_t start = (int64_t)(blockIdx.x - pk.first[ti]) * NCHUNK;
+    float* g = const_cast<float*>(pk.g[ti]) + start;
     const int64_t left = pk.n[ti] - start;
-    const int n = (int)(left < NCHUNK ? left : NCHUNK);
-    g += start;
-    const int n4 = n / 4;
+    const int n = (int)(left < NCHUNK ? left : NCHUNK), n4 = n / 4;
     f32x4 v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -731,21 +732,26 @@ int check_grads(const char* what, const eeggan_adam_tensor* table, int ntensors)
     }
     return 0;
 }
-int64_t norm_parts(const eeggan_adam_tensor* table, int ntensors) {
-    int64_t parts = 0;
-    for (int i = 0; i < ntensors; ++i) parts += (table[i].n + NCHUNK - 1) / NCHUNK;
-    return parts;
-}
 int make_norm_pack(const eeggan_adam_tensor* table, int first, int ntensors, NormPack* pk) {
     pk->count = ntensors - first < NMAXT ? ntensors - first : NMAXT;
-    int blocks = 0;
+    int chunks = 0;
     for (int i = 0; i < pk->count; ++i) {
         pk->g[i] = table[first + i].g;
         pk->n[i] = table[first + i].n;
-        pk->first[i] = blocks;
-        blocks += (int)((table[first + i].n + NCHUNK - 1) / NCHUNK);
+        pk->first[i] = chunks;
+        chunks += (int)((table[first + i].n + NCHUNK - 1) / NCHUNK);
     }
-    return blocks;
+    return pk->chunks = chunks;
+}
+// partial sums of a whole table: those of every launch (of up to NMAXT tensors)
+int64_t norm_parts(const eeggan_adam_tensor* table, int ntensors) {
+    int64_t parts = 0;
+    for (int first = 0; first < ntensors; first += NMAXT) {
+        int64_t chunks = 0;
+        for (int i = first; i < ntensors && i < first + NMAXT; ++i) chunks += (table[i].n + NCHUNK - 1) / NCHUNK;
+        parts += chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS;
+    }
+    return parts;
 }
 // the partial sums; their number goes to *nparts
 int launch_squares(const char* what, const eeggan_adam_tensor* table, int ntensors, double* part, int64_t* nparts,
@@ -753,7 +759,7 @@ int launch_squares(const char* what, const eeggan_adam_tensor* table, int ntenso
     *nparts = 0;
     for (int first = 0; first < ntensors; first += NMAXT) {
         NormPack pk;
-        const int blocks = make_norm_pack(table, first, ntensors, &pk);
+        const int chunks = make_norm_pack(table, first, ntensors, &pk), blocks = chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS;
         hipLaunchKernelGGL(grad_square_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pk, part + *nparts);
         if (check_launch(what)) return 1;
         *nparts += blocks;

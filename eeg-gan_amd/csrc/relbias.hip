@@ -37,7 +37,8 @@ __device__ __forceinline__ void fill_lut(float* lut, const float* table, const e
 // out[n, s, t] = scores[n, s, t] + table[bucket(step s + offset - t), n % H].  A pure stream: a workgroup takes `rows`
 // consecutive rows (n, s) of one n, its threads neighbouring groups of four steps; the value comes from LDS (one read
 // per element, a tenth of what LDS can deliver at the rate the memory can).
-template <bool NT>
+// NT: streaming accesses; HAVE: with scores.
+template <bool NT, bool HAVE>
 __global__ __launch_bounds__(256) void relbias_kernel(const float* __restrict__ scores, const float* __restrict__ table,
                                                       float* __restrict__ out, eeggan_buckets bk, int H, int Tk, int Tq,
                                                       int rows, int chunks) {
@@ -48,50 +49,58 @@ __global__ __launch_bounds__(256) void relbias_kernel(const float* __restrict__ 
     const int s1 = min(Tk, s0 + rows);
     fill_lut(lut, table, bk, H, (int)(n % H), far);
     __syncthreads();
+    if (Tq < 4) {
+        for (int i = threadIdx.x; i < (s1 - s0) * Tq; i += 256) {
+            const int s = s0 + i / Tq, t = i % Tq;
+            const long long at = (n * Tk + s) * Tq + t, d = (long long)t - (long long)bk.step * s - bk.offset + far;
+            out[at] = (scores ? scores[at] : 0.f) + lut[d < 0 ? 0 : d > 2 * far ? 2 * far : (int)d];
+        }
+        return;
+    }
+    // a row's last quad starts at Tq - 4: where it overlaps its neighbour both store the same values
     const int quads = (Tq + 3) / 4;
     const int drow = 256 / quads, dq = 256 % quads;  // (a thread's next item, without a division per item)
     int s = s0 + (int)threadIdx.x / quads, q = (int)threadIdx.x % quads;
-    for (; s < s1;) {
-        const int t = 4 * q;
-        const long long at = (n * Tk + s) * Tq + t;
-        // lut index of the quad's first step (far outside: just outside)
-        const long long wide = (long long)t - (long long)bk.step * s - bk.offset + far;
-        const int i0 = (int)(wide < -4 ? -4 : wide > 2 * far ? 2 * far : wide);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        const int have = min(4, Tq - t);
-        if (scores) {
-            if (have == 4) {
-                const f32x4u* p = reinterpret_cast<const f32x4u*>(scores + at);
-                v = NT ? __builtin_nontemporal_load(p) : *p;
-            } else {
-                v = load_few(scores + at, have);
+    const long long first = n * Tk * Tq;
+    constexpr int U = 4;  // items in flight per thread (past the end: the last row again, not stored)
+    while (s < s1) {
+        int is[U], it[U];
+        f32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            is[u] = s, it[u] = min(4 * q, Tq - 4);
+            const f32x4u* p = reinterpret_cast<const f32x4u*>(scores + first + (long long)min(s, s1 - 1) * Tq + it[u]);
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+            v[u] = HAVE ? (f32x4)(NT ? __builtin_nontemporal_load(p) : *p) : zero;
+            q += dq;
+            s += drow;
+            if (q >= quads) {
+                q -= quads;
+                ++s;
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] += lut[min(max(i0 + e, 0), 2 * far)];
-        }
-        if (have == 4) {
-            const f32x4u o = v;
-            if (NT) __builtin_nontemporal_store(o, reinterpret_cast<f32x4u*>(out + at));
-            else *reinterpret_cast<f32x4u*>(out + at) = o;
-        } else {
-            for (int e = 0; e < have; ++e) out[at + e] = v[e];
-        }
-        q += dq;
-        s += drow;
-        if (q >= quads) {
-            q -= quads;
-            ++s;
+        for (int u = 0; u < U; ++u) {
+            // lut index of the quad's first step (far outside: just outside)
+            const long long wide = (long long)it[u] - (long long)bk.step * is[u] - bk.offset + far;
+            const int i0 = (int)(wide < -4 ? -4 : wide > 2 * far ? 2 * far : wide);
+            f32x4u o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = v[u][e] + lut[min(max(i0 + e, 0), 2 * far)];
+            f32x4u* p = reinterpret_cast<f32x4u*>(out + first + (long long)is[u] * Tq + it[u]);
+            if (is[u] < s1) {
+                if (NT) __builtin_nontemporal_store(o, p);
+                else *p = o;
+            }
         }
     }
 }
 
-// Sums of g by distance.  A wave takes every fourth of its workgroup's rows.  In a row the distances beyond the last
-// edge are two contiguous stretches, added up as a stream; the band between them goes to a histogram by distance in LDS
-// whose entries each belong to one lane of the wave: no atomics, a fixed order, and double throughout (the near entries
-// of a long recording sum millions of terms).  hist: [H][rows of partial sums][2 far + 1]: distances -(far - 1) ..
-// far - 1, then everything behind, then everything ahead.
+// Sums of g by distance.  A wave takes every fourth of its workgroup's rows, 2048 values of a row at a time with all
+// loads in flight.  Four neighbouring values beyond the last edge on one side (most of a long row) go to one sum; the
+// others to a histogram by distance in LDS that belongs to the wave (within an instruction no two lanes share a
+// distance): a fixed order, and double throughout (the near entries of a long recording sum millions of terms).  hist:
+// [H][rows of partial sums][2 far + 1]: distances -(far - 1) .. far - 1, then everything behind, then everything ahead.
 __global__ __launch_bounds__(256) void relbias_sums_kernel(const float* __restrict__ g, double* __restrict__ hist,
                                                            eeggan_buckets bk, int B, int H, int Tk, int Tq, int rows,
                                                            int chunks) {
@@ -103,45 +112,60 @@ __global__ __launch_bounds__(256) void relbias_sums_kernel(const float* __restri
     const long long bh = blockIdx.x / chunks;
     const int chunk = (int)(blockIdx.x % chunks);
     const int s0 = chunk * rows, s1 = min(Tk, s0 + rows);
-    double beyond[2] = {0.0, 0.0};
+    double behind = 0.0, ahead = 0.0;
+    constexpr int U = 8;
     for (int s = s0 + wave; s < s1; s += 4) {
         const float* row = g + (bh * Tk + s) * Tq;
         const long long key = (long long)bk.step * s + bk.offset;  // distance of step t: key - t
         // steps [0, a): ahead of them by `far` or more; [a, b): the band; [b, Tq): behind
         const int a = (int)min((long long)Tq, max(0ll, key - far + 1)), b = (int)min((long long)Tq, max(0ll, key + far));
+        const int at_a = (int)(key - a + width);  // histogram entry of step a (meaningful where the band has steps)
+        for (int t0 = 0; t0 < Tq; t0 += 256 * U) {
+            f32x4 v[U];
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const int from = side ? b : 0, to = side ? Tq : a;
-            double sum = 0.0;
-            int t = from + 4 * lane;
-            for (; t + 3 * 256 + 3 < to; t += 4 * 256) {
-                f32x4 v[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = load4(row + t + 256 * u);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) sum += (double)((v[u][0] + v[u][1]) + (v[u][2] + v[u][3]));
+            for (int u = 0; u < U; ++u) {
+                // (a row's last values are read in the quad that starts at Tq - 4 and moved to their places below)
+                const int t = t0 + 256 * u + 4 * lane;
+                v[u] = Tq >= 4 ? load4(row + min(t, Tq - 4)) : load_few(row, Tq);
             }
-            for (; t < to; t += 256) {
-                f32x4 v;
-                if (t + 3 < to) v = load4(row + t);
-                else v = load_few(row + t, to - t);
-                sum += (double)((v[0] + v[1]) + (v[2] + v[3]));
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int t = t0 + 256 * u + 4 * lane, over = Tq >= 4 ? t - min(t, Tq - 4) : t;
+                if (over > 0) {
+                    const f32x4 w = v[u];
+                    v[u][0] = over == 1 ? w[1] : over == 2 ? w[2] : over == 3 ? w[3] : 0.f;
+                    v[u][1] = over == 1 ? w[2] : over == 2 ? w[3] : 0.f;
+                    v[u][2] = over == 1 ? w[3] : 0.f;
+                    v[u][3] = 0.f;
+                }
             }
-            beyond[side] += sum;
-        }
-        // band index of step t: key - t + width; lane owns the indices = lane mod 64
-        if (a < b) {
-            const int i0 = (int)(key - (b - 1) + width), i1 = (int)(key - a + width);
-            for (int i = (i0 & ~63) + lane; i <= i1; i += 64)
-                if (i >= i0) mine[i] += (double)row[key + width - i];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int t = t0 + 256 * u + 4 * lane;
+                if (t + 4 <= a) {
+                    ahead += (double)((v[u][0] + v[u][1]) + (v[u][2] + v[u][3]));
+                } else if (t >= b) {
+                    behind += (double)((v[u][0] + v[u][1]) + (v[u][2] + v[u][3]));  // (zeros past the row)
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (t + e < a) ahead += (double)v[u][e];
+                        else if (t + e >= b) behind += (double)v[u][e];
+                        else
+                            __hip_atomic_fetch_add(mine + (at_a - (t + e - a)), (double)v[u][e], __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+                    }
+                }
+            }
         }
     }
-#pragma unroll
-    for (int side = 0; side < 2; ++side)
-        for (int o = 32; o > 0; o >>= 1) beyond[side] += __shfl_xor(beyond[side], o, 64);
+    for (int o = 32; o > 0; o >>= 1) {
+        behind += __shfl_xor(behind, o, 64);
+        ahead += __shfl_xor(ahead, o, 64);
+    }
     if (lane == 0) {
-        mine[n] = beyond[1];
-        mine[n + 1] = beyond[0];
+        mine[n] = behind;
+        mine[n + 1] = ahead;
     }
     __syncthreads();
     const long long b = bh / H, h = bh % H;
@@ -174,7 +198,16 @@ __global__ __launch_bounds__(256) void bucket_sums_kernel(const TH* __restrict__
     const int n = max(0, hi - lo + 1), stride = 2 * width + 3;
     const TH* const h0 = hist + (long long)head * rows * stride;
     double sum = 0.0;
-    for (long long k = threadIdx.x; k < rows * n; k += 256) sum += (double)h0[(k / n) * stride + lo + k % n];
+    if (n > 0) {
+        // neighbouring threads on neighbouring entries, as many rows at a time as fit, eight loads in flight
+        const int w = min(n, 256), at = (int)threadIdx.x % w, step = 256 / w, r0 = (int)threadIdx.x / w;
+        if (r0 < step)
+            for (int i = at; i < n; i += w) {
+                const TH* p = h0 + lo + i;
+#pragma unroll 8
+                for (int r = r0; r < (int)rows; r += step) sum += (double)p[(long long)r * stride];
+            }
+    }
     for (long long r = threadIdx.x; r < rows; r += 256) {
         if (behind_at >= 0) sum += (double)h0[r * stride + behind_at];
         if (ahead_at >= 0) sum += (double)h0[r * stride + ahead_at];
@@ -219,12 +252,12 @@ int check_attention(const char* what, const eeggan_attention* a) {
 
 int positions(const eeggan_attention& a, float* rel, Positions* p, hipStream_t st) {
     if (!a.table) {
-        *p = Positions{nullptr, 0, 1, 0, 1};
+        *p = Positions{nullptr, 0, 1, 0, 1, 0};
         return 0;
     }
     const eeggan_buckets bk = *a.buckets;
     const int nrel = (int)positions_entries(a);
-    *p = Positions{rel, nrel, bk.step, bk.offset, bucket_far(bk)};
+    *p = Positions{rel, nrel, bk.step, bk.offset, bucket_far(bk), band_width(bk)};
     const dim3 grid((unsigned)((nrel + 255) / 256), (unsigned)a.H);
     const int first = bk.offset - (a.Tq - 1);
     if (a.table_bf16)
@@ -287,17 +320,15 @@ extern "C" int eeggan_relative_bias(const float* scores, const float* table, con
                                     int B, int H, int Tk, int Tq, void* stream) {
     EEGGAN_REQUIRE(table && out, "relative_bias: null pointer");
     if (check_relbias("relative_bias", buckets, B, H, Tk, Tq)) return 1;
-    // about 16 K elements to a workgroup: enough to hide the table, few enough to fill the chip
+    // 16 K elements to a workgroup: enough to hide its start (the table in LDS), few enough to fill the chip
     const Rows r = rows_of((long long)B * H, Tk, Tq, 16384);
     EEGGAN_REQUIRE(r.blocks < (1ll << 31), "relative_bias: too many rows");
     const size_t lds = (2 * (size_t)bucket_far(*buckets) + 1) * sizeof(float);
     const dim3 grid((unsigned)r.blocks);
-    if (streams_past_caches((size_t)B * H * Tk * Tq * sizeof(float) * (scores ? 2 : 1)))
-        hipLaunchKernelGGL(relbias_kernel<true>, grid, dim3(256), lds, as_stream(stream), scores, table, out, *buckets, H, Tk,
-                           Tq, r.rows, r.chunks);
-    else
-        hipLaunchKernelGGL(relbias_kernel<false>, grid, dim3(256), lds, as_stream(stream), scores, table, out, *buckets, H,
-                           Tk, Tq, r.rows, r.chunks);
+    const bool nt = streams_past_caches((size_t)B * H * Tk * Tq * sizeof(float) * (scores ? 2 : 1));
+    auto kernel = nt ? (scores ? &relbias_kernel<true, true> : &relbias_kernel<true, false>)
+                     : (scores ? &relbias_kernel<false, true> : &relbias_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, as_stream(stream), scores, table, out, *buckets, H, Tk, Tq, r.rows, r.chunks);
     return check_launch("relative_bias");
 }
 
