@@ -36,7 +36,7 @@ struct BwdArgs {
 template <class T, int DK, int DV, int XT>
 struct DqCut {
     static constexpr int NP = Elem<T>::NP;
-    static constexpr int STAGE = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES + TTile<NP, DV, XT>::BYTES;
+    static constexpr int STAGE = Tile<NP, DK, XT>::BYTES + Tile<NP, DV, XT>::BYTES;
     static constexpr int BUFS = 2 * STAGE <= 64 * 1024 ? 2 : 1;  // (two workgroups to a CU, with room for histograms)
     static constexpr int LDS = BUFS * STAGE;
 };
@@ -45,9 +45,7 @@ template <class T, int DK, int DV, int XT, bool BIAS>
 __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     typedef DqCut<T, DK, DV, XT> Cut;
     constexpr int NP = Elem<T>::NP;
-    typedef TTile<NP, DK, XT> KT;
-    typedef NTile<NP, DK, XT> KN;
-    typedef TTile<NP, DV, XT> VT;
+    typedef Tile<NP, DK, XT> KT;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
@@ -58,6 +56,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     const int b = group / a.KV, kvh = group - b * a.KV;
     const int tile = part_of % a.coltiles, head = kvh * a.G + part_of / a.coltiles;
 
+    const int k_off = SRead<NP, DK, XT>::offset(lane), v_off = SRead<NP, DV, XT>::offset(lane);
     const int t0 = (tile * 4 + wave) * 32;
     const bool inside = t0 + l31 < a.Tq;
     const int t = inside ? t0 + l31 : 0;
@@ -115,9 +114,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     f32x16 dinit;
 #pragma unroll
     for (int r = 0; r < 16; ++r) dinit[r] = -delta;
-    f32x16 dq[1][KN::GROUPS];
+    f32x16 dq[1][KT::GROUPS];
 #pragma unroll
-    for (int i = 0; i < KN::GROUPS; ++i) dq[0][i] = zero16();
+    for (int i = 0; i < KT::GROUPS; ++i) dq[0][i] = zero16();
 
     double beyond[2] = {0.0, 0.0};  // sums of dS over far tiles, behind / ahead of the query (thousands of terms)
     float* const hist = BIAS ? band + (2 * a.pos.width + 1) + wave * a.nhist : nullptr;
@@ -143,8 +142,8 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     auto put = [&](int buf) {
         char* const kt = smem + buf * Cut::STAGE;
         next.find(ahead.x0, s_end, ahead.raw, lane);
-        kblk.template store<true, true>(kt, kt + KT::BYTES, a.Dk, next, tid);
-        vblk.template store<true, false>(kt + KT::BYTES + KN::BYTES, nullptr, a.Dv, next, tid);
+        kblk.store(kt, a.Dk, next, tid);
+        vblk.store(kt + KT::BYTES, a.Dv, next, tid);
     };
     int buf = 0;
     if (s_begin < s_end) {
@@ -160,8 +159,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
             if (s0 + 2 * XT < s_end) fetch(s0 + 2 * XT);
         }
         const char* const kt = smem + buf * Cut::STAGE;
-        const char* const kn = kt + KT::BYTES;
-        const char* const vt = kn + KN::BYTES;
+        const char* const vt = kt + KT::BYTES;
 #pragma unroll
         for (int u = 0; u < XT / 32; ++u) {
             const int x0 = 32 * u;
@@ -171,7 +169,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
             // (the scores accumulate from zero and meet lse once: on top of -lse every partial sum would be rounded at
             // its magnitude)
             f32x16 raw[1] = {zero16()}, dsv[1] = {dinit};
-            two_scores<NP, DK, DV, XT>(kt + (x0 + l31) * KT::RS, fq, raw, vt + (x0 + l31) * VT::RS, fg, dsv, h);
+            two_scores<NP, DK, DV, XT>(kt + 2 * x0 + k_off, fq, raw, vt + 2 * x0 + v_off, fg, dsv, h);
             f32x16 &acc = raw[0], &ds = dsv[0];
             const float k1 = NP == 3 ? 1.f : c;
             int side = 0;
@@ -226,7 +224,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
             }
             PFrag<NP> p[1];
             p[0].fill(ds);
-            mma_values<NP, DK, XT, 1>(kn, x0, l31, h, p, dq);
+            mma_values<NP, DK, XT, 1>(kt, x0, l31, h, p, dq);
         }
         if (s0 + XT < s_end) {
             __syncthreads();
@@ -244,11 +242,11 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
         eight_rows<NP, DK>(dq[0][0]);
         T* out = reinterpret_cast<T*>(a.gq) + row * a.Dk * a.Tq + t;
 #pragma unroll
-        for (int i = 0; i < KN::GROUPS; ++i)
+        for (int i = 0; i < KT::GROUPS; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * i + acc_row(r, h);
-                if (d < a.Dk && (!KN::P8 || r < 4)) st1(out + (long long)d * a.Tq, live ? dq[0][i][r] * a.scale : 0.f);
+                if (d < a.Dk && (!KT::P8 || r < 4)) st1(out + (long long)d * a.Tq, live ? dq[0][i][r] * a.scale : 0.f);
             }
     }
     if constexpr (BIAS) {
@@ -274,10 +272,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
 template <class T, int DK, int DV, int WK, int XT>
 struct DkvCut {
     static constexpr int NP = Elem<T>::NP;
-    static constexpr int Q = TTile<NP, DK, XT>::BYTES + NTile<NP, DK, XT>::BYTES;
-    static constexpr int STAGE = Q + TTile<NP, DV, XT>::BYTES + NTile<NP, DV, XT>::BYTES + 2 * XT * (int)sizeof(float);
+    static constexpr int STAGE = Tile<NP, DK, XT>::BYTES + Tile<NP, DV, XT>::BYTES + 2 * XT * (int)sizeof(float);
     static constexpr int BUFS = 2 * STAGE <= 80 * 1024 ? 2 : 1;
-    static constexpr int WORDS = (NTile<NP, DK, XT>::GROUPS + NTile<NP, DV, XT>::GROUPS) * 16 * 64;  // a wave's sums
+    static constexpr int WORDS = (Tile<NP, DK, XT>::GROUPS + Tile<NP, DV, XT>::GROUPS) * 16 * 64;  // a wave's sums
     static constexpr int JOIN = (4 / WK - 1) * WK * WORDS * (int)sizeof(float);
     static constexpr int LDS = BUFS * STAGE > JOIN ? BUFS * STAGE : JOIN;
 };
@@ -286,12 +283,10 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     typedef DkvCut<T, DK, DV, WK, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     constexpr int WT = 4 / WK, SUBS = XT / (32 * WT);
-    typedef TTile<NP, DK, XT> QT;
-    typedef NTile<NP, DK, XT> QN;
-    typedef TTile<NP, DV, XT> GT;
-    typedef NTile<NP, DV, XT> GN;
+    typedef Tile<NP, DK, XT> QT;
+    typedef Tile<NP, DV, XT> GT;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    // a stage: q transposed and as it is, dO likewise, then -lse and -delta of its queries
+    // a stage: q, dO, then -lse and -delta of its queries
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -302,6 +297,7 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     const int b = bkv / a.KV, kvh = bkv - b * a.KV;
     const int H = a.KV * a.G;
 
+    const int q_off = SRead<NP, DK, XT>::offset(lane), g_off = SRead<NP, DV, XT>::offset(lane);
     const int s_tile = (tile * WK + wk) * 32;
     const int s = s_tile + l31;
     const bool inside = s < a.Tk;
@@ -327,11 +323,11 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
         fk[0].fill(h, x);
         fv[0].fill(h, y);
     }
-    f32x16 dk[1][QN::GROUPS], dv[1][GN::GROUPS];
+    f32x16 dk[1][QT::GROUPS], dv[1][GT::GROUPS];
 #pragma unroll
-    for (int i = 0; i < QN::GROUPS; ++i) dk[0][i] = zero16();
+    for (int i = 0; i < QT::GROUPS; ++i) dk[0][i] = zero16();
 #pragma unroll
-    for (int i = 0; i < GN::GROUPS; ++i) dv[0][i] = zero16();
+    for (int i = 0; i < GT::GROUPS; ++i) dv[0][i] = zero16();
 
     const int per_head = (a.Tq + XT - 1) / XT;
     const int stages = a.G * per_head;
@@ -359,15 +355,15 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     };
     auto put = [&](int buf) {
         char* const qt = smem + buf * Cut::STAGE;
-        char* const gt = qt + Cut::Q;
+        char* const gt = qt + QT::BYTES;
         Steps<XT> steps;
         unsigned char all[(XT + 63) / 64];
 #pragma unroll
         for (int i = 0; i < (XT + 63) / 64; ++i) all[i] = 1;
         steps.find(ahead, a.Tq, all, lane);
-        qblk.template store<true, true>(qt, qt + QT::BYTES, a.Dk, steps, tid);
-        gblk.template store<true, true>(gt, gt + GT::BYTES, a.Dv, steps, tid);
-        if (tid < 2 * XT) reinterpret_cast<float*>(gt + GT::BYTES + GN::BYTES)[tid] = stat;
+        qblk.store(qt, a.Dk, steps, tid);
+        gblk.store(gt, a.Dv, steps, tid);
+        if (tid < 2 * XT) reinterpret_cast<float*>(gt + GT::BYTES)[tid] = stat;
     };
     // position bias: near tiles read the stage's head's band in LDS, two of them so that the next head's can be filled
     // while the last one's is in use
@@ -393,10 +389,8 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
         }
         if (BIAS && stage + 1 < last && (stage + 1) / per_head != stage / per_head) put_band((stage + 1) / per_head);
         const char* const qt = smem + buf * Cut::STAGE;
-        const char* const qn = qt + QT::BYTES;
-        const char* const gt = qt + Cut::Q;
-        const char* const gn = gt + GT::BYTES;
-        const float* const stats = reinterpret_cast<const float*>(gn + GN::BYTES);
+        const char* const gt = qt + QT::BYTES;
+        const float* const stats = reinterpret_cast<const float*>(gt + GT::BYTES);
         const int g = stage / per_head, t0 = (stage - g * per_head) * XT;
         if (BIAS && g != head_now) {
             head_now = g;
@@ -434,18 +428,18 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
                     for (int r = 0; r < 16; ++r) acc[r] += r0[-acc_row(r, h)];
                 }
             }
-            two_scores<NP, DK, DV, XT>(qt + (x0 + l31) * QT::RS, fk, raw, gt + (x0 + l31) * GT::RS, fv, dsv, h);
+            two_scores<NP, DK, DV, XT>(qt + 2 * x0 + q_off, fk, raw, gt + 2 * x0 + g_off, fv, dsv, h);
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[r] = NP == 3 ? raw[0][r] + acc[r] : __builtin_fmaf(raw[0][r], c, acc[r]);
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[r] = __builtin_amdgcn_exp2f(acc[r]);
             PFrag<NP> p[1];
             p[0].fill(acc);
-            mma_values<NP, DV, XT, 1>(gn, x0, l31, h, p, dv);
+            mma_values<NP, DV, XT, 1>(gt, x0, l31, h, p, dv);
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] *= acc[r];
             p[0].fill(ds);
-            mma_values<NP, DK, XT, 1>(qn, x0, l31, h, p, dk);
+            mma_values<NP, DK, XT, 1>(qt, x0, l31, h, p, dk);
         }
         if (stage + 1 < last) {
             __syncthreads();
@@ -468,9 +462,9 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
 #pragma unroll
-                for (int i = 0; i < QN::GROUPS; ++i) mine[(16 * i + r) * 64] = dk[0][i][r];
+                for (int i = 0; i < QT::GROUPS; ++i) mine[(16 * i + r) * 64] = dk[0][i][r];
 #pragma unroll
-                for (int i = 0; i < GN::GROUPS; ++i) mine[(16 * (QN::GROUPS + i) + r) * 64] = dv[0][i][r];
+                for (int i = 0; i < GT::GROUPS; ++i) mine[(16 * (QT::GROUPS + i) + r) * 64] = dv[0][i][r];
             }
         }
         __syncthreads();
@@ -480,9 +474,9 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
 #pragma unroll
-                for (int i = 0; i < QN::GROUPS; ++i) dk[0][i][r] += other[(16 * i + r) * 64];
+                for (int i = 0; i < QT::GROUPS; ++i) dk[0][i][r] += other[(16 * i + r) * 64];
 #pragma unroll
-                for (int i = 0; i < GN::GROUPS; ++i) dv[0][i][r] += other[(16 * (QN::GROUPS + i) + r) * 64];
+                for (int i = 0; i < GT::GROUPS; ++i) dv[0][i][r] += other[(16 * (QT::GROUPS + i) + r) * 64];
             }
         }
     }
@@ -490,14 +484,14 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     eight_rows<NP, DK>(dk[0][0]);
     auto each = [&](auto&& put_k, auto&& put_v) {
 #pragma unroll
-        for (int i = 0; i < QN::GROUPS; ++i)
+        for (int i = 0; i < QT::GROUPS; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * i + acc_row(r, h);
-                if (d < a.Dk && (!QN::P8 || r < 4)) put_k(d, live ? dk[0][i][r] * a.scale : 0.f);
+                if (d < a.Dk && (!QT::P8 || r < 4)) put_k(d, live ? dk[0][i][r] * a.scale : 0.f);
             }
 #pragma unroll
-        for (int i = 0; i < GN::GROUPS; ++i)
+        for (int i = 0; i < GT::GROUPS; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * i + acc_row(r, h);

@@ -33,7 +33,7 @@ struct FwdArgs {
 template <class T, int DK, int DV, int XT>
 struct FwdCut {
     static constexpr int NP = Elem<T>::NP;
-    static constexpr int STAGE = TTile<NP, DK, XT>::BYTES + NTile<NP, DV, XT>::BYTES;
+    static constexpr int STAGE = Tile<NP, DK, XT>::BYTES + Tile<NP, DV, XT>::BYTES;
     static constexpr int BUFS = 2 * STAGE <= 80 * 1024 ? 2 : 1;  // (two workgroups to a CU)
     static constexpr int LDS = BUFS * STAGE;
 };
@@ -44,8 +44,9 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
     constexpr int WC = 4 / KW;                  // waves along the columns
     constexpr int SUBS = XT / (32 * KW);        // key tiles a wave takes of a stage
     constexpr int J = CB == 1 && SUBS % 2 == 0 ? 2 : 1;  // ... of them at once: independent chains to overlap
-    typedef TTile<NP, DK, XT> KT;
-    typedef NTile<NP, DV, XT> VT;
+    typedef Tile<NP, DK, XT> KT;
+    typedef Tile<NP, DV, XT> VT;
+    typedef SRead<NP, DK, XT> KR;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
@@ -58,6 +59,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
 
     const int ncols = a.G * a.Tq;
     const int col0 = (tile * WC + wave / KW) * 32 * CB;
+    const int k_off = KR::offset(lane);
     const float c = a.scale * LOG2E;
     // per column block: its lane's query and head
     bool live[CB];
@@ -128,8 +130,8 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
     auto put = [&](int buf) {
         char* const kt = smem + buf * Cut::STAGE;
         next.find(ahead.x0, s_end, ahead.raw, lane);
-        kblk.template store<true, false>(kt, nullptr, a.Dk, next, tid);
-        vblk.template store<false, true>(nullptr, kt + KT::BYTES, a.Dv, next, tid);
+        kblk.store(kt, a.Dk, next, tid);
+        vblk.store(kt + KT::BYTES, a.Dv, next, tid);
     };
     int buf = 0;
     if (s_begin < s_end) {
@@ -162,7 +164,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
                 const int x0 = 32 * (KW == 1 ? u + j : ksub);
 #pragma unroll
                 for (int i = 0; i < CB; ++i) acc[j][i] = zero16();
-                mma_scores<NP, DK, XT, CB>(kt + (x0 + l31) * KT::RS, h, fq, acc[j]);
+                mma_scores<NP, DK, XT, CB>(kt + 2 * x0 + k_off, h, fq, acc[j]);
             }
 #pragma unroll
             for (int i = 0; i < CB; ++i) {

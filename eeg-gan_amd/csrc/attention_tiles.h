@@ -6,13 +6,15 @@
 // through three bf16 pieces per operand (v = p1 + p2 + p3 up to 2^-24 |v|, the six products down to 2^-16 of the
 // leading one: the rounding of an fp32 product); bfloat16 tensors directly.
 //
-// Two products alternate, and the layout makes the second one free of data movement:
-//   * scores-like, rows x = a time axis, reduction over channels: the streamed operand lies in LDS with channels
-//     contiguous ("T" tile, transposed while it is staged), the stationary one in registers (SFrag);
-//   * values-like, rows = channels, reduction over the time axis x: the streamed operand lies in LDS as it lies in
-//     memory ("N" tile), and the other operand is the result registers of the first product as they are: lane half h
-//     holds rows x = 16 kk + 8 a + 4 h + c (kk, a in {0, 1}, c < 4) in registers 8 kk + 4 a + c, so an N tile stores
-//     x at position 16 kk + 8 h + 4 a + c and one 16-byte read yields the matching operand.
+// A streamed operand lies in LDS as it lies in memory, channels in rows, and two products alternate on it:
+//   * scores-like, rows x = a time axis, reduction over channels: read with the transposing LDS loads (16 lanes give the
+//     addresses of four rows' neighbouring values, each lane gets one column of the block), the other operand stationary
+//     in registers (SFrag);
+//   * values-like, rows = channels, reduction over the time axis x: read as it lies, and the other operand is the result
+//     registers of the first product as they are: lane half h holds rows x = 16 kk + 8 a + 4 h + c (kk, a in {0, 1}, c <
+//     4) in registers 8 kk + 4 a + c, so a row stores x at position 16 kk + 8 h + 4 a + c and one 16-byte read yields the
+//     matching operand.
+// (A second, transposed copy of the tiles took a third of the backward kernels' time to write.)
 #pragma once
 #include "common.h"
 
@@ -119,22 +121,15 @@ constexpr bool packed8() { return NP == 3 && D == 8; }
 
 // Row strides are odd multiples of 16 bytes: the 16-byte reads of 32 consecutive rows spread over all banks.
 template <int NP, int D, int XT>
-struct TTile {
-    static constexpr bool P8 = packed8<NP, D>();
-    static constexpr int RS = P8 ? 48 : 2 * D + 16;
-    static constexpr int PIECE = P8 ? 16 : XT * RS;
-    static constexpr int BYTES = P8 ? XT * RS : NP * XT * RS;
-};
-template <int NP, int D, int XT>
-struct NTile {
+struct Tile {
     static constexpr bool P8 = packed8<NP, D>();
     static constexpr int RS = 2 * XT + 16;
-    static constexpr int ROWS = D < 32 ? 32 : D;  // the products read whole groups of 32 rows
+    static constexpr int ROWS = D < 32 ? 32 : D;  // the values-like products read whole groups of 32 rows
     static constexpr int PIECE = P8 ? 8 * RS : ROWS * RS;
     static constexpr int BYTES = P8 ? 32 * RS : NP * ROWS * RS;
     static constexpr int GROUPS = D < 32 ? 1 : D / 32;
 };
-// byte offset of time index x (a multiple of 4) in a row of an N tile
+// byte offset of time index x (a multiple of 4) in a row
 __device__ __forceinline__ int n_off(int x) { return 2 * ((x & ~31) + (x & 16) + ((x & 4) << 1) + ((x & 8) >> 1)); }
 
 // Which steps of a stage count, one bit each (the same in every lane).
@@ -199,24 +194,18 @@ __device__ __forceinline__ void attended_range(const unsigned char* mask, int& b
 }
 
 // A [D, XT] block of a channels-first matrix on its way from memory into LDS: 4 x 4 units (four channels, four time
-// steps).  A wave takes 8 x 8 units where the block has them (its transposed writes then fall on all LDS banks: rows of
-// units lie 16 banks apart, neighbouring channel groups 2), else neighbouring steps first.  Loads never branch per value
+// steps), neighbouring threads on neighbouring steps.  Loads never branch per value
 // (the compiler would wait at every join): whatever lies past the matrix is read at its last row or step.  Such values and
 // those of masked steps become zeros on their way into LDS, so what they hold (NaN included) never meets a product.
 template <class T, int D, int XT>
 struct Block {
     static constexpr int NP = Elem<T>::NP;
     static constexpr int XQ = XT / 4, DB = D / 4, UNITS = DB * XQ, U = (UNITS + THREADS - 1) / THREADS;
-    static constexpr bool SQUARE = XQ % 8 == 0 && DB % 8 == 0;
     typename Elem<T>::raw4 r[U][4];
     unsigned off[U][4];  // byte offsets of the unit's rows from (channel 0, first step of the stage)
 
-    static __device__ __forceinline__ int unit_kq(int unit) {
-        return SQUARE ? 8 * ((unit >> 6) % (XQ / 8)) + (unit & 7) : unit % XQ;
-    }
-    static __device__ __forceinline__ int unit_db(int unit) {
-        return SQUARE ? 8 * ((unit >> 6) / (XQ / 8)) + ((unit >> 3) & 7) : unit / XQ;
-    }
+    static __device__ __forceinline__ int unit_kq(int unit) { return unit % XQ; }
+    static __device__ __forceinline__ int unit_db(int unit) { return unit / XQ; }
 
     // stride (channels, in elements) times 128 fits 32 bits in bytes: checked on the host
     __device__ __forceinline__ void init(long long stride, int channels, int tid) {
@@ -253,11 +242,9 @@ struct Block {
         }
     }
 
-    // WT / WN: write the T tile / the N tile.  steps: which count.
-    template <bool WT, bool WN>
-    __device__ __forceinline__ void store(char* tt, char* nt, int channels, const Steps<XT>& steps, int tid) {
-        typedef TTile<NP, D, XT> TL;
-        typedef NTile<NP, D, XT> NL;
+    // into the tile; steps: which count
+    __device__ __forceinline__ void store(char* tile, int channels, const Steps<XT>& steps, int tid) {
+        typedef Tile<NP, D, XT> TL;
         const bool clean = steps.all() && channels == D;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -292,23 +279,11 @@ struct Block {
             }
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
-                if (WN) {
-                    char* row = nt + p * NL::PIECE + (4 * db) * NL::RS + n_off(4 * kq);
+                char* row = tile + p * TL::PIECE + (4 * db) * TL::RS + n_off(4 * kq);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const u32x2 o = {w[i][0][p], w[i][1][p]};
-                        *reinterpret_cast<u32x2*>(row + i * NL::RS) = o;
-                    }
-                }
-                if (WT) {
-                    char* row = tt + p * TL::PIECE + (4 * kq) * TL::RS + 8 * db;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {  // step e: channels (0, 1) and (2, 3)
-                        const unsigned sel = e & 1 ? 0x07060302u : 0x05040100u;
-                        const u32x2 o = {__builtin_amdgcn_perm(w[1][e >> 1][p], w[0][e >> 1][p], sel),
-                                         __builtin_amdgcn_perm(w[3][e >> 1][p], w[2][e >> 1][p], sel)};
-                        *reinterpret_cast<u32x2*>(row + e * TL::RS) = o;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const u32x2 o = {w[i][0][p], w[i][1][p]};
+                    *reinterpret_cast<u32x2*>(row + i * TL::RS) = o;
                 }
             }
         }
@@ -366,27 +341,46 @@ struct SFrag {
     }
 };
 
-// The operands of a scores-like product for the 32 rows from `row` (= tile + (first row + lane & 31) * RS).
+// Eight channels of one step per lane, out of rows of neighbouring steps: lane s of a group of sixteen gives the address of
+// four steps (quad s % 4) of channel s / 4, and lane i receives step i of the four channels.
+__device__ __forceinline__ bf16x8 lds8_transposed(const char* p, int four_rows) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + four_rows));
+    const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return __builtin_bit_cast(bf16x8, v);
+}
+// The operands of a scores-like product for 32 steps (rows of the result) from `tile` (+ 2 * first step).
 template <int NP, int D, int XT>
 struct SRead {
     static constexpr int N = packed8<NP, D>() ? 3 : NP * D / 16;
+    typedef Tile<NP, D, XT> TL;
     bf16x8 a[N];
-    __device__ __forceinline__ void load(const char* row, int h) {
-        if constexpr (packed8<NP, D>()) {
-            a[0] = lds8(row + 32 * h);
-            a[1] = lds8(row + 16);
-            a[2] = lds8(row);
+    // this lane's address in a tile
+    static __device__ __forceinline__ int offset(int lane) {
+        const int s = lane & 15, h = lane >> 5;
+        return ((s >> 2) + (TL::P8 ? 0 : 8 * h)) * TL::RS + n_off(4 * (4 * ((lane >> 4) & 1) + (s & 3)));
+    }
+    // p: tile + 2 * first step + offset(lane)
+    __device__ __forceinline__ void load(const char* p, int h) {
+        if constexpr (TL::P8) {
+            a[0] = lds8_transposed(p + (h ? 2 * TL::PIECE : 0), 4 * TL::RS);
+            a[1] = lds8_transposed(p + TL::PIECE, 4 * TL::RS);
+            a[2] = lds8_transposed(p, 4 * TL::RS);
         } else {
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-                for (int p = 0; p < NP; ++p) a[NP * j + p] = lds8(row + 32 * j + 16 * h + p * TTile<NP, D, XT>::PIECE);
+                for (int q = 0; q < NP; ++q)
+                    a[NP * j + q] = lds8_transposed(p + 16 * j * TL::RS + q * TL::PIECE, 4 * TL::RS);
         }
     }
     // acc[b][x, column] += sum_d tile[x, d] frag[b][d, column] for CB column blocks: every operand serves all of them
     template <int CB>
     __device__ __forceinline__ void mma(const SFrag<NP, D> (&s)[CB], f32x16 (&acc)[CB]) const {
-        if constexpr (packed8<NP, D>()) {
+        if constexpr (TL::P8) {
 #pragma unroll
             for (int b = 0; b < CB; ++b) acc[b] = mfma(a[0], s[b].f[1], acc[b]);  // p1 q3 | p3 q1
 #pragma unroll
@@ -421,9 +415,9 @@ struct SRead {
 constexpr int READ_AHEAD = 9;
 
 template <int NP, int D, int XT, int CB>
-__device__ __forceinline__ void mma_scores(const char* row, int h, const SFrag<NP, D> (&s)[CB], f32x16 (&acc)[CB]) {
+__device__ __forceinline__ void mma_scores(const char* p, int h, const SFrag<NP, D> (&s)[CB], f32x16 (&acc)[CB]) {
     SRead<NP, D, XT> r;
-    r.load(row, h);
+    r.load(p, h);
     if constexpr (SRead<NP, D, XT>::N <= READ_AHEAD) __builtin_amdgcn_sched_barrier(0);
     r.template mma<CB>(s, acc);
 }
@@ -471,8 +465,8 @@ struct PFrag {
 // instructions instead of six; eight_rows() sums the pieces' results.
 template <int NP, int D, int XT, int CB>
 __device__ __forceinline__ void mma_values(const char* tile, int x0, int l31, int h, const PFrag<NP> (&f)[CB],
-                                           f32x16 (&acc)[CB][NTile<NP, D, XT>::GROUPS]) {
-    typedef NTile<NP, D, XT> NL;
+                                           f32x16 (&acc)[CB][Tile<NP, D, XT>::GROUPS]) {
+    typedef Tile<NP, D, XT> NL;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
