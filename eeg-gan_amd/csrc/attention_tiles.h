@@ -458,6 +458,20 @@ struct PFrag {
             for (int p = 0; p < NP; ++p) f[kk][p] = __builtin_bit_cast(bf16x8, ws[p]);
         }
     }
+    // what fill() rounded away (NP = 1), rounded in turn: 2^-18 of the values is left
+    __device__ __forceinline__ void fill_rest(const f32x16& v) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            u32x4 ws;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = v[8 * kk + 2 * i], y = v[8 * kk + 2 * i + 1];
+                const unsigned w = pack2(x, y);
+                ws[i] = pack2(x - lo_f(w), y - hi_f(w));
+            }
+            f[kk][0] = __builtin_bit_cast(bf16x8, ws);
+        }
+    }
 };
 
 // acc[b][g][row, column] += sum_x tile[32 g + row, x] frag[b][x, column] over the 32 steps from x0.
