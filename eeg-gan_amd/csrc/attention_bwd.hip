@@ -42,7 +42,7 @@ struct DqCut {
 };
 constexpr int SQUARE = 32 * 33;  // a wave's tile of dS on its way into the histogram by distance
 template <class T, int DK, int DV, int XT, bool BIAS>
-__global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
+__global__ __launch_bounds__(THREADS, DK + DV >= 160 && Elem<T>::NP == 3 ? 1 : 2) void attn_dq_kernel(BwdArgs a) {
     typedef DqCut<T, DK, DV, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     typedef Tile<NP, DK, XT> KT;
@@ -74,32 +74,34 @@ __global__ __launch_bounds__(THREADS, 2) void attn_dq_kernel(BwdArgs a) {
     // (float32: error 2.4e-6 of the gradient's norm with one sign, 4e-7 with both).
     const float sign = wave & 1 ? -1.f : 1.f;
     {
-        const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc + t;
-        const T* g = reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq + t;
-        const T* o = reinterpret_cast<const T*>(a.out) + row * a.Dv * a.Tq + t;
+        const T* q = reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc;
+        const T* g = reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq;
+        const T* o = reinterpret_cast<const T*>(a.out) + row * a.Dv * a.Tq;
+        const T* w = reinterpret_cast<const T*>(NP == 1 ? a.rest : a.out) + row * a.Dv * a.Tq;
         typedef SFrag<NP, DK> FK;
         typedef SFrag<NP, DV> FV;
-        float x[FK::VALUES], y[FV::VALUES], z[FV::VALUES];
-        FK::read(q, a.qsc, a.Dk, h, x);
-        FV::read(g, a.Tq, a.Dv, h, y);
-        FV::read(o, a.Tq, a.Dv, h, z);
-        if constexpr (NP == 1) {
-            float w[FV::VALUES];
-            FV::read(reinterpret_cast<const T*>(a.rest) + row * a.Dv * a.Tq + t, a.Tq, a.Dv, h, w);
-#pragma unroll
-            for (int i = 0; i < FV::VALUES; ++i) z[i] += w[i];
-        }
+        float x[FK::VALUES], y[FV::VALUES];
+        FK::read(q, t, a.qsc, a.Dk, h, x);
 #pragma unroll
         for (int i = 0; i < FK::VALUES; ++i) x[i] = live && FK::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
-#pragma unroll
-        for (int i = 0; i < FV::VALUES; ++i) {
-            const bool ok = live && FV::channel(i, h) < a.Dv;
-            y[i] = ok ? y[i] : 0.f;
-            delta = ok ? __builtin_fmaf(y[i], z[i], delta) : delta;
-        }
-#pragma unroll
-        for (int i = 0; i < FV::VALUES; ++i) y[i] *= sign;
         fq[0].fill(h, x);
+        // (sixteen values of a lane at a time: all loads of 128 channels in flight spill registers)
+        constexpr int SOME = FV::VALUES < 16 ? FV::VALUES : 16;
+        static_unroll<FV::VALUES / SOME>([&](auto part) {
+            constexpr int FIRST = decltype(part)::value * SOME;
+            float yy[SOME], z[SOME], zz[SOME];
+            if constexpr (FIRST != 0) __builtin_amdgcn_sched_barrier(0);
+            FV::template read<FIRST>(g, t, a.Tq, a.Dv, h, yy);
+            FV::template read<FIRST>(o, t, a.Tq, a.Dv, h, z);
+            if constexpr (NP == 1) FV::template read<FIRST>(w, t, a.Tq, a.Dv, h, zz);
+#pragma unroll
+            for (int i = 0; i < SOME; ++i) {
+                const bool ok = live && FV::channel(FIRST + i, h) < a.Dv;
+                const float v = ok ? yy[i] : 0.f;
+                delta = ok ? __builtin_fmaf(v, NP == 1 ? z[i] + zz[i] : z[i], delta) : delta;
+                y[FIRST + i] = sign * v;
+            }
+        });
         fg[0].fill(h, y);
         delta = half_sum(delta);
         if (inside && h == 0) a.delta[row * a.Tq + t] = delta;
@@ -285,7 +287,7 @@ struct DkvCut {
     static constexpr int LDS = BUFS * STAGE > JOIN ? BUFS * STAGE : JOIN;
 };
 template <class T, int DK, int DV, int WK, int XT, bool BIAS>
-__global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 2) void attn_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(THREADS, DK + DV >= 160 ? 1 : 2) void attn_dkv_kernel(BwdArgs a) {
     typedef DkvCut<T, DK, DV, WK, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     constexpr int WT = 4 / WK, SUBS = XT / (32 * WT);
@@ -315,18 +317,19 @@ __global__ __launch_bounds__(THREADS, (DK + DV > 160 && Elem<T>::NP == 3) ? 1 : 
     SFrag<NP, DK> fk[1];
     SFrag<NP, DV> fv[1];
     {
-        const T* k = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc + (live ? s : 0);
-        const T* v = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc + (live ? s : 0);
+        const T* k = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc;
+        const T* v = reinterpret_cast<const T*>(a.v) + b * a.vsb + (long long)kvh * a.Dv * a.vsc;
+        const unsigned at = live ? s : 0;
         typedef SFrag<NP, DK> FK;
         typedef SFrag<NP, DV> FV;
         float x[FK::VALUES], y[FV::VALUES];
-        FK::read(k, a.ksc, a.Dk, h, x);
-        FV::read(v, a.vsc, a.Dv, h, y);
+        FK::read(k, at, a.ksc, a.Dk, h, x);
 #pragma unroll
         for (int i = 0; i < FK::VALUES; ++i) x[i] = live && FK::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
+        fk[0].fill(h, x);
+        FV::read(v, at, a.vsc, a.Dv, h, y);
 #pragma unroll
         for (int i = 0; i < FV::VALUES; ++i) y[i] = live && FV::channel(i, h) < a.Dv ? y[i] : 0.f;
-        fk[0].fill(h, x);
         fv[0].fill(h, y);
     }
     f32x16 dk[1][QT::GROUPS], dv[1][GT::GROUPS];
@@ -541,7 +544,7 @@ namespace {
 template <class T, int DK, int DV>
 struct Cut {
     static constexpr bool F32 = Elem<T>::NP == 3;
-    static constexpr int DQ_XT = F32 && DK + DV > 96 ? 32 : 64;
+    static constexpr int DQ_XT = DK + DV > (F32 ? 96 : 128) ? 32 : 64;
     static constexpr int WIDE_XT = F32 && DK + DV > 96 ? 32 : 64;
     static constexpr bool NARROW = !(F32 && DK + DV > 96);  // has a form whose waves share keys
 };

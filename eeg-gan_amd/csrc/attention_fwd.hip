@@ -87,7 +87,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
         // (float32: the scale goes into the split operand; bfloat16 operands stay exact and the scores are scaled)
         typedef SFrag<NP, DK> F;
         float x[F::VALUES];
-        F::read(q, a.qsc, a.Dk, h, x);
+        F::read(q, 0u, a.qsc, a.Dk, h, x);
 #pragma unroll
         for (int e = 0; e < F::VALUES; ++e)
             x[e] = live[i] && F::channel(e, h) < a.Dk ? (NP == 3 ? x[e] * c : x[e]) : 0.f;

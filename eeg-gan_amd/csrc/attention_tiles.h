@@ -290,6 +290,14 @@ struct Block {
     }
 };
 
+template <int N, class F, int I = 0>
+__device__ __forceinline__ void static_unroll(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_unroll<N, F, I + 1>(static_cast<F&&>(f));
+    }
+}
+
 // ---- fragments ----------------------------------------------------------------------------------------------
 // The stationary operand of a scores-like product: this lane's column (one time step) of a [D, T] matrix.  Eight
 // channels in three pieces: two pieces of a term fill the sixteen reduction indices of one instruction, so the six
@@ -303,11 +311,16 @@ struct SFrag {
     static __device__ __forceinline__ int channel(int i, int h) {
         return packed8<NP, D>() ? i : 16 * (i / 8) + 8 * h + i % 8;
     }
-    // the lane's channels of a column (p: channel 0 of it); past the matrix the last channel again, to be zeroed
-    template <class T>
-    static __device__ __forceinline__ void read(const T* p, long long stride, int channels, int h, float (&v)[VALUES]) {
+    // the lane's channels of column `at` of p, values [FIRST, FIRST + N) of them; past the matrix the last channel again, to be
+    // zeroed.  (The rows' offsets are scalars, a lane picks its half's: two instructions a load.)
+    template <int FIRST = 0, int N = VALUES, class T>
+    static __device__ __forceinline__ void read(const T* p, unsigned at, long long stride, int channels, int h, float (&v)[N]) {
 #pragma unroll
-        for (int i = 0; i < VALUES; ++i) v[i] = ld1(p + (long long)min(channel(i, h), channels - 1) * stride);
+        for (int i = 0; i < N; ++i) {
+            const unsigned o0 = min(channel(FIRST + i, 0), channels - 1) * (unsigned)stride;
+            const unsigned o1 = min(channel(FIRST + i, 1), channels - 1) * (unsigned)stride;
+            v[i] = ld1(reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + (size_t)(unsigned)((at + (h ? o1 : o0)) * sizeof(T))));
+        }
     }
     // v: the (already scaled) values, zero past the matrix
     __device__ __forceinline__ void fill(int h, const float (&v)[VALUES]) {
@@ -410,9 +423,9 @@ struct SRead {
         }
     }
 };
-// Whether a tile's operands are all read before the first product: up to this many (the compiler reads each one right
-// before its product and waits for it; past that the registers do not hold them).
-constexpr int READ_AHEAD = 9;
+// Whether a tile's operands are all read before the first product: up to this many for one product, for scores and dP together
+// (the compiler reads each one right before its product and waits for it; past that the registers do not hold them).
+constexpr int READ_AHEAD = 6, READ_AHEAD_TWO = 9;
 
 template <int NP, int D, int XT, int CB>
 __device__ __forceinline__ void mma_scores(const char* p, int h, const SFrag<NP, D> (&s)[CB], f32x16 (&acc)[CB]) {
@@ -425,7 +438,7 @@ __device__ __forceinline__ void mma_scores(const char* p, int h, const SFrag<NP,
 template <int NP, int DK, int DV, int XT>
 __device__ __forceinline__ void two_scores(const char* k, const SFrag<NP, DK> (&fk)[1], f32x16 (&s)[1], const char* v,
                                            const SFrag<NP, DV> (&fv)[1], f32x16 (&dp)[1], int h) {
-    if constexpr (SRead<NP, DK, XT>::N + SRead<NP, DV, XT>::N <= READ_AHEAD) {
+    if constexpr (SRead<NP, DK, XT>::N + SRead<NP, DV, XT>::N <= READ_AHEAD_TWO) {
         SRead<NP, DK, XT> rk;
         SRead<NP, DV, XT> rv;
         rk.load(k, h);
