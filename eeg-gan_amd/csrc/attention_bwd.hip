@@ -42,7 +42,7 @@ struct DqCut {
 };
 constexpr int SQUARE = 32 * 33;  // a wave's tile of dS on its way into the histogram by distance
 template <class T, int DK, int DV, int XT, bool BIAS>
-__global__ __launch_bounds__(THREADS, DK + DV >= 160 && Elem<T>::NP == 3 ? 1 : 2) void attn_dq_kernel(BwdArgs a) {
+__global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2) void attn_dq_kernel(BwdArgs a) {
     typedef DqCut<T, DK, DV, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     typedef Tile<NP, DK, XT> KT;
@@ -287,7 +287,7 @@ struct DkvCut {
     static constexpr int LDS = BUFS * STAGE > JOIN ? BUFS * STAGE : JOIN;
 };
 template <class T, int DK, int DV, int WK, int XT, bool BIAS>
-__global__ __launch_bounds__(THREADS, DK + DV >= 160 ? 1 : 2) void attn_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ? 1 : 2) void attn_dkv_kernel(BwdArgs a) {
     typedef DkvCut<T, DK, DV, WK, XT> Cut;
     constexpr int NP = Elem<T>::NP;
     constexpr int WT = 4 / WK, SUBS = XT / (32 * WT);

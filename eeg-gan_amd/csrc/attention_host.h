@@ -60,6 +60,9 @@ int bucket_sums(const float* hist, void* out, int out_bf16, const eeggan_buckets
         } else if ((a).Dk <= 32) {                                                                        \
             constexpr int DK = 32, DV = 128;                                                              \
             __VA_ARGS__;                                                                                  \
+        } else if ((a).Dk <= 96 && (a).Dv <= 96) {                                                        \
+            constexpr int DK = 96, DV = 96;                                                               \
+            __VA_ARGS__;                                                                                  \
         } else {                                                                                          \
             constexpr int DK = 128, DV = 128;                                                             \
             __VA_ARGS__;                                                                                  \
