@@ -1683,8 +1683,10 @@ class RelativeBuckets:
         if side < 2 or side > 64 or (bidirectional and num_buckets % 2):
             raise ValueError(f"RelativeBuckets: {num_buckets} buckets: 2 .. 64 on a side are supported"
                              f"{', the same number on both' if bidirectional else ''}")
-        if not 1 <= step <= 16:
-            raise ValueError(f"RelativeBuckets: step {step} outside 1 .. 16")
+        if not 1 <= step <= 16 or int(step) != step:
+            raise ValueError(f"RelativeBuckets: step {step}: a whole number of 1 .. 16")
+        if not abs(offset) < 1 << 30 or int(offset) != offset:
+            raise ValueError(f"RelativeBuckets: offset {offset}: a whole number below 2 ** 30")
         exact = side // 2
         if not exact < max_distance <= 1024 or max_distance - exact < side - exact:
             raise ValueError(f"RelativeBuckets: max_distance {max_distance}: up to 1024, and enough for {side} buckets")
@@ -1828,6 +1830,12 @@ def _attention_desc(q, k, v, mask, table, cfg):
                           v.shape[1] // kv_heads, tq, k.shape[2], scale)
 
 
+def _attention_at(q, k, v, table, mask):
+    """Where a descriptor of these tensors points and how it walks them."""
+    return (q.data_ptr(), q.stride(), k.data_ptr(), k.stride(), v.data_ptr(), v.stride(),
+            None if table is None else table.data_ptr(), None if mask is None else mask.data_ptr())
+
+
 def _attention_stored(q, k, v, table, mask, cfg):
     """The same function out of the operators with stored scores, which differentiate twice (float32)."""
     heads, kv, scale, buckets = cfg
@@ -1871,7 +1879,8 @@ class _Attention(Function):
             call("eeggan_attention_fwd", a, out.data_ptr(), None if rest is None else rest.data_ptr(),
                  None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, _stream_of(q))
         if keep:
-            ctx.cfg, ctx.desc = cfg[:4], desc  # (the descriptor points to tensors that are saved below)
+            # (the descriptor points to the tensors that are saved below; saved-tensor hooks may give back others)
+            ctx.cfg, ctx.desc, ctx.at = cfg[:4], desc, _attention_at(q, k, v, table, mask)
             ctx.save_for_backward(q, k, v, table, mask, out, rest, lse)
         return out
 
@@ -1891,7 +1900,12 @@ class _Attention(Function):
             return tuple(grads.get(i) for i in range(4)) + (None,)
         if g.dtype is not q.dtype or not g.is_contiguous():
             g = g.to(q.dtype).contiguous()
-        a = ctypes.addressof(ctx.desc)
+        desc = ctx.desc
+        if _attention_at(q, k, v, table, mask) != ctx.at:  # (moved or recomputed between the passes)
+            q, k, v, out, lse = _rows(q), _rows(k), _rows(v), out.contiguous(), lse.contiguous()
+            table, mask, rest = (t if t is None else t.contiguous() for t in (table, mask, rest))
+            desc = _attention_desc(q, k, v, mask, table, ctx.cfg)
+        a = ctypes.addressof(desc)
         gq, gk, gv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
         gt = torch.empty(table.shape, device=table.device, dtype=table.dtype) if want_table else None
         with _on(q):

@@ -108,6 +108,8 @@ class Adam(torch.optim.Optimizer):
     are in ``p.grad``, and ``grad_norm`` holds the norm it found (a 0-dim device tensor that every step, captured ones
     included, rewrites)."""
 
+    max_grad_norm = _norm = None  # (for objects that were pickled without them)
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, amsgrad=False, max_grad_norm=None):
         if max_grad_norm is not None and not float(max_grad_norm) > 0.0:
             raise ValueError(f"Adam: max_grad_norm {max_grad_norm} is not positive")
@@ -171,6 +173,9 @@ class Adam(torch.optim.Optimizer):
         return None
 
     def _clipped_step(self, work, grads):
+        work = [(group, rows) for group, rows in ((group, [r for r in rows if r[5]]) for group, rows in work) if rows]
+        if not work:  # (tensors without elements)
+            return
         device = grads[0].device
         for g in grads:
             if g.device != device or g.dtype != torch.float32:

@@ -497,7 +497,7 @@ def test_no_cpu_path():
     with pytest.raises(RuntimeError, match="no CPU path"):
         ops.relative_bias(x, torch.zeros(32, 1), ops.RelativeBuckets())
     with pytest.raises(ValueError):
-        ops.set_attention("flash")
+        ops.set_attention("tiled")
 
 
 def test_c_entry_points_refuse_before_any_launch():
@@ -565,3 +565,80 @@ def test_refusals(dev):
                      ((z(2, 4, 5, dt=torch.bfloat16), z(32, 1), b), {}), ((z(2, 0, 5), z(32, 1), b), {}), ((z(2, 4, 5), z(32, 1), None), {})):
         with pytest.raises(RuntimeError):
             ops.relative_bias(*args, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dk,dv", [(96, 96), (90, 70), (33, 65), (65, 33), (96, 97), (97, 96)])
+def test_up_to_96_channels(dev, dk, dv, dtype):
+    from eeggan_amd import ops
+    buckets = ops.RelativeBuckets(16, 40)
+    for B, heads, kv, tq, tk in ((2, 1, 1, 70, 45), (1, 2, 2, 161, 130), (3, 4, 1, 1, 70)):
+        q, k, v, g = make(B, heads, kv, dk, dv, tq, tk, dtype)
+        check(dev, q, k, v, g, heads, kv, what=(dk, dv, tq, tk))
+    q, k, v, g, table = make(1, 2, 2, dk, dv, 140, 131, dtype, table=buckets)
+    check(dev, q, k, v, g, 2, 2, table=table, buckets=buckets, what=(dk, dv, "positions"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,tk", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 200)], ids=["f32", "bf16-short", "bf16"])
+def test_table_gradient_sums_to_zero(dev, dtype, tk):
+    """Every query's dS sum to zero, so all buckets' gradients of a head do.  What is left is rounding: delta and the dP of a
+    query carry errors of random sign, each at most u of sum |dO O| or of |dP| with u = 2^-23 (float32: half a step from the
+    output and half from the sums) or 2^-16 (bfloat16: the output in two parts, P in two pieces), so N queries leave about
+    sqrt(N) u rms(dP): bounded by six times that.  An error that goes the same way in every query would add up to N times
+    itself: 2e-9 of dP in each is past the bound here."""
+    from eeggan_amd import ops
+    B, heads, dk, dv, tq = 32, 2, 8, 32, 2300
+    gen = torch.Generator(device=dev).manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=gen).to(dtype)  # noqa: E731
+    q, k, v, g = rnd(B, heads * dk, tq), rnd(B, heads * dk, tk), rnd(B, heads * dv, tk), rnd(B, heads * dv, tq)
+    buckets = ops.RelativeBuckets(16, 64, step=16)
+    table = torch.randn(16, heads, device=dev, generator=gen).requires_grad_(True)
+    out = ops.attention(q, k, v, heads=heads, scale=dk ** -0.5, bias=table, buckets=buckets)
+    gt, = torch.autograd.grad(out, [table], g)
+    u = 2.0 ** -23 if dtype == torch.float32 else 2.0 ** -16
+    left = gt.double().sum(0).abs().max()
+    bound = 6.0 * (B * tq) ** 0.5 * u * dv ** 0.5  # (rms of dP: a sum of dv products of unit variance)
+    assert float(left) <= bound, (float(left), bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_saved_tensors_that_move(dev, dtype):
+    """Saved-tensor hooks give the backward pass other tensors than the forward pass saved: copies from the host, results of
+    a second forward pass.  Same bits as without them."""
+    from eeggan_amd import ops
+    from torch.utils.checkpoint import checkpoint
+    buckets = ops.RelativeBuckets(16, 40)
+    q, k, v, g, table = (t.to(dev) for t in make(2, 4, 2, 24, 40, 75, 66, dtype, table=buckets))
+    mask = torch.arange(66, device=dev)[None, :] < torch.tensor([[66], [31]], device=dev)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, table)]
+
+    def f(q, k, v, table):
+        wide = torch.cat([k, q[:, :k.shape[1], :66]], 1)  # (the keys are a slice of a wider tensor that only this pass has)
+        return ops.attention(2.0 * q, wide[:, :k.shape[1]], v * 0.5, heads=4, kv_heads=2, scale=0.2, mask=mask.clone(), bias=table * 1.0,
+                             buckets=buckets)
+
+    def grads(run):
+        out = run()
+        junk = [torch.full_like(q, float("nan")) for _ in range(8)]  # (what was freed is written over)
+        got = torch.autograd.grad(out, leaves, g)
+        del junk
+        return [out.detach()] + list(got)
+
+    want = grads(lambda: f(*leaves))
+    with torch.autograd.graph.save_on_cpu():
+        out = f(*leaves)
+    got = [out.detach()] + list(torch.autograd.grad(out, leaves, g))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = grads(lambda: checkpoint(f, *leaves, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("conf", [dict(offset=1 << 30), dict(offset=-(1 << 30)), dict(offset=2 ** 32 + 5), dict(offset=0.5), dict(step=1.5)])
+def test_positions_outside_their_type(conf):
+    from eeggan_amd import ops
+    with pytest.raises(ValueError):
+        ops.RelativeBuckets(**conf)
+    assert ops.RelativeBuckets(offset=(1 << 30) - 1).offset == (1 << 30) - 1

@@ -290,3 +290,16 @@ def test_c_entry_points_refuse_before_any_launch():
     full = optim.build_table([(256, 256, 256, 256, 256, 10)])
     assert lib.eeggan_adam_step_clipped(full, 1, 1e-3, 1.0, 0.99, 1e-8, 256, 256, 64, None) != 0
     assert lib.eeggan_adam_step_clipped(full, 1, 1e-3, 0.0, 0.99, 1e-8, 256, 256, 4, None) != 0
+
+
+@pytest.mark.gpu
+def test_parameters_without_elements(dev):
+    """An empty tensor among the parameters has no part in the norm and no step."""
+    from eeggan_amd import optim
+    full, empty = torch.nn.Parameter(torch.ones(5, device=dev)), torch.nn.Parameter(torch.zeros(0, 3, device=dev))
+    for p in (full, empty):
+        p.grad = torch.ones_like(p)
+    opt = optim.Adam([dict(params=[empty]), dict(params=[full])], lr=0.5, betas=(0.0, 0.99), max_grad_norm=0.1)
+    opt.step()
+    assert abs(float(opt.grad_norm) - 5 ** 0.5) < 1e-6 and float(full.detach().max()) < 1.0
+    assert float(optim.clip_grad_norm_([empty], 1.0)) == 0.0
