@@ -31,6 +31,7 @@ struct BwdArgs {
     int B, KV, G, Dk, Dv, Tq, Tk;
     int coltiles, nsplit, nhist;
     float scale;
+    bool fine;  // bfloat16: P and dS meet their products in two pieces (fine_backward)
 };
 
 template <class T, int DK, int DV, int XT>
@@ -233,6 +234,10 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
             PFrag<NP> p[1];
             p[0].fill(ds);
             mma_values<NP, DK, XT, 1>(kt, x0, l31, h, p, dq);
+            if (NP == 1 && a.fine) {
+                p[0].fill_rest(ds);
+                mma_values<NP, DK, XT, 1>(kt, x0, l31, h, p, dq);
+            }
         }
         if (s0 + XT < s_end) {
             __syncthreads();
@@ -445,10 +450,18 @@ __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ?
             PFrag<NP> p[1];
             p[0].fill(acc);
             mma_values<NP, DV, XT, 1>(gt, x0, l31, h, p, dv);
+            if (NP == 1 && a.fine) {
+                p[0].fill_rest(acc);
+                mma_values<NP, DV, XT, 1>(gt, x0, l31, h, p, dv);
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] *= acc[r];
             p[0].fill(ds);
             mma_values<NP, DK, XT, 1>(qt, x0, l31, h, p, dk);
+            if (NP == 1 && a.fine) {
+                p[0].fill_rest(ds);
+                mma_values<NP, DK, XT, 1>(qt, x0, l31, h, p, dk);
+            }
         }
         if (stage + 1 < last) {
             __syncthreads();
@@ -637,7 +650,7 @@ int backward_all(const eeggan_attention& a, const void* out, const void* rest, c
     f.part = p.nsplit > 1 ? reinterpret_cast<float*>(ws + p.rel + p.delta) : nullptr;
     f.hist = p.nhist ? reinterpret_cast<float*>(ws + p.rel + p.delta + p.part) : nullptr;
     f.B = a.B, f.KV = a.KV, f.G = a.H / a.KV, f.Dk = a.Dk, f.Dv = a.Dv, f.Tq = a.Tq, f.Tk = a.Tk;
-    f.coltiles = 0, f.nsplit = p.nsplit, f.nhist = 0, f.scale = a.scale;
+    f.coltiles = 0, f.nsplit = p.nsplit, f.nhist = 0, f.scale = a.scale, f.fine = fine_backward(a);
     if (positions(a, reinterpret_cast<float*>(ws), &f.pos, st)) return 1;
     if (a.table ? backward<T, DK, DV, true>(f, p, st) : backward<T, DK, DV, false>(f, p, st)) return 1;
     if (p.nsplit > 1) {

@@ -27,6 +27,7 @@ struct FwdArgs {
     int B, KV, G, Dk, Dv, Tq, Tk;
     int coltiles, nsplit, split_keys;
     float scale;
+    bool fine;  // bfloat16: P meets V in two pieces (fine_forward)
 };
 
 // KW waves share the columns and split a stage's keys; CB: column blocks of a wave (its LDS operands serve all of them).
@@ -37,11 +38,7 @@ struct FwdCut {
     static constexpr int BUFS = 2 * STAGE <= 80 * 1024 ? 2 : 1;  // (two workgroups to a CU)
     static constexpr int LDS = BUFS * STAGE;
 };
-// FINE (bfloat16): P meets V in two pieces.  The backward pass takes delta = sum_c dO O for sum_s P dP; with P rounded to
-// bfloat16 in O only, the two differ by 2^-9 / sqrt(keys) of dP, and every dS of the row with them.  That shows in the table's
-// gradient, where thousands of dS of both signs cancel (error 0.0028 of its norm, 3e-4 with two pieces), and in rows of
-// few keys (at 64 it is an eighth of the error of rounding dS, which covers it beyond).  So: with a table, and up to 64 keys.
-// It costs the values' products a second time (4 x 6 heads of 64 over 1537 steps with positions: 57 -> 62 us).
+// FINE: has the code for a.fine (where it is not taken its registers cost few columns 10%)
 template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS, bool FINE>
 __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
     typedef FwdCut<T, DK, DV, XT> Cut;
@@ -250,7 +247,7 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
                 for (int i = 0; i < CB; ++i) p[i].fill(acc[j][i]);
                 mma_values<NP, DV, XT, CB>(vt, 32 * (KW == 1 ? u + j : ksub), l31, h, p, o);
-                if constexpr (FINE) {
+                if (FINE && a.fine) {
 #pragma unroll
                     for (int i = 0; i < CB; ++i) p[i].fill_rest(acc[j][i]);
                     mma_values<NP, DV, XT, CB>(vt, 32 * (KW == 1 ? u + j : ksub), l31, h, p, o);
@@ -381,8 +378,8 @@ using namespace eeggan::attn;
 
 namespace {
 
-// How the forward pass is cut.  Up to 32 query columns per key head: the waves split every stage's keys.  Beyond that
-// each wave has columns of its own.  Keys are split over workgroups until there are `WANTED` of them.
+// How the forward pass is cut.  Up to 32 query columns per key head: the waves split every stage's keys.  Beyond that, and
+// for a single stage of keys, each wave has columns of its own.  Keys are split over workgroups until there are `WANTED` of them.
 struct FwdPlan {
     int kw, xt, cb, coltiles, nsplit, split_keys, nparts;
 };
@@ -401,7 +398,7 @@ FwdPlan plan_of(const eeggan_attention& a) {
     typedef Cuts<T, DK, DV> C;
     FwdPlan p;
     const long long ncols = (long long)(a.H / a.KV) * a.Tq, heads = (long long)a.B * a.KV;
-    const bool few = ncols <= 32;
+    const bool few = few_columns(a);
     p.xt = few ? C::FEW_XT : C::XT;
     p.kw = few ? p.xt / 32 : 1;
     p.cb = !few && C::CB == 2 && heads * ((ncols + 255) / 256) >= WANTED ? 2 : 1;
@@ -424,7 +421,7 @@ size_t part_bytes(const eeggan_attention& a, const FwdPlan& p) {
     return (size_t)a.B * a.KV * p.nparts * ncols * (a.Dv + 2) * sizeof(float);
 }
 
-template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS, bool FINE>
+template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS, bool FINE = Elem<T>::NP == 1>
 int launch(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
     constexpr size_t tiles = FwdCut<T, DK, DV, XT>::LDS, most = tiles + (BIAS ? 4 * CB * MAX_BAND * sizeof(float) : 0);
     static_assert(most <= 160 * 1024, "LDS");
@@ -438,16 +435,19 @@ int launch(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
     return check_launch("attention");
 }
 
-template <class T, int DK, int DV, bool BIAS, bool FINE>
+template <class T, int DK, int DV, bool BIAS>
 int launch_cut(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
     typedef Cuts<T, DK, DV> C;
     if constexpr (C::FEW_XT == 64) {
-        if (p.kw == 2) return launch<T, DK, DV, 2, 64, 1, BIAS, FINE>(f, p, st);
+        if (p.kw == 2) {
+            if (f.fine) return launch<T, DK, DV, 2, 64, 1, BIAS>(f, p, st);
+            return launch<T, DK, DV, 2, 64, 1, BIAS, false>(f, p, st);
+        }
     }
     if constexpr (C::CB == 2) {
-        if (p.cb == 2) return launch<T, DK, DV, 1, C::XT, 2, BIAS, FINE>(f, p, st);
+        if (p.cb == 2) return launch<T, DK, DV, 1, C::XT, 2, BIAS>(f, p, st);
     }
-    return launch<T, DK, DV, 1, C::XT, 1, BIAS, FINE>(f, p, st);
+    return launch<T, DK, DV, 1, C::XT, 1, BIAS>(f, p, st);
 }
 
 template <class T, int DK, int DV>
@@ -463,14 +463,8 @@ int forward(const eeggan_attention& a, void* out, void* rest, float* lse, void* 
     f.B = a.B, f.KV = a.KV, f.G = a.H / a.KV, f.Dk = a.Dk, f.Dv = a.Dv, f.Tq = a.Tq, f.Tk = a.Tk;
     f.coltiles = p.coltiles, f.nsplit = p.nsplit, f.split_keys = p.split_keys, f.scale = a.scale;
     if (positions(a, reinterpret_cast<float*>(ws), &f.pos, st)) return 1;
-    int rc;
-    if (a.table)
-        rc = launch_cut<T, DK, DV, true, Elem<T>::NP == 1>(f, p, st);
-    else if (Elem<T>::NP == 1 && a.Tk <= 64)
-        rc = launch_cut<T, DK, DV, false, Elem<T>::NP == 1>(f, p, st);
-    else
-        rc = launch_cut<T, DK, DV, false, false>(f, p, st);
-    if (rc) return rc;
+    f.fine = fine_forward(a);
+    if (a.table ? launch_cut<T, DK, DV, true>(f, p, st) : launch_cut<T, DK, DV, false>(f, p, st)) return 1;
     if (p.nparts == 1) return 0;
     const long long items = (long long)a.B * a.KV * a.Dv * f.G * a.Tq;
     int lanes = 1;  // threads that share an output's parts: at least four parts each

@@ -642,3 +642,24 @@ def test_positions_outside_their_type(conf):
     with pytest.raises(ValueError):
         ops.RelativeBuckets(**conf)
     assert ops.RelativeBuckets(offset=(1 << 30) - 1).offset == (1 << 30) - 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,heads,kv,dk,dv,tq,tk,train", [(4, 4, 2, 6, 6, 115, 115, True), (2, 2, 1, 128, 5, 257, 5, True), (3, 4, 4, 64, 64, 4, 4, True),
+                                                          (2, 2, 2, 32, 96, 300, 170, True), (2, 4, 4, 32, 32, 1, 9000, False)])
+def test_small_calls_in_bfloat16_round_only_their_results(dev, B, heads, kv, dk, dv, tq, tk, train):
+    """Up to 16 M pairs (few columns over many keys: 1 M) P and dS keep 2^-18 of themselves, and 16 bits of the output go
+    into delta.  The rounding of the result, u = 2^-8, is then nearly all of the error: as much again as rounding the exact
+    result leaves, plus 2^-17 per term of sums that cancel to about a tenth of their terms: 2^-13 of the norm."""
+    from eeggan_amd import ops
+    q, k, v, g = make(B, heads, kv, dk, dv, tq, tk, torch.bfloat16, seed=3)
+    ins = [t.double().requires_grad_(True) for t in (q, k, v)]
+    want = plain(*ins, heads, kv, dk ** -0.5)
+    leaves = [t.to(dev).requires_grad_(train) for t in (q, k, v)]
+    got = ops.attention(*leaves, heads=heads, kv_heads=kv, scale=dk ** -0.5)
+    pairs = [("out", got, want.detach())]
+    if train:
+        pairs += list(zip("qkv", torch.autograd.grad(got, leaves, g.to(dev)), torch.autograd.grad(want, ins, g.double())))
+    for name, a, b in pairs:
+        alone = rel_err(b.to(torch.bfloat16), b)
+        assert rel_err(a, b) <= 1.02 * alone + 2.0 ** -13, (name, rel_err(a, b), alone)
