@@ -425,6 +425,8 @@ FwdPlan plan_of(const eeggan_attention& a) {
     return p;
 }
 
+constexpr size_t NEVER_NONE = 16;  // (a workspace of no bytes says that the descriptor was rejected)
+
 size_t part_bytes(const eeggan_attention& a, const FwdPlan& p) {
     if (p.nparts == 1) return 0;
     const size_t ncols = (size_t)(a.H / a.KV) * a.Tq;
@@ -464,7 +466,7 @@ template <class T, int DK, int DV>
 int forward(const eeggan_attention& a, void* out, void* rest, float* lse, void* ws, size_t bytes, hipStream_t st) {
     const FwdPlan p = plan_of<T, DK, DV>(a);
     const size_t rel = positions_bytes(a);
-    EEGGAN_REQUIRE(bytes >= rel + part_bytes(a, p), "attention: workspace too small");
+    EEGGAN_REQUIRE(bytes >= rel + part_bytes(a, p) + NEVER_NONE, "attention: workspace too small");
     FwdArgs f;
     f.q = a.q, f.k = a.k, f.v = a.v;
     f.qsb = a.q_batch, f.qsc = a.q_channel, f.ksb = a.k_batch, f.ksc = a.k_channel, f.vsb = a.v_batch, f.vsc = a.v_channel;
@@ -491,7 +493,7 @@ extern "C" size_t eeggan_attention_fwd_workspace(const eeggan_attention* a) {
     if (check_attention("attention", a)) return 0;
     size_t parts = 0;
     EEGGAN_ATTENTION_CLASS(*a, parts = part_bytes(*a, (plan_of<T, DK, DV>(*a))))
-    return positions_bytes(*a) + parts + 16;
+    return positions_bytes(*a) + parts + NEVER_NONE;
 }
 
 extern "C" int eeggan_attention_fwd(const eeggan_attention* a, void* out, void* rest, float* lse, void* workspace,
