@@ -1759,22 +1759,29 @@ class _RelBias(Function):
     @staticmethod
     def backward(ctx, g):
         buckets, heads = ctx.cfg
-        gt = _RelBiasSum.apply(_chk(g, "relative bias cotangent"), buckets, heads) if ctx.needs_input_grad[1] else None
+        gt = None
+        if ctx.needs_input_grad[1]:  # (recorded only where a graph for second derivatives is being built)
+            sums = _RelBiasSum.apply if torch.is_grad_enabled() else _bucket_sums
+            gt = sums(_chk(g, "relative bias cotangent"), buckets, heads)
         return g if ctx.needs_input_grad[0] else None, gt, None, None, None
+
+
+def _bucket_sums(g, buckets, heads):
+    out = torch.empty((buckets.num_buckets, heads), device=g.device, dtype=torch.float32)
+    dims = (g.shape[0] // heads, heads, g.shape[1], g.shape[2])
+    with _on(g):
+        nbytes = _lib.load().eeggan_relative_bias_grad_workspace(buckets._ptr(), *dims)
+        ws = torch.empty(max(nbytes, 16), device=g.device, dtype=torch.uint8)
+        call("eeggan_relative_bias_grad", g.data_ptr(), buckets._ptr(), out.data_ptr(), *dims, ws.data_ptr(), nbytes,
+             _stream_of(g))
+    return out
 
 
 class _RelBiasSum(Function):
     @staticmethod
     def forward(ctx, g, buckets, heads):
         ctx.cfg = (buckets, heads, tuple(g.shape))
-        out = torch.empty((buckets.num_buckets, heads), device=g.device, dtype=torch.float32)
-        dims = (g.shape[0] // heads, heads, g.shape[1], g.shape[2])
-        with _on(g):
-            nbytes = _lib.load().eeggan_relative_bias_grad_workspace(buckets._ptr(), *dims)
-            ws = torch.empty(max(nbytes, 16), device=g.device, dtype=torch.uint8)
-            call("eeggan_relative_bias_grad", g.data_ptr(), buckets._ptr(), out.data_ptr(), *dims, ws.data_ptr(), nbytes,
-                 _stream_of(g))
-        return out
+        return _bucket_sums(g, buckets, heads)
 
     @staticmethod
     def backward(ctx, q):
@@ -1906,8 +1913,8 @@ class _Attention(Function):
             table, mask, rest = (t if t is None else t.contiguous() for t in (table, mask, rest))
             desc = _attention_desc(q, k, v, mask, table, ctx.cfg)
         a = ctypes.addressof(desc)
-        gq, gk, gv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
-        gt = torch.empty(table.shape, device=table.device, dtype=table.dtype) if want_table else None
+        gq, gk, gv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        gt = table.new_empty(table.shape) if want_table else None
         with _on(q):
             nbytes = _lib.load().eeggan_attention_bwd_workspace(a, want_table)
             ws = torch.empty(nbytes or 16, device=q.device, dtype=torch.uint8)

@@ -6,6 +6,7 @@ descriptor table travels in the kernel arguments, so ``step()`` makes no host<->
 synchronisation: it can be captured into a HIP graph and replayed."""
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 
@@ -24,8 +25,10 @@ DESC_BYTES = ctypes.sizeof(_Desc)
 
 
 def build_table(rows):
-    """rows: list of (p_ptr, g_ptr, m_ptr, v_ptr, step_ptr, n).  Returns a host ctypes array."""
-    return (_Desc * len(rows))(*rows)
+    """rows: list of (p_ptr, g_ptr, m_ptr, v_ptr, step_ptr, n).  Returns a host ctypes array (of ``_Desc``, whose fields are
+    all 64 bits wide: one flat array, a third of the time of a structure per row)."""
+    flat = array.array("Q", [x or 0 for row in rows for x in row])
+    return (ctypes.c_char * (8 * len(flat))).from_buffer(flat)
 
 
 def _grad_rows(grads, what):
@@ -177,9 +180,9 @@ class Adam(torch.optim.Optimizer):
         if not work:  # (tensors without elements)
             return
         device = grads[0].device
-        for g in grads:
-            if g.device != device or g.dtype != torch.float32:
-                raise RuntimeError(f"Adam: gradients of {g.dtype} on {g.device}, expected float32 on {device}")
+        if len({(g.dtype, g.get_device()) for g in grads} | {(torch.float32, device.index)}) != 1:
+            found = sorted({f"{g.dtype} on {g.device}" for g in grads})
+            raise RuntimeError(f"Adam: gradients of {', '.join(found)}, expected float32 on one device")
         if self._norm is None or self._norm.device != device:
             self._norm = torch.zeros(2, device=device, dtype=torch.float32)
         with torch.cuda.device(device):
