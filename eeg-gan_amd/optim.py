@@ -80,10 +80,10 @@ def grad_norm(grads):
 
 
 @torch.no_grad()
-def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
-    """``torch.nn.utils.clip_grad_norm_`` on this package's kernels: scales the gradients of ``parameters`` in place so
-    that their global 2-norm is at most ``max_norm`` (multiplier min(1, max_norm / (norm + 1e-6))) and returns the norm
-    they had, a 0-dim device tensor.  Nothing waits for the device unless ``error_if_nonfinite`` asks for the check; a
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
+    """``torch.nn.utils.clip_grad_norm_`` on this package's kernels (``foreach`` has no effect): scales the gradients of
+    ``parameters`` in place so that their global 2-norm is at most ``max_norm`` (multiplier
+    min(1, max_norm / (norm + 1e-6))) and returns the norm they had, a 0-dim device tensor.  Nothing waits for the device unless ``error_if_nonfinite`` asks for the check; a
     norm below the bound costs no second pass over the gradients.  ``Adam(max_grad_norm=...)`` needs no call of this:
     its step reads the multiplier and never writes clipped gradients."""
     if float(norm_type) != 2.0:

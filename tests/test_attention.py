@@ -663,3 +663,99 @@ def test_small_calls_in_bfloat16_round_only_their_results(dev, B, heads, kv, dk,
     for name, a, b in pairs:
         alone = rel_err(b.to(torch.bfloat16), b)
         assert rel_err(a, b) <= 1.02 * alone + 2.0 ** -13, (name, rel_err(a, b), alone)
+
+
+@pytest.mark.gpu
+def test_a_cache_past_four_gigabytes(dev):
+    """One new step, four key heads of 128 channels over 5 million keys in bfloat16: the last heads lie past 2^32 bytes.  The
+    last head against float32 products over pieces of the keys (out 2 u as above; the pieces' float32 sums do not count)."""
+    from eeggan_amd import ops
+    kv, d, tk, piece = 4, 128, 5_000_003, 500_000
+    gen = torch.Generator(device=dev).manual_seed(9)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=gen, dtype=torch.bfloat16)  # noqa: E731
+    q, k, v = rnd(1, kv * d, 1), rnd(1, kv * d, tk), rnd(1, kv * d, tk)
+    mask = torch.ones(1, tk, dtype=torch.bool, device=dev)
+    mask[0, 1_000_000:4_000_000] = False
+    with torch.no_grad():
+        got = ops.attention(q, k, v, heads=kv, scale=d ** -0.5, mask=mask)[0, -d:, 0].float()
+    s = torch.cat([q[0, -d:, 0].float() @ k[0, -d:, x:x + piece].float() for x in range(0, tk, piece)]) * d ** -0.5
+    p = torch.softmax(s.double().masked_fill(~mask[0], float("-inf")), 0).float()
+    want = sum(v[0, -d:, x:x + piece].float() @ p[x:x + piece] for x in range(0, tk, piece))
+    assert rel_err(got, want) <= 2 * U[torch.bfloat16]
+
+
+@pytest.mark.gpu
+def test_stored_scores_past_two_to_the_31(dev):
+    """Maps of 48000 x 48000: entry numbers pass 2^31.  scores + table (each entry one float32 addition: exact equality) on
+    rows at both ends, and the gradient of a table of ones' sum: counts of pairs, exact in double and float32 to half a step."""
+    from eeggan_amd import ops
+    n = 48000
+    b = ops.RelativeBuckets(16, 64)
+    table = torch.arange(16, device=dev, dtype=torch.float32)[:, None].requires_grad_(True)
+    scores = torch.full((1, n, n), 0.5, device=dev)
+    out = ops.relative_bias(scores, table, b)
+    bucket = positions(b, 129, 1)[0]  # distances 0 .. -128
+    for s in (0, 64, n - 1):
+        row = out[0, s].detach().cpu()
+        t = torch.arange(s, min(n, s + 129))
+        assert torch.equal(row[t], 0.5 + bucket[:len(t)].float()), s
+    gt, = torch.autograd.grad(out, [table], scores)
+    dist = torch.arange(n, dtype=torch.float64)
+    counts = torch.zeros(16, dtype=torch.float64)
+    for d, c in ((0, n),) + tuple((int(x), n - int(x)) for x in dist[1:64]):
+        counts[b.bucket(-d)] += c
+        if d:
+            counts[b.bucket(d)] += c
+    counts[b.bucket(-64)] += float((n - dist[64:]).sum())
+    counts[b.bucket(64)] += float((n - dist[64:]).sum())
+    assert float(((gt[:, 0].cpu().double() - 0.5 * counts).abs() - U[torch.float32] * 0.5 * counts).max()) <= 0.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [(1 << 30) - 1, -(1 << 30) + 1, 5000, -5000, 131, -131])
+def test_positions_far_from_the_queries(dev, offset):
+    """Every pair in one bucket (or, at the ends of the list, at the border): the bias drops out of the softmax."""
+    from eeggan_amd import ops
+    b = ops.RelativeBuckets(16, 40, step=3, offset=offset)
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v, g, table = (t.to(dev) for t in make(2, 2, 1, 16, 24, 70, 66, dtype, table=b))
+        leaves = [t.requires_grad_(True) for t in (q, k, v, table)]
+        out = ops.attention(*leaves[:3], heads=2, kv_heads=1, scale=0.25, bias=table, buckets=b)
+        got = torch.autograd.grad(out, leaves, g)
+        none = ops.attention(*leaves[:3], heads=2, kv_heads=1, scale=0.25)
+        want = torch.autograd.grad(none, leaves[:3], g)
+        if abs(offset) > 3 * 66 + 70 + 40:
+            assert rel_err(out, none) <= 2 * OUT[dtype] * U[dtype]
+            for a, w in zip(got, want):
+                assert rel_err(a, w) <= 2 * GRAD[dtype] * U[dtype]
+            assert int((got[3] != 0).any(1).sum()) <= 1
+        else:
+            check(dev, *(t.detach().cpu() for t in (q, k, v, g)), 2, 1, scale=0.25, table=table.detach().cpu(), buckets=b, what=offset)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(dev):
+    """Calls that run beside each other on two streams share nothing: the bits of calls that run alone."""
+    from eeggan_amd import ops
+    b = ops.RelativeBuckets(16, 64)
+    sets = [[t.to(dev) for t in make(2, 4, 2, 32, 32, 300 + 17 * i, 700, torch.bfloat16, seed=i, table=b)] for i in (0, 1)]
+    for s in sets:
+        for t in s[:3] + s[4:]:
+            t.requires_grad_(True)
+
+    def run(q, k, v, g, table):
+        out = ops.attention(q, k, v, heads=4, kv_heads=2, scale=0.2, bias=table, buckets=b)
+        return [out.detach()] + list(torch.autograd.grad(out, [q, k, v, table], g))
+
+    alone = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    results = [[], []]
+    for _ in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                results[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for got in results[i]:
+            assert all(torch.equal(a, w) for a, w in zip(got, alone[i]))
