@@ -759,3 +759,16 @@ def test_two_streams_at_once(dev):
     for i in (0, 1):
         for got in results[i]:
             assert all(torch.equal(a, w) for a, w in zip(got, alone[i]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dk,dv", [(32, 64), (24, 40), (17, 33), (33, 32), (32, 65)])
+def test_up_to_32_and_64_channels(dev, dk, dv, dtype):
+    from eeggan_amd import ops
+    buckets = ops.RelativeBuckets(16, 40, step=2)
+    for B, heads, kv, tq, tk in ((2, 1, 1, 70, 45), (1, 2, 2, 161, 130), (3, 4, 1, 1, 70)):
+        q, k, v, g = make(B, heads, kv, dk, dv, tq, tk, dtype)
+        check(dev, q, k, v, g, heads, kv, what=(dk, dv, tq, tk))
+    q, k, v, g, table = make(1, 2, 2, dk, dv, 140, 131, dtype, table=buckets)
+    check(dev, q, k, v, g, 2, 2, table=table, buckets=buckets, what=(dk, dv, "positions"))
