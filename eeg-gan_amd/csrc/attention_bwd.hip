@@ -75,6 +75,7 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
     const float c = a.scale * LOG2E;
     SFrag<NP, DK> fq[1];
     SFrag<NP, DV> fg[1];
+    // (delta in double: where a query's keys all share a bucket, its error is all that the query leaves in the table's gradient)
     float delta = 0.f;
     // Every other tile of queries works on -dS: the matrix instruction rounds an accumulator towards minus infinity where it
     // aligns it with larger products, a bias of 6e-9 of dP that the table's sums over all rows would add up
@@ -92,6 +93,7 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
 #pragma unroll
         for (int i = 0; i < FK::VALUES; ++i) x[i] = live && FK::channel(i, h) < a.Dk ? (NP == 3 ? x[i] * c : x[i]) : 0.f;
         fq[0].fill(h, x);
+        typename std::conditional<NP == 3, double, float>::type sum = 0;
         // (sixteen values of a lane at a time: all loads of 128 channels in flight spill registers)
         constexpr int SOME = FV::VALUES < 16 ? FV::VALUES : 16;
         static_unroll<FV::VALUES / SOME>([&](auto part) {
@@ -105,12 +107,18 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
             for (int i = 0; i < SOME; ++i) {
                 const bool ok = live && FV::channel(FIRST + i, h) < a.Dv;
                 const float v = ok ? yy[i] : 0.f;
-                delta = ok ? __builtin_fmaf(v, NP == 1 ? z[i] + zz[i] : z[i], delta) : delta;
+                if constexpr (NP == 3)
+                    sum = ok ? __builtin_fma((double)v, (double)z[i], sum) : sum;
+                else
+                    sum = ok ? __builtin_fmaf(v, z[i] + zz[i], sum) : sum;
                 y[FIRST + i] = sign * v;
             }
         });
         fg[0].fill(h, y);
-        delta = half_sum(delta);
+        if constexpr (NP == 3)
+            delta = (float)(sum + __shfl_xor(sum, 32, 64));
+        else
+            delta = half_sum(sum);
         if (inside && h == 0) a.delta[row * a.Tq + t] = delta;
     }
     const T* const kb = reinterpret_cast<const T*>(a.k) + b * a.ksb + (long long)kvh * a.Dk * a.ksc;
