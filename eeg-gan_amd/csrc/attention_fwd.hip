@@ -452,8 +452,10 @@ int launch_cut(const FwdArgs& f, const FwdPlan& p, hipStream_t st) {
     typedef Cuts<T, DK, DV> C;
     if constexpr (C::FEW_XT == 64) {
         if (p.kw == 2) {
-            if (f.fine) return launch<T, DK, DV, 2, 64, 1, BIAS>(f, p, st);
-            return launch<T, DK, DV, 2, 64, 1, BIAS, false>(f, p, st);
+            if constexpr (!BIAS) {  // (with a table bfloat16 is always fine)
+                if (!f.fine) return launch<T, DK, DV, 2, 64, 1, BIAS, false>(f, p, st);
+            }
+            return launch<T, DK, DV, 2, 64, 1, BIAS>(f, p, st);
         }
     }
     if constexpr (C::CB == 2) {
