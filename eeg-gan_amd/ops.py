@@ -1898,10 +1898,14 @@ class _Attention(Function):
         want_table = table is not None and need[3] and not _input_grad_only
         if torch.is_grad_enabled():
             # a graph for second derivatives is being built: the pass is made of operators that have them
-            ins = [q, k, v, table]
             wanted = [i for i in range(4) if need[i] and (i < 3 or want_table)]
+            if not wanted:
+                return None, None, None, None, None
             with torch.enable_grad():
-                again = _attention_stored(q, k, v, table, mask, ctx.cfg)
+                # an alias per argument: one tensor may be several of them, or be made from another, and each has to get
+                # its own part of the derivative (the graph behind the aliases is the caller's, which runs once)
+                ins = [t if t is None else t.view_as(t) for t in (q, k, v, table)]
+                again = _attention_stored(*ins, mask, ctx.cfg)
                 got = torch.autograd.grad(again, [ins[i] for i in wanted], g.float(), create_graph=True)
             grads = dict(zip(wanted, got))
             return tuple(grads.get(i) for i in range(4)) + (None,)

@@ -772,3 +772,81 @@ def test_up_to_32_and_64_channels(dev, dk, dv, dtype):
         check(dev, q, k, v, g, heads, kv, what=(dk, dv, tq, tk))
     q, k, v, g, table = make(1, 2, 2, dk, dv, 140, 131, dtype, table=buckets)
     check(dev, q, k, v, g, 2, 2, table=table, buckets=buckets, what=(dk, dv, "positions"))
+
+
+# ------------------------------------------------------------------------- inputs that share tensors, under create_graph
+def _shared(name, x, y, z):
+    """(q, k, v) out of three leaves: how arguments may depend on each other."""
+    return {"apart": (x, y, z), "k is v": (x, y, y), "q is k": (x, x, z), "all one": (x, x, x), "k from q": (x, 0.5 * x + y, z),
+            "v from k": (x, y, 2.0 * y * z)}[name]
+
+
+SHARED = ["apart", "k is v", "q is k", "all one", "k from q", "v from k"]
+
+
+@pytest.mark.parametrize("name", SHARED)
+def test_first_derivatives_under_create_graph_without_a_gpu(name, monkeypatch):
+    """The routing of _Attention.backward, with the formulas in float64 in the place of the stored-score operators: gradients
+    of first and second order, and one call of a hook on every leaf, as without the Function."""
+    from eeggan_amd import ops
+
+    class OnHost(ops._Attention):
+        @staticmethod
+        def forward(ctx, q, k, v, table, cfg):
+            ctx.cfg = cfg
+            ctx.save_for_backward(q, k, v, table, None, None, None, None)
+            return plain(q, k, v, 1, 1, 0.4)
+    monkeypatch.setattr(ops, "_attention_stored", lambda q, k, v, table, mask, cfg: plain(q.double(), k.double(), v.double(), 1, 1, 0.4))
+    gen = torch.Generator().manual_seed(4)
+    x, y, z, g = (torch.randn(2, 6, 9, generator=gen, dtype=torch.float64).requires_grad_(True) for _ in range(4))
+
+    def both(f):
+        calls = []
+        hooks = [t.register_hook(lambda grad, i=i: calls.append(i)) for i, t in enumerate((x, y, z))]
+        out = f(*_shared(name, x, y, z))
+        first = torch.autograd.grad(out, (x, y, z), g.float().double(), create_graph=True, allow_unused=True)
+        for h in hooks:
+            h.remove()
+        second = torch.autograd.grad(sum((t ** 3).sum() for t in first if t is not None), (x, y, z), allow_unused=True)
+        return first + second, sorted(calls)
+    want, want_calls = both(lambda q, k, v: plain(q, k, v, 1, 1, 0.4))
+    got, calls = both(lambda q, k, v: OnHost.apply(q, k, v, None, ()))
+    assert calls == want_calls
+    for a, b in zip(got, want):
+        assert (a is None) == (b is None)
+        # (the Function passes its cotangent on in float32: 2^-24 per pass; the rest is float64)
+        assert a is None or rel_err(a, b) <= 4 * 2.0 ** -24, (name, rel_err(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", SHARED)
+def test_derivatives_of_inputs_that_share_tensors(dev, name):
+    """First derivatives with and without create_graph, and second ones, against the formulas in float64 (GRAD, twice that
+    for the second, as above); leaves in a table's place too."""
+    from eeggan_amd import ops
+    b = ops.RelativeBuckets(16, 30)
+    x, y, z, g = make(2, 2, 2, 12, 12, 40, 40, torch.float32, seed=6)
+    table = torch.randn(16, 2, generator=torch.Generator().manual_seed(6))
+
+    def all_of(leaves, g, f, kernels):
+        x, y, z, t = leaves
+        args = _shared(name, x, y, z)
+        out = f(*args, t + x.mean() if name == "all one" else t)
+        quick = torch.autograd.grad(out, leaves, g, retain_graph=True, allow_unused=True) if kernels else None
+        first = torch.autograd.grad(out, leaves, g, create_graph=True, allow_unused=True)
+        second = torch.autograd.grad(sum((d ** 2).sum() for d in first if d is not None), leaves, allow_unused=True)
+        return quick, first, second
+    ins64 = [t.double().requires_grad_(True) for t in (x, y, z, table)]
+    _, want1, want2 = all_of(ins64, g.double(), lambda q, k, v, t: plain(q, k, v, 2, 2, 0.3, None, t, b), False)
+    ins = [t.to(dev).requires_grad_(True) for t in (x, y, z, table)]
+    quick, got1, got2 = all_of(ins, g.to(dev), lambda q, k, v, t: ops.attention(q, k, v, heads=2, scale=0.3, bias=t, buckets=b), True)
+    tap = []
+    args = _shared(name, *(t.detach() for t in ins64[:3]))
+    out = plain(*args, 2, 2, 0.3, None, ins64[3].detach() + (ins64[0].detach().mean() if name == "all one" else 0.0), b, tap)
+    terms, _ = table_terms(tap, out, g.double())  # (a table's gradient of first order: relative to its terms)
+    for got, want, bound in ((quick, want1, 1024), (got1, want1, 1024), (got2, want2, 2048)):
+        for i, (a, w) in enumerate(zip(got, want)):
+            assert (a is None) == (w is None)
+            if a is not None:
+                size = float(w.detach().norm()) if i < 3 or want is want2 else max(float(w.detach().norm()), terms)
+                assert float((a.detach().cpu().double() - w.detach()).norm()) <= bound * 2.0 ** -24 * size, (name, i, rel_err(a, w))
