@@ -109,7 +109,8 @@ class Adam(torch.optim.Optimizer):
     """``max_grad_norm``: bound of the global 2-norm of the gradients of a step (all parameter groups together, after
     ``grad_scale``); the step then uses min(1, max_grad_norm / (norm + 1e-6)) times the gradients, which stay as they
     are in ``p.grad``, and ``grad_norm`` holds the norm it found (a 0-dim device tensor that every step, captured ones
-    included, rewrites)."""
+    included, rewrites).  The bound is an attribute like ``grad_scale``: copies and pickles of the optimizer have it, its
+    ``state_dict`` (torch's layout) does not."""
 
     max_grad_norm = _norm = None  # (for objects that were pickled without them)
 
@@ -122,6 +123,12 @@ class Adam(torch.optim.Optimizer):
         self.grad_scale = 1.0  # set to 1/world_size when gradients arrive as a sum over ranks
         self.max_grad_norm = max_grad_norm
         self._norm = None  # device: (norm, multiplier) of the last clipped step
+
+    def __getstate__(self):
+        """Copies and pickles keep the bound and the gradients' scale (the base class keeps groups and state only); the norm
+        of the last step is not taken along."""
+        own = {k: self.__dict__[k] for k in ("grad_scale", "max_grad_norm") if k in self.__dict__}
+        return dict(super().__getstate__(), **own)
 
     @property
     def grad_norm(self):

@@ -303,3 +303,33 @@ def test_parameters_without_elements(dev):
     opt.step()
     assert abs(float(opt.grad_norm) - 5 ** 0.5) < 1e-6 and float(full.detach().max()) < 1.0
     assert float(optim.clip_grad_norm_([empty], 1.0)) == 0.0
+
+
+def test_copies_and_pickles_keep_the_bound():
+    import copy
+    import pickle
+    from eeggan_amd import optim
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = optim.Adam([p], lr=0.25, max_grad_norm=0.75)
+    opt.grad_scale = 0.5
+    opt._norm = torch.ones(2)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt)), copy.copy(opt)):
+        assert (other.max_grad_norm, other.grad_scale, other.grad_norm) == (0.75, 0.5, None)
+        assert other.param_groups[0]["lr"] == 0.25
+    assert copy.deepcopy(optim.Adam([p])).max_grad_norm is None
+
+
+@pytest.mark.gpu
+def test_a_copied_optimizer_steps_alike(dev):
+    import copy
+    from eeggan_amd import optim
+    p = torch.nn.Parameter(torch.ones(700, device=dev))
+    opt = optim.Adam([p], lr=0.1, betas=(0.5, 0.99), max_grad_norm=0.5)
+    opt.grad_scale = 0.25
+    p.grad = torch.linspace(-3, 5, 700, device=dev)
+    opt.step()
+    both = copy.deepcopy([p, opt])
+    both[0].grad = p.grad.clone()
+    opt.step()
+    both[1].step()
+    assert torch.equal(p, both[0]) and torch.equal(opt.grad_norm, both[1].grad_norm) and both[1].grad_norm is not None
