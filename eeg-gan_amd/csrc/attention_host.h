@@ -30,19 +30,21 @@ constexpr size_t MAX_BAND = 2 * (1024 + 31 * 16 + 31) + 1;  // 2 width + 1 at th
 inline bool few_columns(const eeggan_attention& a) { return (long long)(a.H / a.KV) * a.Tq <= 32 && a.Tk > 64; }
 
 // bfloat16: whether P and dS meet their products in two bf16 pieces (2^-18 of them is left) instead of one (2^-9).
-//   * A call of up to 16 M pairs takes as long as its launches; there the second pieces cost nothing that can be measured
-//     (8 x 8 heads of 64 channels, 512 steps, 16 M pairs: training 133 us without, 131 with, forward 17 and 17) and leave
-//     the results' own rounding as the largest.  Beyond, they cost up to 30% (1024 steps: 131 and 144 us, 2048: 387 and
-//     496).  A few columns over many keys are bound by reading those: 8 x 16 heads of 128 over 16384 keys, 48 us without,
-//     55 with; there from 1 M pairs on there is one piece.
+//   * By the pairs of ONE sample (all its heads), so that a sample is rounded alike alone and in any batch.
+//   * Up to 16 M of them: in calls of no more pairs than that the second pieces cost nothing that can be measured (8 x 8 heads
+//     of 64 channels, 512 steps, 16 M pairs: training 133 us without, 131 with, forward 17 and 17), and they leave the results'
+//     own rounding as the largest; in larger batches of such samples they cost up to 10% (1024 steps: 131 and 144 us).
+//     Samples beyond have one piece: there the second would cost up to 30% (2048 steps: 387 and 496).  A few columns over
+//     many keys are bound by reading those: two pieces up to 1 M pairs (8 samples x 16 heads of 128 over 16384 keys, 0.26 M
+//     each: 57 us without, 63 with).
 //   * The forward pass also with a table, and for up to 64 keys.  The backward pass takes delta = sum_c dO O for
 //     sum_s P dP: with P rounded in O only, the two differ by 2^-9 / sqrt(keys) of dP, and every dS of the row with them.
 //     That shows in the table's gradient, where thousands of dS of both signs cancel (0.0028 of its norm, against 3e-4),
 //     and in rows of few keys.
-inline double pairs(const eeggan_attention& a) { return (double)a.B * a.H * a.Tq * a.Tk; }
-inline bool fine_backward(const eeggan_attention& a) { return a.bf16 && pairs(a) <= 16777216.0; }
+inline double sample_pairs(const eeggan_attention& a) { return (double)a.H * a.Tq * a.Tk; }
+inline bool fine_backward(const eeggan_attention& a) { return a.bf16 && sample_pairs(a) <= 16777216.0; }
 inline bool fine_forward(const eeggan_attention& a) {
-    return a.bf16 && (a.table || a.Tk <= 64 || pairs(a) <= (few_columns(a) ? 1048576.0 : 16777216.0));
+    return a.bf16 && (a.table || a.Tk <= 64 || sample_pairs(a) <= (few_columns(a) ? 1048576.0 : 16777216.0));
 }
 
 int check_attention(const char* what, const eeggan_attention* a);

@@ -1970,6 +1970,10 @@ def attention(q, k, v, *, heads: int = 1, kv_heads: Optional[int] = None, scale:
     left has zeros and no gradient.  ``bias`` [buckets.num_buckets, heads] (the operands' type or float32): learned bias
     by relative position; entries <= -1e30 bar their pairs.
 
+    bfloat16: a sample with up to 2^24 pairs heads * Tq * Tk (2^20 where at most 32 query columns share a key head) is off
+    by the rounding of its results; in larger ones the probabilities and their gradients are rounded to bfloat16 on the way
+    (error 1.4 times that).  The batch a sample comes in does not matter.
+
     Gradients of q, k, v and the table come from kernels with a fixed order of summation.  Under ``create_graph=True``
     the backward pass is made of the operators with stored scores instead (float32), which are twice differentiable."""
     kv_heads = heads if kv_heads is None else kv_heads

@@ -396,9 +396,9 @@ int eeggan_dot(const float* a, const float* b, float* out, size_t n, void* works
  * mask: [B, Tk] bytes, zero = key not attended by any query of the sample (its k and v are never used, whatever they
  * hold); NULL: all attended.  A query without any key to attend has a zero column in `out` and zero gradients.
  * All of q, k, v, out and the gradients are float32 (products exact to float32 rounding) or, with bf16 = 1, bfloat16
- * (P and dS enter their products as one bfloat16 piece; as two, which leave 2^-18, in calls of up to 2^24 pairs (2^20
- * where up to 32 query columns share a key head), and in the forward pass also with a table and for up to 64 keys; sums
- * and statistics are float32).  Dk, Dv <= 128; any alignment of the elements' own size; channel strides and Tq up to
+ * (P and dS enter their products as one bfloat16 piece; as two, which leave 2^-18, where a sample has up to 2^24 pairs
+ * H Tq Tk (2^20 where up to 32 query columns share a key head), and in the forward pass also with a table and for up to 64
+ * keys: whatever B is; sums and statistics are float32).  Dk, Dv <= 128; any alignment of the elements' own size; channel strides and Tq up to
  * 2^31 / 128 bytes.
  * Positions: query t lies at t, key s at step * s + offset; distance rel = step * s + offset - t.  table is
  * [count, H], float32 or (table_bf16) bfloat16; bias(s,t) = table[bucket(rel), h].  Entries <= -1e30 bar their pairs. */

@@ -850,3 +850,25 @@ def test_derivatives_of_inputs_that_share_tensors(dev, name):
             if a is not None:
                 size = float(w.detach().norm()) if i < 3 or want is want2 else max(float(w.detach().norm()), terms)
                 assert float((a.detach().cpu().double() - w.detach()).norm()) <= bound * 2.0 ** -24 * size, (name, i, rel_err(a, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,heads,kv,dk,dv,tq,tk,train", [(50, 2, 2, 16, 16, 420, 420, True), (9, 8, 4, 32, 32, 1, 20000, False)])
+def test_a_sample_is_rounded_alike_in_any_batch(dev, B, heads, kv, dk, dv, tq, tk, train):
+    """bfloat16: how P and dS are rounded depends on a sample, not on its neighbours: calls of more than 2^24 pairs (2^20
+    for few columns) in small samples keep the bound of small calls above."""
+    from eeggan_amd import ops
+    assert B * heads * tq * tk > (1 << 24 if tq > 1 else 1 << 20) >= heads * tq * tk
+    q, k, v, g = make(B, heads, kv, dk, dv, tq, tk, torch.bfloat16, seed=8)
+    leaves = [t.to(dev).requires_grad_(train) for t in (q, k, v)]
+    got = ops.attention(*leaves, heads=heads, kv_heads=kv, scale=dk ** -0.5)
+    grads = torch.autograd.grad(got, leaves, g.to(dev)) if train else ()
+    for b in (0, B - 1):
+        ins = [t[b:b + 1].double().requires_grad_(True) for t in (q, k, v)]
+        want = plain(*ins, heads, kv, dk ** -0.5)
+        pairs = [("out", got[b:b + 1], want.detach())]
+        if train:
+            pairs += list(zip("qkv", (x[b:b + 1] for x in grads), torch.autograd.grad(want, ins, g[b:b + 1].double())))
+        for name, a, w in pairs:
+            alone = rel_err(w.to(torch.bfloat16), w)
+            assert rel_err(a, w) <= 1.02 * alone + 2.0 ** -13, (b, name, rel_err(a, w), alone)
