@@ -225,8 +225,10 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
                     } else {
                         // the tile goes through LDS and every lane adds up one distance's pairs (row i, column
                         // step i - distance, of the tile), 64 distances at a time
+                        wave_exchange();  // (the last tile's values are read, its histogram entries written)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) square[acc_row(r, h) * 33 + l31] = ds[r];
+                        wave_exchange();
                         const int step = a.pos.step, span = 31 * step + 32, most = (32 + step - 1) / step;
                         float* const hp = hist + (int)((long long)step * s + a.pos.offset - t0 + width) - 31;
                         for (int d0 = 0; d0 < span; d0 += 64) {

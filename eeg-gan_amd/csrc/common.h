@@ -131,6 +131,14 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
+// Between the lanes of one wave that hand each other values through LDS: everything before is written before anything
+// after is read.  (The hardware keeps a wave's LDS accesses in order and waits for nothing here; the compiler has to be told.)
+__device__ __forceinline__ void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Sum over a 256-thread block; every thread gets the result.  `red` holds >= 4 floats.
 __device__ __forceinline__ float block_sum_256(float v, float* red) {
     v = wave_sum(v);

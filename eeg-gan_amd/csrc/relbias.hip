@@ -110,6 +110,7 @@ __global__ __launch_bounds__(256) void relbias_sums_kernel(const float* __restri
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double* const mine = band + wave * (n + 2);
     for (int i = lane; i < n + 2; i += 64) mine[i] = 0.0;
+    wave_exchange();
     const long long bh = blockIdx.x / chunks;
     const int chunk = (int)(blockIdx.x % chunks);
     const int s0 = chunk * rows, s1 = min(Tk, s0 + rows);
