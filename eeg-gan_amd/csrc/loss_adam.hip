@@ -601,40 +601,41 @@ __global__ __launch_bounds__(256) void grad_square_kernel(NormPack pk, double* _
     if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// The partial sums' sum -> out[0] = norm, out[1] = multiplier.
+__global__ __launch_bounds__(1024) void grad_norm_final_kernel(const double* __restrict__ part, int64_t nparts, double scale,
+                                                               double max_norm, float* __restrict__ out) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < nparts; i += 1024) s += part[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < 16; ++i) t += red[i];
+        const double norm = fabs(scale) * sqrt(t);
+        const double c = max_norm / (norm + 1e-6);
+        out[0] = (float)norm;
+        out[1] = (float)(scale * (c > 1.0 ? 1.0 : c));  // (a NaN norm spoils the multiplier, as it should)
+    }
+}
+
 constexpr int SMAXT = 384;
 struct StepPack {
     float* step[SMAXT];
     int count;
 };
 
-// The partial sums' sum -> out[0] = norm, out[1] = multiplier (nparts > 0); then, for an optimizer step, the tensors'
-// step counters advance and their bias corrections are formed (in double: 1 - 0.99^t loses six bits in float32).
-__global__ __launch_bounds__(1024) void grad_norm_final_kernel(const double* __restrict__ part, int64_t nparts, double scale,
-                                                               double max_norm, float* __restrict__ out, StepPack sp,
-                                                               float* __restrict__ factors, double lr, double b1, double b2) {
-    __shared__ double red[16];
-    if (nparts > 0) {
-        double s = 0.0;
-        for (int64_t i = threadIdx.x; i < nparts; i += 1024) s += part[i];
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            double t = 0.0;
-            for (int i = 0; i < 16; ++i) t += red[i];
-            const double norm = fabs(scale) * sqrt(t);
-            const double c = max_norm / (norm + 1e-6);
-            out[0] = (float)norm;
-            out[1] = (float)(scale * (c > 1.0 ? 1.0 : c));  // (a NaN norm spoils the multiplier, as it should)
-        }
-    }
-    for (int i = threadIdx.x; i < sp.count; i += 1024) {
-        const float step = sp.step[i][0] + 1.f;
-        sp.step[i][0] = step;
-        factors[2 * i] = (float)(lr / (1.0 - pow(b1, (double)step)));
-        factors[2 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)step)));
-    }
+// The tensors' step counters advance, and their bias corrections are formed (in double: 1 - 0.99^t loses six bits in float32).
+__global__ __launch_bounds__(SMAXT) void adam_factors_kernel(StepPack sp, float* __restrict__ factors, double lr, double b1,
+                                                             double b2) {
+    const int i = threadIdx.x;
+    if (i >= sp.count) return;
+    const float step = sp.step[i][0] + 1.f;
+    sp.step[i][0] = step;
+    factors[2 * i] = (float)(lr / (1.0 - pow(b1, (double)step)));
+    factors[2 * i + 1] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)step)));
 }
 
 // g *= multiplier in place; a multiplier of one leaves the tensors as they are, without touching them
@@ -788,10 +789,8 @@ extern "C" int eeggan_grad_norm(const eeggan_adam_tensor* table, int ntensors, f
     double* part = reinterpret_cast<double*>(workspace);
     int64_t nparts;
     if (launch_squares("grad_norm", table, ntensors, part, &nparts, as_stream(stream))) return 1;
-    StepPack none;
-    none.count = 0;
     hipLaunchKernelGGL(grad_norm_final_kernel, dim3(1), dim3(1024), 0, as_stream(stream), part, nparts, (double)scale, max_norm,
-                       norm, none, nullptr, 0.0, 0.0, 0.0);
+                       norm);
     return check_launch("grad_norm (sum)");
 }
 
@@ -825,8 +824,7 @@ extern "C" int eeggan_adam_step_clipped(const eeggan_adam_tensor* table, int nte
         StepPack sp;
         sp.count = ntensors - first < SMAXT ? ntensors - first : SMAXT;
         for (int i = 0; i < sp.count; ++i) sp.step[i] = table[first + i].step;
-        hipLaunchKernelGGL(grad_norm_final_kernel, dim3(1), dim3(1024), 0, st, nullptr, (int64_t)0, 0.0, 0.0, nullptr, sp,
-                           factors + 2 * first, lr, beta1, beta2);
+        hipLaunchKernelGGL(adam_factors_kernel, dim3(1), dim3(SMAXT), 0, st, sp, factors + 2 * first, lr, beta1, beta2);
         if (check_launch("adam_step_clipped (steps)")) return 1;
     }
     for (int first = 0; first < ntensors; first += MAXT) {
