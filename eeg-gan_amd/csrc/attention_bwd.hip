@@ -389,10 +389,7 @@ __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ?
         char* const qt = smem + buf * Cut::STAGE;
         char* const gt = qt + QT::BYTES;
         Steps<XT> steps;
-        unsigned char all[(XT + 63) / 64];
-#pragma unroll
-        for (int i = 0; i < (XT + 63) / 64; ++i) all[i] = 1;
-        steps.find(ahead, a.Tq, all, lane);
+        steps.find(ahead, a.Tq, 1, lane);
         qblk.store(qt, a.Dk, steps, tid);
         gblk.store(gt, a.Dv, steps, tid);
         if (tid < 2 * XT) reinterpret_cast<float*>(gt + GT::BYTES)[tid] = stat;

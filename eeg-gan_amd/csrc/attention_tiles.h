@@ -135,38 +135,27 @@ __device__ __forceinline__ int n_off(int x) { return 2 * ((x & ~31) + (x & 16) +
 // Which steps of a stage count, one bit each (the same in every lane).
 template <int XT>
 struct Steps {
-    unsigned long long w[(XT + 63) / 64];
+    static_assert(XT <= 64, "one word");
+    unsigned long long w;
     // steps [x0, x0 + XT) of `len`, less the masked ones: `raw` is what StepsAhead read for them
-    __device__ __forceinline__ void find(int x0, int len, const unsigned char (&raw)[(XT + 63) / 64], int lane) {
-#pragma unroll
-        for (int i = 0; i < (XT + 63) / 64; ++i)
-            w[i] = __ballot(64 * i + lane < XT && x0 + 64 * i + lane < len && raw[i] != 0);
+    __device__ __forceinline__ void find(int x0, int len, unsigned char raw, int lane) {
+        w = __ballot(lane < XT && x0 + lane < len && raw != 0);
     }
-    __device__ __forceinline__ bool all() const {
-        bool a = true;
-#pragma unroll
-        for (int i = 0; i < (XT + 63) / 64; ++i) a = a && w[i] == (XT >= 64 ? ~0ull : (1ull << (XT & 63)) - 1);
-        return a;
-    }
-    __device__ __forceinline__ unsigned tile(int x0) const {  // the 32 steps from x0
-        return (unsigned)(w[XT > 64 && x0 >= 64 ? (XT + 63) / 64 - 1 : 0] >> (x0 & 32));
-    }
-    __device__ __forceinline__ unsigned quad(int kq) const {  // the four steps from 4 kq
-        return (unsigned)((XT > 64 && kq >= 16 ? w[(XT + 63) / 64 - 1] : w[0]) >> (4 * (kq & 15))) & 15u;
-    }
+    __device__ __forceinline__ bool all() const { return w == ~0ull >> (64 - XT); }
+    __device__ __forceinline__ unsigned tile(int x0) const { return (unsigned)(w >> x0); }            // the 32 steps from x0
+    __device__ __forceinline__ unsigned quad(int kq) const { return (unsigned)(w >> (4 * kq)) & 15u; }  // the four from 4 kq
 };
 
 // The mask bytes of a stage on their way: read with the stage's data and looked at only when that is stored (a vote right
 // behind the loads would wait for all of them).
 template <int XT>
 struct StepsAhead {
-    unsigned char raw[(XT + 63) / 64];
+    unsigned char raw;
     int x0;
     // mask: nonzero bytes count; null: all
     __device__ __forceinline__ void load(int first, int len, const unsigned char* mask, int lane) {
         x0 = first;
-#pragma unroll
-        for (int i = 0; i < (XT + 63) / 64; ++i) raw[i] = mask ? mask[min(first + 64 * i + lane, len - 1)] : 1;
+        raw = mask ? mask[min(first + lane, len - 1)] : 1;
     }
 };
 
