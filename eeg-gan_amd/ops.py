@@ -1968,7 +1968,12 @@ def attention(q, k, v, *, heads: int = 1, kv_heads: Optional[int] = None, scale:
     layouts are copied).  ``kv_heads`` (default ``heads``): query head h reads key head h // (heads // kv_heads).
     ``mask``: bool [B, Tk], True = this key may be attended; what masked keys hold is never used.  A query with no key
     left has zeros and no gradient.  ``bias`` [buckets.num_buckets, heads] (the operands' type or float32): learned bias
-    by relative position; entries <= -1e30 bar their pairs.
+    by relative position; entries <= -1e30 bar their pairs (weight zero).
+
+    Attended inputs have to be finite, and so do the float32 sums they go into: scale * log2(e) * sum |k q|, and
+    256 * Tk * max |v|, because the weights are divided by their sum at the end.  Anything else that is attended makes what
+    it reaches (a query its column, a value its channel, a key its sample's queries) NaN or infinite, not always as the
+    formula would: float32 operands are multiplied in three pieces, and an infinity has none.
 
     bfloat16: a sample with up to 2^24 pairs heads * Tq * Tk (2^20 where at most 32 query columns share a key head) is off
     by the rounding of its results; in larger ones the probabilities and their gradients are rounded to bfloat16 on the way

@@ -395,6 +395,9 @@ int eeggan_dot(const float* a, const float* b, float* out, size_t n, void* works
  * strides are given in elements.  H = KV * (query heads that share a key head): query head h reads key head h / (H / KV).
  * mask: [B, Tk] bytes, zero = key not attended by any query of the sample (its k and v are never used, whatever they
  * hold); NULL: all attended.  A query without any key to attend has a zero column in `out` and zero gradients.
+ * What is attended has to be finite, as do |scale| log2(e) sum |k q| and 256 Tk max |v| (float32 sums, divided at the end);
+ * an infinity or NaN there spoils its own query's, value's or key's part of the results, as NaN where a formula might keep an
+ * infinity.
  * All of q, k, v, out and the gradients are float32 (products exact to float32 rounding) or, with bf16 = 1, bfloat16
  * (P and dS enter their products as one bfloat16 piece; as two, which leave 2^-18, where a sample has up to 2^24 pairs
  * H Tq Tk (2^20 where up to 32 query columns share a key head), and in the forward pass also with a table and for up to 64

@@ -872,3 +872,34 @@ def test_a_sample_is_rounded_alike_in_any_batch(dev, B, heads, kv, dk, dv, tq, t
         for name, a, w in pairs:
             alone = rel_err(w.to(torch.bfloat16), w)
             assert rel_err(a, w) <= 1.02 * alone + 2.0 ** -13, (b, name, rel_err(a, w), alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("tq", [64, 2])
+def test_infinities_stay_where_they_belong(dev, tq, dtype):
+    """An infinite query spoils its own column, an infinite value its own channel (as NaN or infinity): nothing else, and
+    nothing of it looks like a number.  The largest values whose sums stay finite (256 Tk |v| < 2^128, and 2^120 twice in a
+    score of partners 2^-120) are numbers like any others."""
+    from eeggan_amd import ops
+    q, k, v, _ = make(2, 1, 1, 16, 32, tq, 70, dtype)
+    run = lambda q, k, v: ops.attention(q.to(dev), k.to(dev), v.to(dev), scale=0.25).cpu()  # noqa: E731
+    ref = run(q, k, v)
+    for inf in (float("inf"), float("-inf")):
+        q2, v2 = q.clone(), v.clone()
+        q2[0, 3, 1] = inf
+        v2[1, 5, 20] = inf
+        got = run(q2, k, v2)
+        bad = torch.zeros(got.shape, dtype=torch.bool)
+        bad[0, :, 1] = True
+        bad[1, 5, :] = True
+        assert not bool(torch.isfinite(got[bad]).any()) and torch.equal(got[~bad], ref[~bad])
+    v2, k2, q2 = v.clone(), k.clone(), q.clone()
+    v2[0, 3] *= 2.0 ** 110
+    q2[0, 1] *= 2.0 ** 120
+    k2[0, 1] *= 2.0 ** -120
+    got = run(q2, k2, v2)
+    want64 = plain(q.double(), k.double(), v.double(), 1, 1, 0.25)
+    want64[0, 3] *= 2.0 ** 110
+    for c in range(32):
+        assert rel_err(got[:, c], want64[:, c]) <= OUT[dtype] * U[dtype], c
