@@ -1,5 +1,5 @@
-// Backward pass of the fused attention: the probabilities are formed again from q, k and the forward's lse.
-//   P[s,t] = 2^(S log2e - lse[t]);  delta[t] = sum_c O dO;  dP = V^T dO;  dS = P (dP - delta)
+// Backward pass of the fused attention: the probabilities are formed again from q, k and the forward's m and log2 l.
+//   P[s,t] = 2^((S log2e - m[t]) - log2 l[t]);  delta[t] = sum_c O dO;  dP = V^T dO;  dS = P (dP - delta)
 //   dQ[d,t] = scale sum_s K[d,s] dS[s,t]          (attn_dq_kernel: a wave owns 32 queries, the keys stream through LDS)
 //   dV[c,s] = sum_t dO[c,t] P[s,t],  dK[d,s] = scale sum_t Q[d,t] dS[s,t]
 //                                                 (attn_dkv_kernel: a wave owns 32 keys, q and dO stream)
@@ -26,7 +26,7 @@ struct BwdArgs {
     long long qsb, qsc, ksb, ksc, vsb, vsc;
     const unsigned char* mask;
     const void *out, *rest, *g;  // [B, H Dv, Tq]; out + rest: the output before its rounding (float32: rest null)
-    const float* lse;
+    const float* lse;  // [2, B, H, Tq]: m, log2 l (infinite: no key)
     float* delta;  // [B, H, Tq]: written by attn_dq_kernel, read by attn_dkv_kernel
     void *gq, *gk, *gv;
     float* part;  // dK, dV of a split over the queries; null: not split
@@ -68,9 +68,10 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
     const bool inside = t0 + l31 < a.Tq;
     const int t = inside ? t0 + l31 : 0;
     const long long row = (long long)b * H + head;
-    float lse = a.lse[row * a.Tq + t];
-    const bool live = inside && lse != INFINITY;  // (a query without keys takes no part)
-    if (!live) lse = INFINITY;
+    const long long queries = (long long)a.B * H * a.Tq;
+    float ref = a.lse[row * a.Tq + t], lsum = a.lse[queries + row * a.Tq + t];
+    const bool live = inside && lsum != INFINITY;  // (a query without keys takes no part)
+    if (!live) ref = 0.f, lsum = INFINITY;
 
     const float c = a.scale * LOG2E;
     SFrag<NP, DK> fq[1];
@@ -129,8 +130,8 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
     float* const band = reinterpret_cast<float*>(smem + Cut::LDS);
     float side_bias[2] = {0.f, 0.f};
     if constexpr (BIAS) {
-        side_bias[0] = rel_at(a.pos, rel, a.Tq, -a.pos.far) - lse;
-        side_bias[1] = rel_at(a.pos, rel, a.Tq, a.pos.far) - lse;
+        side_bias[0] = (rel_at(a.pos, rel, a.Tq, -a.pos.far) - ref) - lsum;
+        side_bias[1] = (rel_at(a.pos, rel, a.Tq, a.pos.far) - ref) - lsum;
         fill_band(band, a.pos, rel, a.Tq, tid, THREADS);
     }
 
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
             const unsigned word = now.tile(x0);
             if (word == 0) continue;
             const int s = s0 + x0;
-            // (the scores accumulate from zero and meet lse once: on top of -lse every partial sum would be rounded at
-            // its magnitude)
+            // (the scores accumulate from zero and meet m and log2 l once: on top of them every partial sum would be rounded
+            // at their magnitude)
             f32x16 raw[1] = {zero16()}, dsv[1] = {dinit};
             two_scores<NP, DK, DV, XT>(kt + 2 * x0 + k_off, fq, raw, vt + 2 * x0 + v_off, fg, dsv, h);
             f32x16 &acc = raw[0], &ds = dsv[0];
@@ -202,9 +203,9 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
                                         a.pos.step * 4 * h - l31;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    acc[r] = __builtin_fmaf(acc[r], k1, r0[a.pos.step * ((r & 3) + 8 * (r >> 2))] - lse);
+                    acc[r] = __builtin_fmaf(acc[r], k1, (r0[a.pos.step * ((r & 3) + 8 * (r >> 2))] - ref) - lsum);
             } else {
-                const float base = !BIAS ? -lse : side < 0 ? side_bias[0] : side_bias[1];
+                const float base = !BIAS ? -(ref + lsum) : side < 0 ? side_bias[0] : side_bias[1];
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[r] = __builtin_fmaf(acc[r], k1, base);
             }
@@ -298,10 +299,11 @@ __global__ __launch_bounds__(THREADS, DK + DV > 160 && Elem<T>::NP == 3 ? 1 : 2)
 }
 
 // WK waves along the keys, WT = 4 / WK along the queries of a stage (their sums are joined through LDS at the end).
-template <class T, int DK, int DV, int WK, int XT>
+template <class T, int DK, int DV, int WK, int XT, bool BIAS>
 struct DkvCut {
     static constexpr int NP = Elem<T>::NP;
-    static constexpr int STAGE = Tile<NP, DK, XT>::BYTES + Tile<NP, DV, XT>::BYTES + 2 * XT * (int)sizeof(float);
+    static constexpr int STATS = BIAS ? 3 : 2;  // numbers per query
+    static constexpr int STAGE = Tile<NP, DK, XT>::BYTES + Tile<NP, DV, XT>::BYTES + STATS * XT * (int)sizeof(float);
     static constexpr int BUFS = 2 * STAGE <= 80 * 1024 ? 2 : 1;
     static constexpr int WORDS = (Tile<NP, DK, XT>::GROUPS + Tile<NP, DV, XT>::GROUPS) * 16 * 64;  // a wave's sums
     static constexpr int JOIN = (4 / WK - 1) * WK * WORDS * (int)sizeof(float);
@@ -311,13 +313,13 @@ struct DkvCut {
 // at 32 + 128 channels 78 / 54 us, at 96 94 / 111, at 128 107 / 279; float32 at 64 259 / 228, at 32 + 128 287 / 409).
 template <class T, int DK, int DV, int WK, int XT, bool BIAS>
 __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ? 1 : 2) void attn_dkv_kernel(BwdArgs a) {
-    typedef DkvCut<T, DK, DV, WK, XT> Cut;
+    typedef DkvCut<T, DK, DV, WK, XT, BIAS> Cut;
     constexpr int NP = Elem<T>::NP;
     constexpr int WT = 4 / WK, SUBS = XT / (32 * WT);
     typedef Tile<NP, DK, XT> QT;
     typedef Tile<NP, DV, XT> GT;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    // a stage: q, dO, then -lse and -delta of its queries
+    // a stage: q, dO, then of its queries -delta and -(m + log2 l), with a bias -delta, -log2 l and -m
 
     const int tid = threadIdx.x, lane = tid & 63, l31 = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -369,6 +371,7 @@ __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ?
     Block<T, DV, XT> gblk;
     qblk.init(a.qsc, a.Dk, tid);
     gblk.init(a.Tq, a.Dv, tid);
+    const long long queries = (long long)a.B * H * a.Tq;
     float stat = 0.f;
     int ahead = 0;  // first query of the stage that is on its way
     auto fetch = [&](int stage) {
@@ -378,11 +381,12 @@ __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ?
         qblk.load(reinterpret_cast<const T*>(a.q) + b * a.qsb + (long long)head * a.Dk * a.qsc, t0, a.Tq, tid);
         gblk.load(reinterpret_cast<const T*>(a.g) + row * a.Dv * a.Tq, t0, a.Tq, tid);
         ahead = t0;
-        if (tid < 2 * XT) {
-            const int t = t0 + tid % XT;
-            const float* p = (tid < XT ? a.lse : a.delta) + row * a.Tq;
-            const float x = -p[min(t, a.Tq - 1)];
-            stat = t < a.Tq ? x : tid < XT ? -INFINITY : 0.f;
+        if (tid < Cut::STATS * XT) {
+            const int t = t0 + tid % XT, which = tid / XT;
+            const long long at = row * a.Tq + min(t, a.Tq - 1);
+            float x = (which == 0 ? a.delta : which == 1 ? a.lse + queries : a.lse)[at];
+            if (!BIAS && which == 1) x += a.lse[at];
+            stat = t < a.Tq ? -x : which == 1 ? -INFINITY : 0.f;
         }
     };
     auto put = [&](int buf) {
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ?
         steps.find(ahead, a.Tq, 1, lane);
         qblk.store(qt, a.Dk, steps, tid);
         gblk.store(gt, a.Dv, steps, tid);
-        if (tid < 2 * XT) reinterpret_cast<float*>(gt + GT::BYTES)[tid] = stat;
+        if (tid < Cut::STATS * XT) reinterpret_cast<float*>(gt + GT::BYTES)[tid] = stat;
     };
     // position bias: near tiles read the stage's head's band in LDS, two of them so that the next head's can be filled
     // while the last one's is in use
@@ -436,11 +440,11 @@ __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ?
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 e = *reinterpret_cast<const f32x4*>(stats + x0 + 8 * i + 4 * h);
-                const f32x4 f = *reinterpret_cast<const f32x4*>(stats + XT + x0 + 8 * i + 4 * h);
+                const f32x4 f = *reinterpret_cast<const f32x4*>(stats + (BIAS ? 2 : 1) * XT + x0 + 8 * i + 4 * h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    acc[4 * i + j] = e[j];
-                    ds[4 * i + j] = f[j];
+                    ds[4 * i + j] = e[j];
+                    acc[4 * i + j] = f[j];
                 }
             }
             if constexpr (BIAS) {
@@ -455,6 +459,12 @@ __global__ __launch_bounds__(THREADS, DK + DV > (Elem<T>::NP == 3 ? 128 : 160) ?
                                             a.pos.step * l31;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[r] += r0[-acc_row(r, h)];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 e = *reinterpret_cast<const f32x4*>(stats + XT + x0 + 8 * i + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[4 * i + j] += e[j];
                 }
             }
             two_scores<NP, DK, DV, XT>(qt + 2 * x0 + q_off, fk, raw, gt + 2 * x0 + g_off, fv, dsv, h);
@@ -629,9 +639,9 @@ int launch_dq(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
 
 template <class T, int DK, int DV, int WK, int XT, bool BIAS>
 int launch_dkv(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
-    constexpr size_t tiles = DkvCut<T, DK, DV, WK, XT>::LDS, most = tiles + (BIAS ? 2 * MAX_BAND * sizeof(float) : 0);
+    constexpr size_t tiles = DkvCut<T, DK, DV, WK, XT, BIAS>::LDS, most = tiles + (BIAS ? 2 * MAX_BAND * sizeof(float) : 0);
     const size_t lds = tiles + (BIAS ? 2 * (2 * (size_t)f.pos.width + 1) * sizeof(float) : 0);
-    static_assert(most <= 160 * 1024 && 2 * XT <= THREADS, "LDS");
+    static_assert(most <= 160 * 1024 && 3 * XT <= THREADS, "LDS");
     auto kernel = &attn_dkv_kernel<T, DK, DV, WK, XT, BIAS>;
     static LdsReady ready;
     if (ready.reserve("attention backward", reinterpret_cast<const void*>(kernel), most)) return 1;

@@ -1,13 +1,16 @@
 // Attention over time, channels first, without storing the probabilities:
 //   S[s, t] = scale * sum_d K[d, s] Q[d, t] (+ the position bias of (s, t));  O[c, t] = sum_s V[c, s] softmax_s(S)[s, t]
 // One pass over the keys per query column with a running reference m and sum l (P' = 2^(S log2e - m), O = sum V P' / l);
-// what the backward pass needs besides its inputs is one number per query, lse = m + log2 l.
+// what the backward pass needs besides its inputs and the output are two numbers per query, m and log2 l (as their sum, log2 l
+// would be rounded at the magnitude of m, which is that of the position bias).
 //
 // A wave owns 32 query columns; the head's keys pass through LDS in stages shared by the workgroup's four waves.
 // A lane holds one query's column of S, so the statistics are per-lane scalars: the maximum over its sixteen
 // registers and one exchange between the lane halves, the sum without any exchange until the end.  The reference m
 // moves only when a score exceeds it by 8 (a factor 256: the sums stay far inside float32's range and lose
-// nothing), which after the first stages is rare, so the accumulators are hardly ever rescaled.
+// nothing), which after the first stages is rare, so the accumulators are hardly ever rescaled.  Where it moves far (scores
+// of -10^4 or -10^9 from a position bias, then ordinary ones), the tile's scores are formed again against the new one: on
+// top of the old one they were rounded at the distance's magnitude.
 // Few query columns (a single new step): the waves share the columns and split each stage's keys (KW > 1), and the keys
 // are split over workgroups; every part leaves (O unscaled, m, l) and attn_join_kernel combines them in a fixed order.
 //
@@ -27,7 +30,7 @@ struct FwdArgs {
     const unsigned char* mask;               // [B, Tk], nonzero = attended; null: all
     void* out;                               // [B, H Dv, Tq]
     void* rest;                              // what the rounding of out left over (bfloat16); null: not wanted
-    float* lse;                              // [B, H, Tq]; null: not wanted
+    float* lse;                              // [2, B, H, Tq]: m, log2 l; null: not wanted
     float* part;                             // parts of a split: O, then m, then l; null: not split
     Positions pos;
     int B, KV, G, Dk, Dv, Tq, Tk;
@@ -44,6 +47,9 @@ struct FwdCut {
     static constexpr int BUFS = 2 * STAGE <= 80 * 1024 ? 2 : 1;  // (two workgroups to a CU)
     static constexpr int LDS = BUFS * STAGE;
 };
+// A move of the reference by more than this has the tile's scores formed again: up to it they are rounded at 2^-16 at most.
+// (Moves up by more than 150 leave nothing of the sums so far: 2^-256 of them is zero.)
+constexpr float FAR_MOVE = 256.f;
 // FINE: has the code for a.fine (where it is not taken its registers cost few columns 10%)
 template <class T, int DK, int DV, int KW, int XT, int CB, bool BIAS, bool FINE>
 __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
@@ -167,76 +173,98 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
             }
             if (any == 0 || col0 >= ncols) continue;  // (the same for every lane of the wave)
             f32x16 acc[J][CB];
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int x0 = 32 * (KW == 1 ? u + j : ksub);
-#pragma unroll
-                for (int i = 0; i < CB; ++i) acc[j][i] = zero16();
-                mma_scores<NP, DK, XT, CB>(kt + 2 * x0 + k_off, h, fq, acc[j]);
-            }
-#pragma unroll
-            for (int i = 0; i < CB; ++i) {
+            auto form = [&](bool first) __attribute__((always_inline)) {
+                int at = s0;
+                if constexpr (BIAS) asm volatile("" : "+s"(at));  // (or the loop below keeps every address in registers)
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const int x0 = 32 * (KW == 1 ? u + j : ksub);
-                    if constexpr (BIAS) {
-                        const int s = s0 + x0, n0 = col0 + 32 * i, t0 = n0 % a.Tq;
-                        const int side = one_head[i] ? tile_side(a.pos, s, t0) : 0;
-                        if (side != 0) {
-                            const float base = (side < 0 ? beyond[i][0] : beyond[i][1]) - m[i];
 #pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c, base);
-                        } else if (one_head[i]) {
-                            const float* const r0 = bands + i * (2 * a.pos.width + 1) +
-                                                    (int)((long long)a.pos.step * s + a.pos.offset - t0 + a.pos.width) +
-                                                    a.pos.step * 4 * h - l31;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c,
-                                                              r0[a.pos.step * ((r & 3) + 8 * (r >> 2))] - m[i]);
-                        } else {
-                            const int first = min(s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
-                            const float* r0 = rel[i] + (long long)a.pos.step * first;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c,
-                                                              r0[a.pos.step * min((r & 3) + 8 * (r >> 2), last)] - m[i]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            acc[j][i][r] = NP == 3 ? acc[j][i][r] - m[i] : __builtin_fmaf(acc[j][i][r], c, -m[i]);
-                    }
-                    if (word[j] != 0xffffffffu) {
-                        const unsigned w = word[j] >> (4 * h);
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            acc[j][i][r] = (w >> ((r & 3) + 8 * (r >> 2))) & 1u ? acc[j][i][r] : -INFINITY;
-                    }
+                    for (int i = 0; i < CB; ++i) acc[j][i] = zero16();
+                    mma_scores<NP, DK, XT, CB>(kt + 2 * x0 + k_off, h, fq, acc[j]);
                 }
-                float top = acc[0][i][0];
+                bool again = false;
 #pragma unroll
-                for (int j = 0; j < J; ++j)
+                for (int i = 0; i < CB; ++i) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[j][i][r]);
-                top = half_max(top);
-                const bool move = top > threshold[i];
-                if (__any(move)) {
-                    const float d = move ? top : 0.f;
-                    const float f = move && threshold[i] > 0.f ? __builtin_amdgcn_exp2f(-d) : 1.f;
-                    if (move) threshold[i] = 8.f;
-                    m[i] += d;
-                    l[i] *= f;
+                    for (int j = 0; j < J; ++j) {
+                        const int x0 = 32 * (KW == 1 ? u + j : ksub);
+                        if constexpr (BIAS) {
+                            const int s = at + x0, n0 = col0 + 32 * i, t0 = n0 % a.Tq;
+                            const int side = one_head[i] ? tile_side(a.pos, s, t0) : 0;
+                            if (side != 0) {
+                                const float base = (side < 0 ? beyond[i][0] : beyond[i][1]) - m[i];
 #pragma unroll
-                    for (int e = 0; e < VT::GROUPS; ++e)
+                                for (int r = 0; r < 16; ++r)
+                                    acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c, base);
+                            } else if (one_head[i]) {
+                                const float* const r0 = bands + i * (2 * a.pos.width + 1) +
+                                                        (int)((long long)a.pos.step * s + a.pos.offset - t0 + a.pos.width) +
+                                                        a.pos.step * 4 * h - l31;
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) o[i][e][r] *= f;
+                                for (int r = 0; r < 16; ++r)
+                                    acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c,
+                                                                  r0[a.pos.step * ((r & 3) + 8 * (r >> 2))] - m[i]);
+                            } else {
+                                const int first = min(s + 4 * h, a.Tk - 1), last = a.Tk - 1 - first;
+                                const float* r0 = rel[i] + (long long)a.pos.step * first;
+#pragma unroll
+                                for (int r = 0; r < 16; ++r)
+                                    acc[j][i][r] = __builtin_fmaf(acc[j][i][r], NP == 3 ? 1.f : c,
+                                                                  r0[a.pos.step * min((r & 3) + 8 * (r >> 2), last)] - m[i]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                acc[j][i][r] = NP == 3 ? acc[j][i][r] - m[i] : __builtin_fmaf(acc[j][i][r], c, -m[i]);
+                        }
+                        if (word[j] != 0xffffffffu) {
+                            const unsigned w = word[j] >> (4 * h);
+#pragma unroll
+                            for (int r = 0; r < 16; ++r)
+                                acc[j][i][r] = (w >> ((r & 3) + 8 * (r >> 2))) & 1u ? acc[j][i][r] : -INFINITY;
+                        }
+                    }
+                    float top = acc[0][i][0];
 #pragma unroll
                     for (int j = 0; j < J; ++j)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[j][i][r] -= d;
+                        for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[j][i][r]);
+                    top = half_max(top);
+                    const bool move = top > threshold[i];
+                    if (__any(move)) {
+                        // (d: what m really moves by)
+                        const float to = move ? m[i] + top : m[i], d = to - m[i];
+                        const bool far = move && first && fabsf(top) > FAR_MOVE;
+                        const float f = move && threshold[i] > 0.f ? __builtin_amdgcn_exp2f(-d) : 1.f;
+                        // far: nothing is left of the sums (f = 0, or there were none), and the second time starts them
+                        if (move) threshold[i] = far ? -INFINITY : 8.f;
+                        again = again || far;
+                        m[i] = to;
+                        l[i] *= f;
+#pragma unroll
+                        for (int e = 0; e < VT::GROUPS; ++e)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[i][e][r] *= f;
+#pragma unroll
+                        for (int j = 0; j < J; ++j)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) acc[j][i][r] -= d;
+                    }
                 }
+                return again;
+            };
+            // A second time where a reference moved far (see above): the scores are read again, not kept in registers for this.
+            // With a bias one copy of the code in a loop, without one two of them (loop / copies: a ragged batch with positions
+            // 258 / 285 us, one step over 16384 keys 66 / 59).
+            if constexpr (BIAS) {
+                for (bool first = true; __any(form(first)); first = false) asm volatile("" ::: "memory");
+            } else if (__builtin_expect(__any(form(true)), 0)) {
+                asm volatile("" ::: "memory");
+                form(false);
+            }
+#pragma unroll
+            for (int i = 0; i < CB; ++i) {
                 float s4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < J; ++j)
@@ -280,7 +308,11 @@ __global__ __launch_bounds__(THREADS, 2) void attn_fwd_kernel(FwdArgs a) {
         if (a.part == nullptr) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;  // (no key: a column of zeros)
             const long long row = (long long)b * a.KV * a.G + head[i];
-            if (a.lse && h == 0) a.lse[row * a.Tq + t[i]] = sum == 0.f ? INFINITY : m[i] + __builtin_amdgcn_logf(sum);
+            if (a.lse && h == 0) {
+                float* const stat = a.lse + row * a.Tq + t[i];
+                stat[0] = m[i];
+                stat[(long long)a.B * a.KV * a.G * a.Tq] = sum == 0.f ? INFINITY : __builtin_amdgcn_logf(sum);
+            }
             T* out = reinterpret_cast<T*>(a.out) + row * a.Dv * a.Tq + t[i];
             T* rest = NP == 1 && a.rest ? reinterpret_cast<T*>(a.rest) + row * a.Dv * a.Tq + t[i] : nullptr;
 #pragma unroll
@@ -373,7 +405,11 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(FwdArgs a, int npart
     const long long at = (row * a.Dv + d) * a.Tq + t;
     st1(reinterpret_cast<T*>(a.out) + at, v);
     if (Elem<T>::NP == 1 && a.rest) st1(reinterpret_cast<T*>(a.rest) + at, v - (float)(T)v);
-    if (a.lse && d == 0) a.lse[row * a.Tq + t] = l == 0.f ? INFINITY : top + __builtin_amdgcn_logf(l);
+    if (a.lse && d == 0) {
+        float* const stat = a.lse + row * a.Tq + t;
+        stat[0] = l == 0.f ? 0.f : top;
+        stat[(long long)a.B * a.KV * a.G * a.Tq] = l == 0.f ? INFINITY : __builtin_amdgcn_logf(l);
+    }
 }
 
 }  // namespace attn

@@ -1879,7 +1879,7 @@ class _Attention(Function):
         B, _, tq = q.shape
         out = q.new_empty((B, v.shape[1] // cfg[1] * heads, tq))
         rest = torch.empty_like(out) if keep and q.dtype is torch.bfloat16 else None
-        lse = torch.empty((B, heads, tq), device=q.device, dtype=torch.float32) if keep else None
+        lse = torch.empty((2, B, heads, tq), device=q.device, dtype=torch.float32) if keep else None
         with _on(q):
             nbytes = _lib.load().eeggan_attention_fwd_workspace(a)
             ws = torch.empty(nbytes or 16, device=q.device, dtype=torch.uint8)

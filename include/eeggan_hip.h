@@ -423,7 +423,8 @@ typedef struct {
     int B, H, KV, Dk, Dv, Tq, Tk;
     float scale;
 } eeggan_attention;
-/* out [B, H Dv, Tq]; lse [B, H, Tq] (float32, log2 of the softmax sums) and, for bfloat16, rest (like out: what the
+/* out [B, H Dv, Tq]; lse [2, B, H, Tq] (float32: log2 of the softmax sums as a reference and the log2 of the sum relative to
+ * it, infinite for a query without a key) and, for bfloat16, rest (like out: what the
  * rounding of out left over, so that sum_c out dO, from which dS is subtracted, is formed from 16 bits instead of 8);
  * both NULL when no backward pass follows, rest NULL for float32.
  * workspace: device memory of the size the _workspace function returns (0 for a rejected descriptor). */

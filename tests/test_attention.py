@@ -903,3 +903,35 @@ def test_infinities_stay_where_they_belong(dev, tq, dtype):
     want64[0, 3] *= 2.0 ** 110
     for c in range(32):
         assert rel_err(got[:, c], want64[:, c]) <= OUT[dtype] * U[dtype], c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("low", [-1e4, -1e9])
+@pytest.mark.parametrize("heads,kv,dk,dv,tq,tk,step,offset", [(2, 2, 8, 32, 300, 300, 1, 0), (2, 1, 64, 64, 200, 330, 1, -60), (1, 1, 16, 16, 2, 700, 1, -680),
+                                                              (2, 2, 32, 32, 40, 33, 1, 0), (1, 1, 24, 40, 130, 1100, 2, -1900)])
+def test_low_position_entries(dev, heads, kv, dk, dv, tq, tk, step, offset, low, dtype):
+    """Entries far below the scores that bar nothing (>= -1e30), as tables are written to keep attention near: everything far
+    behind, so that a row's first tiles are all low and ordinary scores follow; or (second head) all entries, which drop out
+    of the softmax.  The bias is added to scores of about 8 once, relative to the row's reference: the bounds are those of
+    ordinary tables."""
+    from eeggan_amd import ops
+    b = ops.RelativeBuckets(16, 40, step=step, offset=offset)
+    q, k, v, g, table = make(2, heads, kv, dk, dv, tq, tk, dtype, seed=5, table=b)
+    table[7, 0] = low  # (40 steps behind and more)
+    if heads > 1:
+        table[:, 1] = low
+    check(dev, q, k, v, g, heads, kv, table=table, buckets=b, what=(low, tq, tk))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("tq,tk", [(150, 300), (3, 2000), (500, 70)])
+def test_scores_that_rise_far(dev, tq, tk, dtype):
+    """Scores of -3000 and, some tiles later, ordinary ones: what is left of the row is as exact as without the others."""
+    n = 40 if tk < 300 else 130
+    q, k, v, g = make(2, 2, 2, 16, 32, tq, tk, dtype, seed=7)
+    q[:, ::16] = 8.0
+    k[:, ::16, :n] = -1500.0
+    k[:, ::16, n:] = 0.0
+    check(dev, q, k, v, g, 2, 2, what=(tq, tk))
