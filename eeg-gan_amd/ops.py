@@ -1857,7 +1857,8 @@ def _attention_stored(q, k, v, table, mask, cfg):
         t = table.float()
         barred = t <= -1e30
         s = relative_bias(s, t.masked_fill(barred, -1e30), buckets, heads)
-        mask_s = s.detach() > -5e29  # (barred pairs: weight zero, like masked keys)
+        with torch.no_grad():  # (barred pairs: weight zero, like masked keys)
+            mask_s = _RelBias.apply(None, (~barred).float(), buckets, heads, tuple(s.shape)) != 0
     else:
         mask_s = None
     if mask is not None:
@@ -1980,7 +1981,8 @@ def attention(q, k, v, *, heads: int = 1, kv_heads: Optional[int] = None, scale:
     (error 1.4 times that).  The batch a sample comes in does not matter.
 
     Gradients of q, k, v and the table come from kernels with a fixed order of summation.  Under ``create_graph=True``
-    the backward pass is made of the operators with stored scores instead (float32), which are twice differentiable."""
+    the backward pass is made of the operators with stored scores instead (float32, a bias far below the scores rounds
+    them), which are twice differentiable."""
     kv_heads = heads if kv_heads is None else kv_heads
     _attention_check(q, k, v, heads, kv_heads, mask, bias, buckets)
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad

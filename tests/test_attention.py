@@ -935,3 +935,20 @@ def test_scores_that_rise_far(dev, tq, tk, dtype):
     k[:, ::16, :n] = -1500.0
     k[:, ::16, n:] = 0.0
     check(dev, q, k, v, g, 2, 2, what=(tq, tk))
+
+
+@pytest.mark.gpu
+def test_entries_that_almost_bar_pairs(dev):
+    """Entries above -1e30 bar nothing, however low: a head whose entries are all -9e29 weighs keys of equal scores alike,
+    one whose entries are -1e30 has none; with and without create_graph."""
+    from eeggan_amd import ops
+    b = ops.RelativeBuckets(16, 40)
+    q, k, v, g = (t.to(dev) for t in make(2, 2, 2, 8, 16, 50, 33, torch.float32))
+    table = torch.full((16, 2), -9e29, device=dev)
+    table[:, 1] = -1e30
+    v.requires_grad_(True)
+    for graph in (False, True):
+        out = ops.attention(q, k, v, heads=2, scale=0.0, bias=table, buckets=b)
+        gv, = torch.autograd.grad(out, [v], g, create_graph=graph)
+        assert rel_err(gv[:, :16], (g[:, :16].double().sum(2, keepdim=True) / 33).expand(2, 16, 33)) <= 256 * 2.0 ** -24, graph
+        assert not gv[:, 16:].any() and not out[:, 16:].any()
