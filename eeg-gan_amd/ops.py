@@ -1760,7 +1760,7 @@ class _RelBias(Function):
     def backward(ctx, g):
         buckets, heads = ctx.cfg
         gt = None
-        if ctx.needs_input_grad[1]:  # (recorded only where a graph for second derivatives is being built)
+        if ctx.needs_input_grad[1] and not _input_grad_only:  # (recorded only where a graph for second derivatives is built)
             sums = _RelBiasSum.apply if torch.is_grad_enabled() else _bucket_sums
             gt = sums(_chk(g, "relative bias cotangent"), buckets, heads)
         return g if ctx.needs_input_grad[0] else None, gt, None, None, None

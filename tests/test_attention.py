@@ -952,3 +952,27 @@ def test_entries_that_almost_bar_pairs(dev):
         gv, = torch.autograd.grad(out, [v], g, create_graph=graph)
         assert rel_err(gv[:, :16], (g[:, :16].double().sum(2, keepdim=True) / 33).expand(2, 16, 33)) <= 256 * 2.0 ** -24, graph
         assert not gv[:, 16:].any() and not out[:, 16:].any()
+
+
+@pytest.mark.gpu
+def test_the_penalty_pass_forms_no_table_gradient(dev, monkeypatch):
+    """Where only the inputs' gradients are wanted (ops.input_grad_only: the gradient penalty's first pass) the sums by
+    buckets are left out, as weight gradients are; the penalty's own gradients are the same with them."""
+    from eeggan_amd import ops
+    b = ops.RelativeBuckets(16, 40)
+    gen = torch.Generator().manual_seed(3)
+    s, table = (torch.randn(*shape, generator=gen).to(dev).requires_grad_(True) for shape in ((4, 30, 60), (16, 2)))
+    counts, call = [], ops.call
+    monkeypatch.setattr(ops, "call", lambda name, *a: (counts.append(name), call(name, *a))[1])
+
+    def penalty():
+        out = ops.softmax_dim1(ops.relative_bias(s, table, b, heads=2))
+        first, = torch.autograd.grad((out ** 2).sum(), [s], create_graph=True)
+        return (first ** 2).sum()
+    want = torch.autograd.grad(penalty(), [s, table])
+    assert counts.count("eeggan_relative_bias_grad") == 2
+    counts.clear()
+    with ops.input_grad_only():
+        value = penalty()
+    assert "eeggan_relative_bias_grad" not in counts
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(value, [s, table]), want))
