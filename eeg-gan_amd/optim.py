@@ -160,6 +160,9 @@ class Adam(torch.optim.Optimizer):
                 g = grads.get(p) if grads is not None else p.grad
                 if g is None:
                     continue
+                if grads is not None and (g.numel() != p.numel() or g.dtype != p.dtype or g.device != p.device):
+                    raise RuntimeError(f"Adam: a gradient of {g.numel()} elements, {g.dtype} on {g.device}, for a parameter of "
+                                       f"{p.numel()}, {p.dtype} on {p.device}")
                 if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
                     raise RuntimeError("Adam: parameters must be contiguous float32 device tensors")
                 if not g.is_contiguous():

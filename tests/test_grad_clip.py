@@ -333,3 +333,16 @@ def test_a_copied_optimizer_steps_alike(dev):
     opt.step()
     both[1].step()
     assert torch.equal(p, both[0]) and torch.equal(opt.grad_norm, both[1].grad_norm) and both[1].grad_norm is not None
+
+
+@pytest.mark.parametrize("bound", [None, 1.0])
+def test_gradients_that_do_not_fit_are_refused(bound):
+    """Gradients handed to the step by hand (``p.grad`` is checked by torch): the kernel reads as many as the parameter has."""
+    from eeggan_amd import optim
+    p = torch.nn.Parameter(torch.zeros(5, 2))
+    opt = optim.Adam([p], max_grad_norm=bound)
+    for g in (torch.zeros(9), torch.zeros(10, dtype=torch.bfloat16), torch.zeros(10, device="meta")):
+        with pytest.raises(RuntimeError, match="for a parameter of 10, torch.float32 on cpu"):
+            opt.step(grads={p: g})
+    with pytest.raises(RuntimeError, match="contiguous float32 device tensors"):
+        opt.step(grads={p: torch.zeros(10)})
