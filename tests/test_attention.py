@@ -976,3 +976,34 @@ def test_the_penalty_pass_forms_no_table_gradient(dev, monkeypatch):
         value = penalty()
     assert "eeggan_relative_bias_grad" not in counts
     assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(value, [s, table]), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("positions_too", [False, True], ids=["plain", "positions"])
+@pytest.mark.parametrize("dtype,dk,dv", [(torch.bfloat16, 16, 32), (torch.bfloat16, 16, 64), (torch.bfloat16, 32, 32), (torch.bfloat16, 32, 64),
+                                         (torch.bfloat16, 64, 64), (torch.float32, 8, 32), (torch.float32, 32, 32)])
+@pytest.mark.parametrize("B,heads,kv,tq,tk", [(32, 8, 8, 300, 150), (128, 8, 4, 45, 70)])
+def test_calls_that_fill_the_chip(dev, B, heads, kv, tq, tk, dtype, dk, dv, positions_too):
+    """From 512 workgroups of 256 columns on, where a wave of the forward pass has two blocks of columns: against float64,
+    with masks (one sample without keys), with query heads that share a block, with a row's first tiles far below the rest."""
+    from eeggan_amd import ops
+    assert B * kv * ((heads // kv * tq + 255) // 256) >= 512
+    b = ops.RelativeBuckets(16, 40) if positions_too else None
+    q, k, v, g, *table = make(B, heads, kv, dk, dv, tq, tk, dtype, seed=11, table=b)
+    if b is not None:
+        table[0][7, ::2] = -1e9
+    mask = torch.rand(B, tk, generator=torch.Generator().manual_seed(1)) < 0.9
+    mask[B // 2] = False
+    mask[1, :100] = False
+    check(dev, q, k, v, g, heads, kv, mask=mask, table=table[0] if table else None, buckets=b, what=(B, tq, tk))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,dk,dv,masked", [(8, 64, 64, False), (2, 24, 40, True)])
+def test_samples_of_many_pairs_in_bfloat16(dev, kv, dk, dv, masked):
+    """More than 2^24 pairs in a sample: P and dS in one piece, the bounds of which are this file's general ones."""
+    heads, tq, tk = 8, 1530, 1477
+    assert heads * tq * tk > 1 << 24
+    q, k, v, g = make(1, heads, kv, dk, dv, tq, tk, torch.bfloat16, seed=12)
+    mask = torch.rand(1, tk, generator=torch.Generator().manual_seed(2)) < 0.95 if masked else None
+    check(dev, q, k, v, g, heads, kv, mask=mask, what=(kv, dk, dv))

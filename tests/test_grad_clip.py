@@ -346,3 +346,28 @@ def test_gradients_that_do_not_fit_are_refused(bound):
             opt.step(grads={p: g})
     with pytest.raises(RuntimeError, match="contiguous float32 device tensors"):
         opt.step(grads={p: torch.zeros(10)})
+
+
+@pytest.mark.gpu
+def test_more_elements_than_one_pass_of_the_grid(dev):
+    """Past 16.8 M elements the norm's workgroups walk over several chunks: norm, clipping and the bounded step."""
+    from eeggan_amd import optim
+    sizes = [20_000_003, 5, 9_000_001]
+    gen = torch.Generator(device=dev).manual_seed(1)
+    gs = [torch.randn(n, device=dev, generator=gen) * (1 + i) for i, n in enumerate(sizes)]
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in gs))
+    assert abs(float(optim.grad_norm(gs)) - norm) <= 2 * U * norm
+    ps = [torch.nn.Parameter(torch.zeros_like(g)) for g in gs]
+    for p, g in zip(ps, gs):
+        p.grad = g.clone()
+    opt = optim.Adam(ps, lr=0.5, betas=(0.0, 0.99), max_grad_norm=0.25 * norm)
+    opt.step()
+    c = 0.25 * norm / (norm + 1e-6)
+    for p, g in zip(ps, gs):
+        # (the first step with beta1 = 0: m = c g, v / (1 - 0.99) = m^2, so that every element moves by lr)
+        assert float((opt.state[p]["exp_avg"].double() - c * g.double()).abs().max()) <= 3 * U * c * float(g.abs().max())
+        seen = g.abs() > 1e-3
+        assert float((p.detach().double().abs()[seen] - 0.5).abs().max()) <= 0.5 * (64 * U + 1e-8 / (c * 1e-3))
+    assert abs(float(optim.clip_grad_norm_(ps, 0.25 * norm)) - norm) <= 2 * U * norm
+    for p, g in zip(ps, gs):
+        assert float((p.grad.double() - c * g.double()).abs().max()) <= 2 * U * c * float(g.abs().max())
