@@ -1853,21 +1853,20 @@ def _attention_stored(q, k, v, table, mask, cfg):
     rows = lambda t: t.reshape(B * heads, -1, t.shape[2])  # noqa: E731
     share = lambda t: rows(t.reshape(B, kv, 1, -1, tk).expand(B, kv, G, t.shape[1] // kv, tk).reshape(B, -1, tk))  # noqa: E731
     s = bmm(share(k), rows(q), trans_a=True, alpha=scale)
+    maps, keep = (B, heads, tk, tq), None  # (keep: pairs with a weight, broadcast over the maps)
     if table is not None:
         t = table.float()
         barred = t <= -1e30
         s = relative_bias(s, t.masked_fill(barred, -1e30), buckets, heads)
         with torch.no_grad():  # (barred pairs: weight zero, like masked keys)
-            mask_s = _RelBias.apply(None, (~barred).float(), buckets, heads, tuple(s.shape)) != 0
-    else:
-        mask_s = None
+            keep = (_RelBias.apply(None, (~barred).float(), buckets, heads, (heads, tk, tq)) != 0)[None]
     if mask is not None:
-        m = mask[:, None, :, None].expand(B, heads, tk, tq).reshape(B * heads, tk, tq)
-        mask_s = m if mask_s is None else m & mask_s
-        s = s.masked_fill(~m, -1e30)
+        mask = mask[:, None, :, None]
+        s = s.view(maps).masked_fill(~mask, -1e30).view(s.shape)
+        keep = mask if keep is None else keep & mask
     p = softmax_dim1(s)
-    if mask_s is not None:
-        p = p * mask_s
+    if keep is not None:
+        p = (p.view(maps) * keep).view(p.shape)
     return bmm(share(v), p).reshape(B, heads * dv, tq)
 
 
