@@ -13,9 +13,10 @@
 // histogram by distance that belongs to the wave: a fixed order, no races.  (LDS float atomics in the place of that took
 // ~300 cycles per instruction: 73 us of 167 at 4 x 6 heads over 1537 steps.)
 //
-// Measured, bfloat16, 8 samples x 8 heads of 64 channels over 2048 steps: queries 142 us = 725 TFLOP/s, keys 186 us = 740
-// (a large library product: 1330); float32, 8 x 8 x 1024: 147 us = 175 and 229 us = 150 TFLOP/s (library: 154).  Bound as
-// the forward pass is: the products fill half of the time, exponentials and staging the rest.
+// Measured (calls one after the other, both kernels together): bfloat16, 8 samples x 8 heads of 64 channels over 2048 steps
+// 273 us = 881 TFLOP/s over the seven products (a large library product: 1330), the keys' kernel 1.3 times as long as the
+// queries'; float32, 8 x 8 x 1024: 342 us = 176 TFLOP/s (library: 154).  Bound as the forward pass is: the products fill two
+// thirds of the time, exponentials and staging the rest.
 #include "attention_host.h"
 
 namespace eeggan {

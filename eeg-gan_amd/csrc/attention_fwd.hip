@@ -14,11 +14,12 @@
 // Few query columns (a single new step): the waves share the columns and split each stage's keys (KW > 1), and the keys
 // are split over workgroups; every part leaves (O unscaled, m, l) and attn_join_kernel combines them in a fixed order.
 //
-// Measured: bfloat16, 8 samples x 8 heads of 64 channels over 2048 steps 112 us = 610 TFLOP/s (a large library product: 1330).
-// What bounds it: products, exponentials with their sums, and the tiles' way through LDS share a wave's issue slots, and two
-// waves per SIMD do not overlap them fully (the exponentials left out save 20 us, the staging 35, the products 45).  Float32 (six products each, three pieces of P formed per pair): 8 x 8 x 1024 at 64 channels 115 us =
-// 149 TFLOP/s, the rate of a large float32 library product.  One step over 16384 keys (8 x 4 key heads of 128, bfloat16):
-// 48 us = 5.6 TB/s, all of it reading keys and values.
+// Measured (calls one after the other): bfloat16, 8 samples x 8 heads of 64 channels over 2048 steps 107 us = 642 TFLOP/s (a
+// large library product: 1330).  What bounds it: products, exponentials with their sums, and the tiles' way through LDS
+// share a wave's issue slots, and two waves per SIMD do not overlap them fully (the exponentials left out save 20 us, the
+// staging 35, the products 45).  Float32 (six products each, three pieces of P formed per pair): 8 x 8 x 1024 at 64 channels
+// 106 us = 162 TFLOP/s, the rate of a large float32 library product.  One step over 16384 keys (8 x 4 key heads of 128,
+// bfloat16, P in two pieces): 51 us = 5.3 TB/s, all of it reading keys and values.
 #include "attention_host.h"
 
 namespace eeggan {

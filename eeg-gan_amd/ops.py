@@ -1964,8 +1964,8 @@ def attention(q, k, v, *, heads: int = 1, kv_heads: Optional[int] = None, scale:
     [Tk, Tq] map ever being stored: the backward pass forms it again.
 
     q [B, heads * Dk, Tq], k [B, kv_heads * Dk, Tk], v [B, kv_heads * Dv, Tk], all float32 or all bfloat16 -> out
-    [B, heads * Dv, Tq]; Dk and Dv up to 128, any lengths from one step, any strides with unit stride in time (other
-    layouts are copied).  ``kv_heads`` (default ``heads``): query head h reads key head h // (heads // kv_heads).
+    [B, heads * Dv, Tq]; Dk and Dv up to 128, from one step to 2^22 (bfloat16 2^23), any strides with unit stride
+    in time (other layouts are copied).  ``kv_heads`` (default ``heads``): query head h reads key head h // (heads // kv_heads).
     ``mask``: bool [B, Tk], True = this key may be attended; what masked keys hold is never used.  A query with no key
     left has zeros and no gradient.  ``bias`` [buckets.num_buckets, heads] (the operands' type or float32): learned bias
     by relative position; entries <= -1e30 bar their pairs (weight zero).
