@@ -658,6 +658,7 @@ template <class T, int DK, int DV, bool BIAS>
 int backward(const BwdArgs& f, const BwdPlan& p, hipStream_t st) {
     typedef Cut<T, DK, DV> C;
     if (launch_dq<T, DK, DV, BIAS>(f, p, st)) return 1;
+    if (!f.gk) return 0;
     if constexpr (C::NARROW) {
         if (p.narrow) return launch_dkv<T, DK, DV, 2, 64, BIAS>(f, p, st);
     }
@@ -680,7 +681,7 @@ int backward_all(const eeggan_attention& a, const void* out, const void* rest, c
     f.coltiles = 0, f.nsplit = p.nsplit, f.nhist = 0, f.scale = a.scale, f.fine = fine_backward(a);
     if (positions(a, reinterpret_cast<float*>(ws), &f.pos, st)) return 1;
     if (a.table ? backward<T, DK, DV, true>(f, p, st) : backward<T, DK, DV, false>(f, p, st)) return 1;
-    if (p.nsplit > 1) {
+    if (p.nsplit > 1 && gk) {
         const long long nk = (long long)a.B * a.KV * a.Dk * a.Tk, nv = (long long)a.B * a.KV * a.Dv * a.Tk;
         const long long blocks = (nk + nv + THREADS - 1) / THREADS;
         EEGGAN_REQUIRE(blocks < (1ll << 31), "attention backward: too many outputs");
@@ -707,7 +708,7 @@ extern "C" int eeggan_attention_bwd(const eeggan_attention* a, const void* out, 
                                     const void* g, void* gq, void* gk, void* gv, void* g_table, void* workspace,
                                     size_t workspace_bytes, void* stream) {
     if (check_attention("attention backward", a)) return 1;
-    EEGGAN_REQUIRE(out && lse && g && gq && gk && gv && workspace, "attention backward: null pointer");
+    EEGGAN_REQUIRE(out && lse && g && gq && !gk == !gv && workspace, "attention backward: null pointer");
     EEGGAN_REQUIRE(!a->bf16 || rest, "attention backward: bfloat16 needs the rest of the output");
     EEGGAN_REQUIRE(!g_table || a->table, "attention backward: a table gradient without a table");
     int rc = 1;

@@ -99,7 +99,8 @@ __global__ __launch_bounds__(256) void relbias_kernel(const float* __restrict__ 
 // Sums of g by distance.  A wave takes every fourth of its workgroup's rows, 2048 values of a row at a time with all
 // loads in flight.  Four neighbouring values beyond the last edge on one side (most of a long row) go to one sum; the
 // others to a histogram by distance in LDS that belongs to the wave (within an instruction no two lanes share a
-// distance): a fixed order, and double throughout (the near entries of a long recording sum millions of terms).
+// distance): a fixed order, and in double (the near entries of a long recording sum millions of terms) but for
+// those four, which are added in float32.
 // 64 maps of 1920 x 1920: 168 us, 5.6 TB/s.  hist: [H][rows of partial sums][2 far + 1]: distances -(far - 1) .. far - 1,
 // then everything behind, then everything ahead.
 __global__ __launch_bounds__(256) void relbias_sums_kernel(const float* __restrict__ g, double* __restrict__ hist,

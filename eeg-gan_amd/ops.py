@@ -1917,13 +1917,15 @@ class _Attention(Function):
             table, mask, rest = (t if t is None else t.contiguous() for t in (table, mask, rest))
             desc = _attention_desc(q, k, v, mask, table, ctx.cfg)
         a = ctypes.addressof(desc)
-        gq, gk, gv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        gq = q.new_empty(q.shape)
+        gk, gv = (k.new_empty(k.shape), v.new_empty(v.shape)) if need[1] or need[2] else (None, None)
         gt = table.new_empty(table.shape) if want_table else None
         with _on(q):
             nbytes = _lib.load().eeggan_attention_bwd_workspace(a, want_table)
             ws = torch.empty(nbytes or 16, device=q.device, dtype=torch.uint8)
             call("eeggan_attention_bwd", a, out.data_ptr(), None if rest is None else rest.data_ptr(), lse.data_ptr(),
-                 g.data_ptr(), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), None if gt is None else gt.data_ptr(),
+                 g.data_ptr(), gq.data_ptr(), None if gk is None else gk.data_ptr(), None if gv is None else gv.data_ptr(),
+                 None if gt is None else gt.data_ptr(),
                  ws.data_ptr(), nbytes, _stream_of(q))
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, gt, None
 

@@ -431,8 +431,8 @@ typedef struct {
 size_t eeggan_attention_fwd_workspace(const eeggan_attention* a);
 int eeggan_attention_fwd(const eeggan_attention* a, void* out, void* rest, float* lse, void* workspace,
                          size_t workspace_bytes, void* stream);
-/* Gradients for the cotangent g of `out` (dense, like out): gq, gk, gv dense in their inputs' shapes and types,
- * g_table [count, H] in the table's type (NULL: not wanted).  Sums over samples, queries and shared heads run in a
+/* Gradients for the cotangent g of `out` (dense, like out): gq, gk, gv dense in their inputs' shapes and types (gk and gv
+ * both NULL: not wanted), g_table [count, H] in the table's type (NULL: not wanted).  Sums over samples, queries and shared heads run in a
  * fixed order: equal inputs give equal bits. */
 size_t eeggan_attention_bwd_workspace(const eeggan_attention* a, int want_table);
 int eeggan_attention_bwd(const eeggan_attention* a, const void* out, const void* rest, const float* lse, const void* g,

@@ -1007,3 +1007,44 @@ def test_samples_of_many_pairs_in_bfloat16(dev, kv, dk, dv, masked):
     q, k, v, g = make(1, heads, kv, dk, dv, tq, tk, torch.bfloat16, seed=12)
     mask = torch.rand(1, tk, generator=torch.Generator().manual_seed(2)) < 0.95 if masked else None
     check(dev, q, k, v, g, heads, kv, mask=mask, what=(kv, dk, dv))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_gradients_that_nobody_wants(dev, dtype, monkeypatch):
+    """Any subset of the inputs may want gradients: the bits of the call that wants all.  Where neither keys nor values are
+    among them the keys' pass does not run."""
+    from eeggan_amd import ops
+    b = ops.RelativeBuckets(16, 40)
+    base = [t.to(dev) for t in make(2, 2, 1, 16, 24, 300, 5000, dtype, table=b)]
+    g = base.pop(3)
+    calls, call = [], ops.call
+    monkeypatch.setattr(ops, "call", lambda name, *a: (calls.append((name, a)), call(name, *a))[1])
+
+    def grads(which):
+        ins = [t.clone().requires_grad_(i in which) for i, t in enumerate(base)]
+        out = ops.attention(*ins[:3], heads=2, kv_heads=1, scale=0.25, bias=ins[3], buckets=b)
+        calls.clear()
+        got = dict(zip(which, torch.autograd.grad(out, [ins[i] for i in which], g)))
+        (name, args), = calls
+        assert name == "eeggan_attention_bwd" and (args[6] is None) == (args[7] is None) == (not {1, 2} & set(which))
+        return got
+    want = grads((0, 1, 2, 3))
+    for which in ((0,), (1,), (2,), (3,), (0, 3), (1, 2), (0, 1)):
+        got = grads(which)
+        assert all(torch.equal(got[i], want[i]) for i in which), which
+
+
+def test_the_c_entry_point_takes_both_key_gradients_or_none():
+    import ctypes
+    from eeggan_amd import _lib, ops
+    lib = _lib.load()
+    a = ops._AttentionDesc()
+    a.q, a.k, a.v, a.B, a.H, a.KV, a.Dk, a.Dv, a.Tq, a.Tk, a.scale = 256, 512, 768, 1, 1, 1, 8, 8, 10, 10, 1.0
+    a.q_batch, a.q_channel, a.k_batch, a.k_channel, a.v_batch, a.v_channel = 80, 10, 80, 10, 80, 10
+    for gk, gv in ((256, None), (None, 256)):
+        assert lib.eeggan_attention_bwd(ctypes.byref(a), 256, None, 256, 256, 256, gk, gv, None, 256, 1 << 30, None) != 0
+        assert b"null pointer" in lib.eeggan_last_error()
+    # (neither: past this check, to the next that fails, the workspace's size)
+    assert lib.eeggan_attention_bwd(ctypes.byref(a), 256, None, 256, 256, 256, None, None, None, 256, 0, None) != 0
+    assert b"workspace too small" in lib.eeggan_last_error()
