@@ -268,6 +268,7 @@ def family_chain(dev, launches):
     layer, all of the step's layer sizes -- but nothing of the other kernels of the step or of the second chain that
     shares the chip with it; unlike a profiler's per-kernel durations it is measured on the unprofiled launch path."""
     from eeggan_amd import ops
+    from eeggan_amd.graphs import capture
     cache, flips = {}, {}
 
     def flipped(w):  # the flipped view an input gradient reads: kept per weight, as the layers keep theirs
@@ -299,7 +300,7 @@ def family_chain(dev, launches):
     run()
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with capture(graph):
         run()
     for _ in range(2):
         graph.replay()

@@ -26,16 +26,22 @@ from .utils import cudize
 
 @contextlib.contextmanager
 def capture(graph):
-    """``torch.cuda.graph(graph)`` with the garbage collector out of the way.  A collection that starts while a stream
-    is capturing (on any thread: autograd's backward thread allocates Python objects too) can free device objects of
-    earlier, unrelated work -- the graphs, streams and tensors of a discarded trainer that sat in a reference cycle --
-    and the runtime calls that release them are not allowed while a capture in the default (global) mode is under
-    way: the process aborts.  So: collect first, outside the capture, and keep the collector off until it ends."""
+    """``torch.cuda.graph(graph)`` with the garbage collector out of the way, in the thread-local mode.
+
+    A collection that starts while a stream is capturing (on any thread: autograd's backward thread allocates Python
+    objects too) can free device objects of earlier, unrelated work -- the graphs, streams and tensors of a discarded
+    trainer that sat in a reference cycle -- and the runtime calls that release them are not allowed on a capturing
+    thread.  So: collect first, outside the capture, and keep the collector off until it ends.
+
+    In the default (global) mode such calls are errors on EVERY thread while a capture is under way.  A process group of
+    the nccl backend has a thread that asks for the state of its collectives' events ten times a second, and an error there
+    ends the process: a capture that begins shortly after a collective (a barrier, a bucket's sum) could meet it.  What
+    other threads do is no part of what is captured here, so the mode that leaves them alone is the right one."""
     gc.collect()
     was_enabled = gc.isenabled()
     gc.disable()
     try:
-        with torch.cuda.graph(graph):
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
             yield
     finally:
         if was_enabled:

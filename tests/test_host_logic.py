@@ -311,3 +311,21 @@ def test_eval_discriminator_plugin_logs_the_mean_score():
         U.cudize = saved
     assert asked == [(1024, False, 3, 0.5)]
     assert abs(tr.stats["memorization"]["val"] - 2.0) < 1e-6 and tr.stats["memorization"]["epoch"] == 2
+
+
+def test_captures_bind_only_their_own_thread(monkeypatch):
+    """graphs.capture takes the thread-local mode: in the global one a call of another thread (a process group's that asks
+    for its collectives' events) is an error while a capture is under way."""
+    import contextlib
+    import gc
+    from eeggan_amd import graphs
+    seen = []
+
+    @contextlib.contextmanager
+    def graph(g, **kw):
+        seen.append((g, kw, gc.isenabled()))
+        yield
+    monkeypatch.setattr(torch.cuda, "graph", graph)
+    with graphs.capture("a graph"):
+        pass
+    assert seen == [("a graph", {"capture_error_mode": "thread_local"}, False)] and gc.isenabled()

@@ -837,3 +837,47 @@ def test_flip_cache_of_a_copied_network(dev):
     (gx0,) = torch.autograd.grad(conv(x), x, gy)  # the original still answers with its own weights
     ref0 = F.conv_transpose1d(gy.double().cpu(), conv.conv.weight.detach().double().cpu(), padding=1) * conv.scale
     assert rel(gx0, ref0) < TOL
+
+
+def test_captures_beside_a_thread_that_queries_events(dev):
+    """A thread that asks for the state of events while graphs are captured, as a process group's does: no error on either
+    side, and the graphs hold what was captured."""
+    import threading
+    from eeggan_amd.graphs import capture
+    x = torch.ones(1000, device=dev)
+    y = torch.zeros(1000, device=dev)
+    y.add_(x)
+    events = [torch.cuda.Event() for _ in range(4)]
+    for e in events:
+        e.record()
+    torch.cuda.synchronize()
+    stop, asked, errors = threading.Event(), [], []
+
+    def ask():
+        try:
+            while not stop.is_set():
+                asked.append(all(e.query() for e in events))
+        except Exception as e:  # (reported below: an error here is what the mode has to avoid)
+            errors.append(e)
+    thread = threading.Thread(target=ask)
+    thread.start()
+    try:
+        graphs = []
+        for _ in range(20):
+            graph = torch.cuda.CUDAGraph()
+            before = len(asked)
+            with capture(graph):
+                y.add_(x)
+                for _ in range(1000):
+                    if len(asked) > before + 3 or errors:
+                        break
+                    stop.wait(0.001)
+            graphs.append(graph)
+    finally:
+        stop.set()
+        thread.join()
+    assert not errors and all(asked), errors
+    for graph in graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    assert bool((y == 21.0).all())
